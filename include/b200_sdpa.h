@@ -52,11 +52,15 @@ typedef enum b200_sdpa_status {
   B200_SDPA_ERR_CACHE_FULL = 12,  /* (status word only) decode with append met a
                                      sequence whose cache is full: its new row was
                                      not stored and not attended to; [1] = batch    */
-  B200_SDPA_ERR_BOUNDS = 13       /* (status word only, checked build of the library)
+  B200_SDPA_ERR_BOUNDS = 13,      /* (status word only, checked build of the library)
                                      an index left its tensor, a scratch slot its
                                      buffer or a tensor-memory access its columns;
                                      the access was skipped; [1] = site, [2] = index,
                                      [3] = limit                                    */
+  B200_SDPA_ERR_PAGE = 14         /* (status word only) a block table names a page
+                                     outside the pool, or a position lies before the
+                                     table: nothing was read or written there;
+                                     [1] = sequence, [2] = position, [3] = pages    */
 } b200_sdpa_status;
 
 typedef enum b200_sdpa_dtype {
@@ -401,11 +405,119 @@ int b200_sdpa_bwd(const B200SdpaBwdParams* params, void* stream);
 int b200_sdpa_merge(const B200SdpaMergeParams* params, void* stream);
 
 /*
+ * Rotary position embedding with one to four position axes (one time axis, or time,
+ * height and width, ...).  Pair i of the first `rot` elements of every head -- (i, i + rot/2),
+ * or (2i, 2i+1) when `interleaved` -- is turned by pos[axis(i)] * inv_freq[i]; section[a]
+ * consecutive pairs belong to axis a.  Elements behind `rot` are copied.  `inverse` turns by
+ * the opposite angle: the gradient of the same call.  x[1] (the keys) may be absent: heads[1] = 0.
+ * Angles are formed in 64 bits, the rest is computed in 32 and rounded once.
+ */
+typedef struct B200RotaryParams {
+  uint32_t struct_size;          /* sizeof(B200RotaryParams)                          */
+  int32_t dtype;                 /* b200_sdpa_dtype of x and y                        */
+  int32_t device;
+  int32_t inverse;
+  const void* x[2];              /* (B, heads[w], L, D)                               */
+  void* y[2];                    /* may not overlap x unless it is the same tensor    */
+  int64_t x_stride[2][4], y_stride[2][4];
+  int32_t heads[2];
+  int32_t B, L, D, rot;          /* rot even, 0 < rot <= D                            */
+  int32_t axes;                  /* 1 .. 4                                            */
+  int32_t interleaved;
+  int32_t section[4];            /* pairs of each axis; their sum is rot / 2          */
+  const void* positions;         /* (axes, B, L), int32 or int64                      */
+  int64_t pos_stride[3];
+  const void* inv_freq;          /* (rot / 2,), fp32 or fp64, contiguous              */
+  int32_t positions_i64;
+  int32_t inv_freq_f64;
+  int32_t* status;
+} B200RotaryParams;
+
+/* Enqueue the rotation of `x` into `y`. */
+int b200_sdpa_rotary(const B200RotaryParams* params, void* stream);
+
+/*
+ * Rows into or out of an 8-bit paged cache: e4m3 values and one power of two 2^e (its biased
+ * exponent, e8m0) for each row of D elements, the least e >= -127 with amax <= 448 * 2^e (e = 0 for
+ * a row of zeros; NaN, 255, for a row with a NaN or an infinity, which reads back as NaN).
+ * Writing: row i of sequence b (i < lens[b], or i < L without lens) goes to position
+ * start[b] + i; a position beyond the table is dropped and reported as B200_SDPA_ERR_CACHE_FULL.
+ * Reading: positions 0 .. L-1 of each sequence; rows at or behind lens[b] become zeros.
+ */
+typedef struct B200CacheRowsParams {
+  uint32_t struct_size;          /* sizeof(B200CacheRowsParams)                       */
+  int32_t dtype;                 /* f16 or bf16: the dense rows                       */
+  int32_t device;
+  int32_t page_size;             /* a power of two                                    */
+  const void* k;                 /* (B, Hkv, L, D), unit inner stride; written by the */
+  const void* v;                 /* reading call                                      */
+  int64_t k_stride[3], v_stride[3];            /* batch, head, row                    */
+  void* k_pages;                 /* e4m3 pools, 16-byte aligned rows                  */
+  void* v_pages;
+  int64_t k_pages_stride[3], v_pages_stride[3];    /* page, head, row in page         */
+  void* k_scales;                /* e8m0, one byte a row                              */
+  void* v_scales;
+  int64_t k_scales_stride[3], v_scales_stride[3];
+  int32_t B, Hkv, L, D;          /* D a multiple of 16, at most 256                   */
+  const int32_t* block_table;    /* (B, block_table_stride)                           */
+  int32_t block_table_stride;
+  int32_t n_pages;               /* pages of the pools                                */
+  const int32_t* start;          /* (B,), writing only                                */
+  const int32_t* lens;           /* (B,); optional when writing                       */
+  int32_t* status;
+} B200CacheRowsParams;
+
+int b200_sdpa_cache_write(const B200CacheRowsParams* params, void* stream);
+int b200_sdpa_cache_read(const B200CacheRowsParams* params, void* stream);
+
+/*
+ * One query row per sequence against a paged cache, 8-bit (k_scales and v_scales set) or of the
+ * query's 16-bit dtype, with an optional prefix that all sequences share: `prefix_len` keys in the
+ * pages of `prefix_table` come before every sequence's own kv_lens[b] keys and are read and multiplied
+ * once for the whole batch.  Without a prefix only the 8-bit cache is served here
+ * (b200_sdpa_decode serves the other).  D is 64 or 128, unit inner strides, 16-byte aligned rows.
+ */
+typedef struct B200CacheDecodeParams {
+  uint32_t struct_size;          /* sizeof(B200CacheDecodeParams)                     */
+  int32_t dtype;                 /* f16 or bf16: q and out                            */
+  int32_t device;
+  int32_t page_size;             /* a power of two                                    */
+  const void* q;                 /* (B, Hq, 1, D): strides of batch, head, element    */
+  void* out;
+  float* lse;                    /* optional (B, Hq)                                  */
+  int64_t q_stride[3], out_stride[3], lse_stride[2];
+  const void* k_pages;
+  const void* v_pages;
+  int64_t k_pages_stride[3], v_pages_stride[3];    /* page, head, row in page         */
+  const void* k_scales;          /* NULL: the pools hold the query's dtype            */
+  const void* v_scales;
+  int64_t k_scales_stride[3], v_scales_stride[3];
+  int32_t B, Hq, Hkv, D;
+  float scale;                   /* positive                                          */
+  int32_t n_pages;
+  const int32_t* block_table;    /* (B, block_table_stride); may have no column       */
+  const int32_t* kv_lens;        /* (B,): keys of the sequence's own                  */
+  int32_t block_table_stride;
+  int32_t prefix_len;            /* 0: no prefix                                      */
+  const int32_t* prefix_table;   /* ceil(prefix_len / page_size) pages                */
+  int32_t kv_chunk;              /* keys of one CTA over the own part; 0: chosen      */
+  int32_t reserved;
+  void* workspace;               /* as the plan says, on 16 bytes                     */
+  uint64_t workspace_bytes;
+  int32_t* status;
+} B200CacheDecodeParams;
+
+/* Fills launches, kv_splits (of the own part), block_n (keys of one split), workspace_bytes. */
+int b200_sdpa_cache_decode_plan(const B200CacheDecodeParams* params, B200SdpaPlan* plan);
+int b200_sdpa_cache_decode(const B200CacheDecodeParams* params, void* stream);
+
+/*
  * Launch counters, one per kernel family, so a caller can prove which kernel ran.
  * Upstream counterpart: executed-op tracking
  *   torch_neuronx/__init__.py:528-546, tests/utils/neuron_test_utils.py:18-135.
  * kernel ids: 0 generic, 1 prefill, 2 decode partial, 3 decode combine, 4 merge,
- * 5 backward grad_q, 6 backward grad_k/grad_v, 7 backward row statistics.
+ * 5 backward grad_q, 6 backward grad_k/grad_v, 7 backward row statistics, 8 rotary,
+ * 9 cache write, 10 cache read.
  */
 uint64_t b200_sdpa_launch_count(int kernel_id);
 void b200_sdpa_reset_launch_counts(void);

@@ -28,6 +28,7 @@ from .ops import (
     sdpa_forward,
     sdpa_forward_accumulate,
 )
+from .cache import paged_read, paged_write, shared_prefix_decode
 from .masks import MaskStructure, classify_mask
 from .ring import (
     ring_attention,
@@ -37,6 +38,7 @@ from .ring import (
     shard_sequence,
     unshard_sequence,
 )
+from .rotary import rotary_embedding
 from .sharding import as_units, from_units, local_units, partition_units
 
 register_aten_override()
@@ -47,8 +49,8 @@ reset_launch_counts = _lib.reset_launch_counts
 __all__ = [
     "MaskStructure", "alloc_like_query", "as_units", "check_device_status", "classify_mask", "decode_append", "enable_sdpa_routing",
     "from_units", "fused_attention_overrideable", "fused_attention_overrideable_backward", "launch_counts",
-    "local_units", "merge_partials", "native_multi_head_attn_mid", "paged_decode", "partition_units", "register_aten_override", "reset_launch_counts",
-    "ring_attention", "ring_attention_backward", "ring_attention_backward_virtual", "ring_attention_virtual", "scaled_dot_product_attention",
+    "local_units", "merge_partials", "native_multi_head_attn_mid", "paged_decode", "paged_read", "paged_write", "partition_units", "register_aten_override", "reset_launch_counts",
+    "ring_attention", "ring_attention_backward", "ring_attention_backward_virtual", "ring_attention_virtual", "rotary_embedding", "scaled_dot_product_attention",
     "scaled_dot_product_attention_backward_kernel", "scaled_dot_product_attention_kernel", "sdpa_backward",
-    "sdpa_forward", "sdpa_forward_accumulate", "set_mask_recognition", "shard_sequence", "unshard_sequence",
+    "sdpa_forward", "sdpa_forward_accumulate", "set_mask_recognition", "shard_sequence", "shared_prefix_decode", "unshard_sequence",
 ]

@@ -33,7 +33,7 @@ STATIC_SCRATCH_BYTES = 16 << 20  # B200_SDPA_STATIC_SCRATCH_BYTES
 # b200_sdpa_status
 OK = 0
 ERR_NULL, ERR_STRUCT, ERR_DTYPE, ERR_SHAPE, ERR_UNSUPPORTED = 1, 2, 3, 4, 5
-ERR_WORKSPACE, ERR_ALIGNMENT, ERR_CUDA, ERR_DEVICE, ERR_TIMEOUT, ERR_TOO_LARGE, ERR_CACHE_FULL, ERR_BOUNDS = 6, 7, 8, 9, 10, 11, 12, 13
+ERR_WORKSPACE, ERR_ALIGNMENT, ERR_CUDA, ERR_DEVICE, ERR_TIMEOUT, ERR_TOO_LARGE, ERR_CACHE_FULL, ERR_BOUNDS, ERR_PAGE = 6, 7, 8, 9, 10, 11, 12, 13, 14
 
 # b200_sdpa_dtype
 F32, F16, BF16 = 0, 1, 2
@@ -43,8 +43,9 @@ PATH_AUTO, PATH_GENERIC, PATH_PREFILL, PATH_DECODE = 0, 1, 2, 3
 PATH_NAMES = {PATH_AUTO: "auto", PATH_GENERIC: "generic", PATH_PREFILL: "prefill", PATH_DECODE: "decode"}
 
 # launch-counter ids
-KID_GENERIC, KID_PREFILL, KID_DECODE, KID_COMBINE, KID_MERGE, KID_BWD_DQ, KID_BWD_DKV, KID_BWD_PREP = range(8)
-KERNEL_NAMES = ("generic", "prefill", "decode_partial", "decode_combine", "merge", "bwd_dq", "bwd_dkv", "bwd_prep")
+KID_GENERIC, KID_PREFILL, KID_DECODE, KID_COMBINE, KID_MERGE, KID_BWD_DQ, KID_BWD_DKV, KID_BWD_PREP, KID_ROTARY, KID_CACHE_WRITE, KID_CACHE_READ = range(11)
+KERNEL_NAMES = ("generic", "prefill", "decode_partial", "decode_combine", "merge", "bwd_dq", "bwd_dkv", "bwd_prep",
+                "rotary", "cache_write", "cache_read")
 
 
 class Params(C.Structure):
@@ -198,6 +199,109 @@ class BwdParams(C.Structure):
     ]
 
 
+class RotaryParams(C.Structure):
+    """Mirror of ``B200RotaryParams``."""
+
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("dtype", C.c_int32),
+        ("device", C.c_int32),
+        ("inverse", C.c_int32),
+        ("x", C.c_void_p * 2),
+        ("y", C.c_void_p * 2),
+        ("x_stride", (C.c_int64 * 4) * 2),
+        ("y_stride", (C.c_int64 * 4) * 2),
+        ("heads", C.c_int32 * 2),
+        ("B", C.c_int32),
+        ("L", C.c_int32),
+        ("D", C.c_int32),
+        ("rot", C.c_int32),
+        ("axes", C.c_int32),
+        ("interleaved", C.c_int32),
+        ("section", C.c_int32 * 4),
+        ("positions", C.c_void_p),
+        ("pos_stride", C.c_int64 * 3),
+        ("inv_freq", C.c_void_p),
+        ("positions_i64", C.c_int32),
+        ("inv_freq_f64", C.c_int32),
+        ("status", C.c_void_p),
+    ]
+
+
+class CacheRowsParams(C.Structure):
+    """Mirror of ``B200CacheRowsParams``."""
+
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("dtype", C.c_int32),
+        ("device", C.c_int32),
+        ("page_size", C.c_int32),
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("k_stride", C.c_int64 * 3),
+        ("v_stride", C.c_int64 * 3),
+        ("k_pages", C.c_void_p),
+        ("v_pages", C.c_void_p),
+        ("k_pages_stride", C.c_int64 * 3),
+        ("v_pages_stride", C.c_int64 * 3),
+        ("k_scales", C.c_void_p),
+        ("v_scales", C.c_void_p),
+        ("k_scales_stride", C.c_int64 * 3),
+        ("v_scales_stride", C.c_int64 * 3),
+        ("B", C.c_int32),
+        ("Hkv", C.c_int32),
+        ("L", C.c_int32),
+        ("D", C.c_int32),
+        ("block_table", C.c_void_p),
+        ("block_table_stride", C.c_int32),
+        ("n_pages", C.c_int32),
+        ("start", C.c_void_p),
+        ("lens", C.c_void_p),
+        ("status", C.c_void_p),
+    ]
+
+
+class CacheDecodeParams(C.Structure):
+    """Mirror of ``B200CacheDecodeParams``."""
+
+    _fields_ = [
+        ("struct_size", C.c_uint32),
+        ("dtype", C.c_int32),
+        ("device", C.c_int32),
+        ("page_size", C.c_int32),
+        ("q", C.c_void_p),
+        ("out", C.c_void_p),
+        ("lse", C.c_void_p),
+        ("q_stride", C.c_int64 * 3),
+        ("out_stride", C.c_int64 * 3),
+        ("lse_stride", C.c_int64 * 2),
+        ("k_pages", C.c_void_p),
+        ("v_pages", C.c_void_p),
+        ("k_pages_stride", C.c_int64 * 3),
+        ("v_pages_stride", C.c_int64 * 3),
+        ("k_scales", C.c_void_p),
+        ("v_scales", C.c_void_p),
+        ("k_scales_stride", C.c_int64 * 3),
+        ("v_scales_stride", C.c_int64 * 3),
+        ("B", C.c_int32),
+        ("Hq", C.c_int32),
+        ("Hkv", C.c_int32),
+        ("D", C.c_int32),
+        ("scale", C.c_float),
+        ("n_pages", C.c_int32),
+        ("block_table", C.c_void_p),
+        ("kv_lens", C.c_void_p),
+        ("block_table_stride", C.c_int32),
+        ("prefix_len", C.c_int32),
+        ("prefix_table", C.c_void_p),
+        ("kv_chunk", C.c_int32),
+        ("reserved", C.c_int32),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_uint64),
+        ("status", C.c_void_p),
+    ]
+
+
 # Every symbol include/b200_sdpa.h declares: name -> (restype, argtypes)
 EXPORTS = {
     "b200_sdpa_abi_version": (C.c_int, []),
@@ -209,6 +313,11 @@ EXPORTS = {
     "b200_sdpa_bwd_query_plan": (C.c_int, [C.POINTER(BwdParams), C.POINTER(Plan)]),
     "b200_sdpa_bwd": (C.c_int, [C.POINTER(BwdParams), C.c_void_p]),
     "b200_sdpa_merge": (C.c_int, [C.POINTER(MergeParams), C.c_void_p]),
+    "b200_sdpa_rotary": (C.c_int, [C.POINTER(RotaryParams), C.c_void_p]),
+    "b200_sdpa_cache_write": (C.c_int, [C.POINTER(CacheRowsParams), C.c_void_p]),
+    "b200_sdpa_cache_read": (C.c_int, [C.POINTER(CacheRowsParams), C.c_void_p]),
+    "b200_sdpa_cache_decode_plan": (C.c_int, [C.POINTER(CacheDecodeParams), C.POINTER(Plan)]),
+    "b200_sdpa_cache_decode": (C.c_int, [C.POINTER(CacheDecodeParams), C.c_void_p]),
     "b200_sdpa_launch_count": (C.c_uint64, [C.c_int]),
     "b200_sdpa_reset_launch_counts": (None, []),
     "b200_sdpa_checked_build": (C.c_int, []),

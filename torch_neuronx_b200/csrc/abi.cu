@@ -300,6 +300,72 @@ int choose_bwd(const B200SdpaBwdParams* a, const BwdProblem& bp, int* path) {
   return B200_SDPA_OK;
 }
 
+bool half_dtype(int dtype) { return dtype == B200_SDPA_F16 || dtype == B200_SDPA_BF16; }
+bool page_size_ok(int n) { return n >= 1 && (n & (n - 1)) == 0; }
+
+int validate_rotary(const B200RotaryParams* a) {
+  if (a == nullptr) return B200_SDPA_ERR_NULL;
+  if (a->struct_size != sizeof(B200RotaryParams)) return B200_SDPA_ERR_STRUCT;
+  if (a->dtype != B200_SDPA_F32 && !half_dtype(a->dtype)) return B200_SDPA_ERR_DTYPE;
+  if (a->B <= 0 || a->L <= 0 || a->D <= 0 || a->heads[0] <= 0 || a->heads[1] < 0 || a->rot <= 0 || a->rot > a->D || a->rot % 2 != 0)
+    return B200_SDPA_ERR_SHAPE;
+  if (a->axes < 1 || a->axes > 4) return B200_SDPA_ERR_SHAPE;
+  int64_t pairs = 0;
+  for (int i = 0; i < a->axes; ++i) {
+    if (a->section[i] < 0) return B200_SDPA_ERR_SHAPE;
+    pairs += a->section[i];
+  }
+  if (pairs != a->rot / 2) return B200_SDPA_ERR_SHAPE;
+  // the grid's second dimension, and the shared-memory table of four tokens
+  if (a->B > 65535 || a->rot > 1024 || static_cast<int64_t>(a->heads[0]) + a->heads[1] > (1 << 16)) return B200_SDPA_ERR_UNSUPPORTED;
+  for (int w = 0; w < 2; ++w)
+    if (a->heads[w] > 0 && (a->x[w] == nullptr || a->y[w] == nullptr)) return B200_SDPA_ERR_NULL;
+  if (a->positions == nullptr || a->inv_freq == nullptr) return B200_SDPA_ERR_NULL;
+  return B200_SDPA_OK;
+}
+
+// Rows of a pool: bases on 16 bytes, strides in whole 16-byte pieces.
+bool pool_aligned(const void* base, const int64_t* stride, int esize) {
+  if (reinterpret_cast<uintptr_t>(base) % 16) return false;
+  for (int i = 0; i < 3; ++i)
+    if (stride[i] < 0 || (stride[i] * esize) % 16) return false;
+  return true;
+}
+
+int validate_rows(const B200CacheRowsParams* a) {
+  if (a == nullptr) return B200_SDPA_ERR_NULL;
+  if (a->struct_size != sizeof(B200CacheRowsParams)) return B200_SDPA_ERR_STRUCT;
+  if (!half_dtype(a->dtype)) return B200_SDPA_ERR_DTYPE;
+  if (a->B <= 0 || a->Hkv <= 0 || a->L <= 0 || a->D <= 0 || a->n_pages <= 0) return B200_SDPA_ERR_SHAPE;
+  if (!page_size_ok(a->page_size) || a->block_table_stride < 1) return B200_SDPA_ERR_SHAPE;
+  if (a->D % 16 != 0 || a->D > 256 || a->B > 65535 || a->Hkv > (1 << 16)) return B200_SDPA_ERR_UNSUPPORTED;
+  if (static_cast<int64_t>(a->block_table_stride) * a->page_size > 0x7fffffff) return B200_SDPA_ERR_UNSUPPORTED;
+  if (a->k == nullptr || a->v == nullptr || a->k_pages == nullptr || a->v_pages == nullptr || a->k_scales == nullptr ||
+      a->v_scales == nullptr || a->block_table == nullptr)
+    return B200_SDPA_ERR_NULL;
+  if (!pool_aligned(a->k_pages, a->k_pages_stride, 1) || !pool_aligned(a->v_pages, a->v_pages_stride, 1)) return B200_SDPA_ERR_ALIGNMENT;
+  return B200_SDPA_OK;
+}
+
+int validate_cache_decode(const B200CacheDecodeParams* a) {
+  if (a == nullptr) return B200_SDPA_ERR_NULL;
+  if (a->struct_size != sizeof(B200CacheDecodeParams)) return B200_SDPA_ERR_STRUCT;
+  if (!half_dtype(a->dtype)) return B200_SDPA_ERR_DTYPE;
+  if (a->B <= 0 || a->Hq <= 0 || a->Hkv <= 0 || a->Hq % a->Hkv != 0 || a->n_pages <= 0) return B200_SDPA_ERR_SHAPE;
+  if (!page_size_ok(a->page_size) || a->block_table_stride < 0 || a->prefix_len < 0) return B200_SDPA_ERR_SHAPE;
+  if ((a->D != 64 && a->D != 128) || a->B > 65535) return B200_SDPA_ERR_UNSUPPORTED;
+  if (!(a->scale > 0.f) || !(a->scale < 1e30f)) return B200_SDPA_ERR_UNSUPPORTED;
+  if (static_cast<int64_t>(a->block_table_stride) * a->page_size > 0x7fffffff) return B200_SDPA_ERR_UNSUPPORTED;
+  if (a->q == nullptr || a->out == nullptr || a->k_pages == nullptr || a->v_pages == nullptr || a->kv_lens == nullptr) return B200_SDPA_ERR_NULL;
+  if ((a->k_scales == nullptr) != (a->v_scales == nullptr)) return B200_SDPA_ERR_NULL;
+  if (a->block_table == nullptr && a->block_table_stride > 0) return B200_SDPA_ERR_NULL;
+  if (a->prefix_len > 0 && a->prefix_table == nullptr) return B200_SDPA_ERR_NULL;
+  const int esize = a->k_scales != nullptr ? 1 : 2;
+  if (!pool_aligned(a->k_pages, a->k_pages_stride, esize) || !pool_aligned(a->v_pages, a->v_pages_stride, esize))
+    return B200_SDPA_ERR_ALIGNMENT;
+  return cache_decode_served(*a);
+}
+
 }  // namespace
 
 void count_launch(int kernel_id) {
@@ -338,7 +404,8 @@ const char* b200_sdpa_strerror(int status) {
     case B200_SDPA_ERR_BOUNDS: return "checked build: an index, scratch slot or tensor-memory column left its range (access skipped)";
     case B200_SDPA_ERR_TIMEOUT: return "a device-side wait gave up (kernel drained and returned)";
     case B200_SDPA_ERR_TOO_LARGE: return "request exceeds the fixed capacity of this entry point";
-    case B200_SDPA_ERR_CACHE_FULL: return "decode with append: a sequence's cache is full, its new row was dropped";
+    case B200_SDPA_ERR_CACHE_FULL: return "a sequence's cache is full: a new row was dropped";
+    case B200_SDPA_ERR_PAGE: return "a block table names a page outside the pool";
     default: return "unknown status";
   }
 }
@@ -484,6 +551,47 @@ int b200_sdpa_merge(const B200SdpaMergeParams* m, void* stream) {
   DeviceScope scope(m->device);
   if (scope.status() != B200_SDPA_OK) return scope.status();
   return launch_merge(*m, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int b200_sdpa_rotary(const B200RotaryParams* a, void* stream) {
+  const int rc = validate_rotary(a);
+  if (rc != B200_SDPA_OK) return rc;
+  DeviceScope scope(a->device);
+  if (scope.status() != B200_SDPA_OK) return scope.status();
+  return launch_rotary(*a, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int b200_sdpa_cache_write(const B200CacheRowsParams* a, void* stream) {
+  int rc = validate_rows(a);
+  if (rc != B200_SDPA_OK) return rc;
+  if (a->start == nullptr) return B200_SDPA_ERR_NULL;
+  DeviceScope scope(a->device);
+  if (scope.status() != B200_SDPA_OK) return scope.status();
+  return launch_cache_write(*a, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int b200_sdpa_cache_read(const B200CacheRowsParams* a, void* stream) {
+  int rc = validate_rows(a);
+  if (rc != B200_SDPA_OK) return rc;
+  if (a->lens == nullptr) return B200_SDPA_ERR_NULL;
+  DeviceScope scope(a->device);
+  if (scope.status() != B200_SDPA_OK) return scope.status();
+  return launch_cache_read(*a, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int b200_sdpa_cache_decode_plan(const B200CacheDecodeParams* a, B200SdpaPlan* plan) {
+  if (plan == nullptr) return B200_SDPA_ERR_NULL;
+  if (plan->struct_size != sizeof(B200SdpaPlan)) return B200_SDPA_ERR_STRUCT;
+  const int rc = validate_cache_decode(a);
+  return rc != B200_SDPA_OK ? rc : plan_cache_decode(*a, plan);
+}
+
+int b200_sdpa_cache_decode(const B200CacheDecodeParams* a, void* stream) {
+  const int rc = validate_cache_decode(a);
+  if (rc != B200_SDPA_OK) return rc;
+  DeviceScope scope(a->device);
+  if (scope.status() != B200_SDPA_OK) return scope.status();
+  return launch_cache_decode(*a, reinterpret_cast<cudaStream_t>(stream));
 }
 
 uint64_t b200_sdpa_launch_count(int kernel_id) {

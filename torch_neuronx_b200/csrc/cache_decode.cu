@@ -1,0 +1,303 @@
+// One query row per sequence against a paged cache: the 8-bit cache, and a prefix that the whole batch shares.
+//
+// With a shared prefix of P keys the softmax runs over P + kv_lens[b] keys, but only the sequence's own keys differ:
+//   * prefix: the batch's query rows are the rows of one attention problem (B * group rows for each kv head against P
+//     keys, no mask), so its keys are read once for all of them and multiplied by full tensor-core tiles -- the split form
+//     of the prefill kernel (prefill_sm100.cu), whose fp32 partials stay in the scratch;
+//   * own keys: split-KV decode (decode_mma.cu, decode_fp8.cu), partials beside them;
+//   * one merge over both lists, exact in the usual way: o = sum 2^(m_i - m) o_i / sum 2^(m_i - m) l_i.
+// Bound by HBM: (P + sum of own lengths) Hkv rows once; the prefix's products by the tensor cores from about 60 sequences
+// on (32 / 8 heads).
+#include "common.cuh"
+#include "debug.cuh"
+
+namespace b200 {
+
+// cache_rows.cu: rows [0, n) of the table's pages, dense in the rows' dtype (scales null: a copy of 16-bit rows)
+int launch_cache_gather(const B200CacheRowsParams& p, cudaStream_t stream);
+
+namespace {
+
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kCombineWarps = 4;
+
+struct Partials {
+  const float* o;    // [row][n][D]
+  const float* ml;   // [row][n][2]
+  int n;
+};
+
+// One CTA per (sequence, query head): the prefix's partials (row h * B + b) and the own ones in use (row b * Hq + h).
+template <typename T, int D>
+__global__ void __launch_bounds__(kCombineWarps * 32)
+    cache_combine_kernel(const Problem p, const int chunk, const Partials own, const Partials prefix) {
+  constexpr int C = D / 32;   // columns per lane
+  __shared__ float sm_o[kCombineWarps][D];
+  __shared__ float sm_l[kCombineWarps];
+  const int h = blockIdx.x % p.Hq, b = blockIdx.x / p.Hq;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_wait();
+  pdl_launch_dependents();
+  int used = 0;
+  if (own.n > 0) {
+    used = (valid_keys(p, b) + chunk - 1) / chunk;
+    used = used < 1 ? 1 : (used > own.n ? own.n : used);
+  }
+  const int64_t own0 = (static_cast<int64_t>(b) * p.Hq + h) * own.n, pre0 = (static_cast<int64_t>(h) * p.B + b) * prefix.n;
+  if (!dbg_range(p.status, DBG_CACHE_DECODE * 100 + 1, own0, used, static_cast<int64_t>(p.B) * p.Hq * own.n) ||
+      !dbg_bhrc(p.status, DBG_CACHE_DECODE * 100 + 2, b, p.B, h, p.Hq, 0, 1, lane * C, C, p.Dv))
+    return;
+  const int total = prefix.n + used;
+  auto pair_of = [&](int s) {
+    return *reinterpret_cast<const float2*>(s < prefix.n ? prefix.ml + (pre0 + s) * 2 : own.ml + (own0 + s - prefix.n) * 2);
+  };
+  float mx = -CUDART_INF_F;
+  for (int s = lane; s < total; s += 32) mx = fmaxf(mx, pair_of(s).x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  const float ms = (mx == -CUDART_INF_F) ? 0.f : mx;
+  float acc[C], lsum = 0.f;
+#pragma unroll
+  for (int c = 0; c < C; ++c) acc[c] = 0.f;
+#pragma unroll 4
+  for (int s = warp; s < total; s += kCombineWarps) {
+    const float2 ml = pair_of(s);
+    // a range without a visible key has the sum 0, and the prefix kernel wrote nothing else for it (a NaN sum counts)
+    if (ml.y == 0.f) continue;
+    const float* src = (s < prefix.n ? prefix.o + (pre0 + s) * D : own.o + (own0 + s - prefix.n) * D) + lane * C;
+    float v[C];
+    if constexpr (C == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src);
+    else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(src);
+    const float w = exp2f(ml.x - ms);
+    lsum = fmaf(ml.y, w, lsum);
+#pragma unroll
+    for (int c = 0; c < C; ++c) acc[c] = fmaf(v[c], w, acc[c]);
+  }
+#pragma unroll
+  for (int c = 0; c < C; ++c) sm_o[warp][lane * C + c] = acc[c];
+  if (lane == 0) sm_l[warp] = lsum;
+  __syncthreads();
+  float l = 0.f;
+#pragma unroll
+  for (int w = 0; w < kCombineWarps; ++w) l += sm_l[w];
+  const float inv = l != 0.f ? 1.f / l : 0.f;
+  for (int d = threadIdx.x; d < D; d += kCombineWarps * 32) {
+    float o = 0.f;
+#pragma unroll
+    for (int w = 0; w < kCombineWarps; ++w) o += sm_o[w][d];
+    reinterpret_cast<T*>(p.out)[b * p.os[0] + h * p.os[1] + d * p.os[3]] = from_f32<T>(o * inv);
+  }
+  if (p.lse != nullptr && threadIdx.x == 0)
+    p.lse[b * p.ls[0] + h * p.ls[1]] = l == 0.f ? -CUDART_INF_F : fmaf(mx, kLn2, logf(l));
+}
+
+struct Geometry {
+  int chunk, nsplit;          // own keys; nsplit = 0: no table
+  PackGeom pack;              // prefix
+  uint64_t own_bytes, prefix_bytes, dense_bytes;
+  uint64_t total() const { return own_bytes + prefix_bytes + dense_bytes; }
+};
+
+uint64_t aligned(uint64_t n) { return (n + 255) / 256 * 256; }
+
+Problem own_problem(const B200CacheDecodeParams& a) {
+  Problem p = {};
+  p.q = a.q;
+  p.k = a.k_pages;
+  p.v = a.v_pages;
+  p.out = a.out;
+  p.lse = a.lse;
+  const int64_t qs[4] = {a.q_stride[0], a.q_stride[1], 0, a.q_stride[2]}, os[4] = {a.out_stride[0], a.out_stride[1], 0, a.out_stride[2]};
+  for (int i = 0; i < 4; ++i) {
+    p.qs[i] = qs[i];
+    p.os[i] = os[i];
+    p.ks[i] = i < 3 ? a.k_pages_stride[i] : 1;
+    p.vs[i] = i < 3 ? a.v_pages_stride[i] : 1;
+  }
+  p.ls[0] = a.lse_stride[0];
+  p.ls[1] = a.lse_stride[1];
+  p.B = a.B;
+  p.Hq = a.Hq;
+  p.Hkv = a.Hkv;
+  p.L = 1;
+  p.S = a.block_table_stride * a.page_size;
+  p.E = p.Dv = a.D;
+  p.group = a.Hq / a.Hkv;
+  p.scale = a.scale;
+  p.kv_lens = a.kv_lens;
+  p.status = a.status;
+  p.block_table = a.block_table;
+  p.table_stride = a.block_table_stride;
+  while ((1 << p.page_shift) < a.page_size) ++p.page_shift;
+  return p;
+}
+
+// The batch's rows against the prefix, dense rows at `k` and `v` ((Hkv, P, D)).
+Problem prefix_problem(const B200CacheDecodeParams& a, const void* k, const void* v) {
+  Problem p = own_problem(a);
+  p.k = k;
+  p.v = v;
+  p.out = nullptr;
+  p.lse = nullptr;
+  const int64_t kv[4] = {static_cast<int64_t>(a.Hkv) * a.prefix_len * a.D, static_cast<int64_t>(a.prefix_len) * a.D, a.D, 1};
+  for (int i = 0; i < 4; ++i) p.ks[i] = p.vs[i] = kv[i];
+  p.qs[0] = static_cast<int64_t>(a.B) * a.q_stride[0];
+  p.qs[2] = a.q_stride[0];
+  p.L = a.B;
+  p.B = 1;
+  p.S = a.prefix_len;
+  p.kv_lens = nullptr;
+  p.block_table = nullptr;
+  return p;
+}
+
+// Keys of one CTA: enough CTAs for every slot of the GPU, ranges long enough to pay for a CTA's start and end.
+int default_chunk(const Problem& p) {
+  const int heads = p.group <= 8 ? 8 : 16;
+  const int64_t units = static_cast<int64_t>(p.B) * p.Hkv * ((p.group + heads - 1) / heads);
+  const int64_t slots = heads == 8 ? 444 : 296;
+  int best = 256;
+  double best_us = 1e30;
+  for (int chunk = 64; chunk <= 4096; chunk += chunk < 512 ? 64 : 256) {
+    const int n = (p.S + chunk - 1) / chunk;
+    const double fill = static_cast<double>(units) * n / slots;
+    const double rounds = fill < 1.0 ? 1.0 : fill + 0.35;
+    const double us = rounds * (3.5 + chunk / 64.0 * (0.5 + 0.8 * (fill < 1.0 ? fill : 1.0))) * (1.0 + 0.002 * n);
+    if (us < best_us) {
+      best_us = us;
+      best = chunk;
+    }
+    if (chunk >= p.S) break;
+  }
+  return best;
+}
+
+}  // namespace
+
+int cache_decode_served(const B200CacheDecodeParams& a) {
+  if (static_cast<int64_t>(a.B) * a.Hq > 0x7fffffffLL) return B200_SDPA_ERR_UNSUPPORTED;
+  if (a.prefix_len == 0) return a.k_scales != nullptr ? B200_SDPA_OK : B200_SDPA_ERR_UNSUPPORTED;
+  const Problem f = prefix_problem(a, reinterpret_cast<void*>(256), reinterpret_cast<void*>(256));
+  if (f.group > 128) return B200_SDPA_ERR_UNSUPPORTED;
+  return prefix_eligible(f, a.dtype) ? B200_SDPA_OK : B200_SDPA_ERR_ALIGNMENT;
+}
+
+namespace {
+
+int geometry(const B200CacheDecodeParams& a, Geometry* g) {
+  const int rc = cache_decode_served(a);
+  if (rc != B200_SDPA_OK) return rc;
+  const Problem p = own_problem(a);
+  *g = {};
+  const int64_t rows = static_cast<int64_t>(a.B) * a.Hq;
+  if (p.S > 0) {
+    g->chunk = a.kv_chunk > 0 ? (a.kv_chunk + 31) / 32 * 32 : default_chunk(p);
+    g->nsplit = (p.S + g->chunk - 1) / g->chunk;
+    if (g->nsplit > 65535 || static_cast<int64_t>(p.Hkv) * ((p.group + 7) / 8) > 65535) return B200_SDPA_ERR_UNSUPPORTED;
+    g->own_bytes = aligned(static_cast<uint64_t>(rows) * g->nsplit * (a.D + 2) * sizeof(float));
+  }
+  if (a.prefix_len > 0) {
+    const Problem f = prefix_problem(a, reinterpret_cast<void*>(256), reinterpret_cast<void*>(256));
+    prefix_geometry(f, &g->pack);
+    g->prefix_bytes = aligned(g->pack.ws_bytes);
+    g->dense_bytes = 2 * aligned(static_cast<uint64_t>(a.Hkv) * a.prefix_len * a.D * 2);
+  }
+  return B200_SDPA_OK;
+}
+
+template <typename T>
+int launch_combine(const Problem& p, int chunk, const Partials& own, const Partials& prefix, cudaStream_t stream) {
+  auto kern = p.E == 128 ? cache_combine_kernel<T, 128> : cache_combine_kernel<T, 64>;
+  if (!launch_pdl(kern, dim3(p.B * p.Hq), kCombineWarps * 32, 0, stream, p, chunk, own, prefix)) return B200_SDPA_ERR_CUDA;
+  count_launch(KID_COMBINE);
+  return B200_SDPA_OK;
+}
+
+}  // namespace
+
+int plan_cache_decode(const B200CacheDecodeParams& a, B200SdpaPlan* plan) {
+  Geometry g;
+  const int rc = geometry(a, &g);
+  if (rc != B200_SDPA_OK) return rc;
+  const int heads = a.Hq / a.Hkv <= 8 && a.k_scales != nullptr ? 8 : 16;
+  plan->path = B200_SDPA_PATH_DECODE;
+  plan->block_m = 1;
+  plan->block_n = g.chunk;
+  plan->grid_x = a.Hkv * ((a.Hq / a.Hkv + heads - 1) / heads);
+  plan->grid_y = a.B;
+  plan->grid_z = g.nsplit;
+  plan->threads = 128;
+  plan->smem_bytes = 0;
+  plan->kv_splits = g.nsplit;
+  plan->launches = 1 + (g.nsplit > 0 ? 1 : 0) + (a.prefix_len > 0 ? 2 : 0);
+  plan->workspace_bytes = g.total();
+  return B200_SDPA_OK;
+}
+
+int launch_cache_decode(const B200CacheDecodeParams& a, cudaStream_t stream) {
+  Geometry g;
+  int rc = geometry(a, &g);
+  if (rc != B200_SDPA_OK) return rc;
+  if (g.total() > 0 && (a.workspace == nullptr || a.workspace_bytes < g.total() || reinterpret_cast<uintptr_t>(a.workspace) % 16))
+    return B200_SDPA_ERR_WORKSPACE;
+  const Problem p = own_problem(a);
+  const int64_t rows = static_cast<int64_t>(a.B) * a.Hq;
+  char* ws = static_cast<char*>(a.workspace);
+  float* own_o = reinterpret_cast<float*>(ws);
+  float* own_ml = own_o + rows * g.nsplit * a.D;
+  float* pre_o = reinterpret_cast<float*>(ws + g.own_bytes);
+  float* pre_ml = pre_o + rows * g.pack.n_split * a.D;
+  if (a.prefix_len > 0) {
+    char* dense = ws + g.own_bytes + g.prefix_bytes;
+    B200CacheRowsParams r = {};
+    r.dtype = a.dtype;
+    r.page_size = a.page_size;
+    r.k = dense;
+    r.v = dense + g.dense_bytes / 2;
+    r.k_pages = const_cast<void*>(a.k_pages);
+    r.v_pages = const_cast<void*>(a.v_pages);
+    r.k_scales = const_cast<void*>(a.k_scales);
+    r.v_scales = const_cast<void*>(a.v_scales);
+    for (int i = 0; i < 3; ++i) {
+      r.k_pages_stride[i] = a.k_pages_stride[i];
+      r.v_pages_stride[i] = a.v_pages_stride[i];
+      r.k_scales_stride[i] = a.k_scales_stride[i];
+      r.v_scales_stride[i] = a.v_scales_stride[i];
+    }
+    r.k_stride[1] = r.v_stride[1] = static_cast<int64_t>(a.prefix_len) * a.D;
+    r.k_stride[2] = r.v_stride[2] = a.D;
+    r.B = 1;
+    r.Hkv = a.Hkv;
+    r.L = a.prefix_len;
+    r.D = a.D;
+    r.block_table = a.prefix_table;
+    r.block_table_stride = (a.prefix_len + a.page_size - 1) / a.page_size;
+    r.n_pages = a.n_pages;
+    r.status = a.status;
+    rc = launch_cache_gather(r, stream);
+    if (rc != B200_SDPA_OK) return rc;
+    rc = launch_prefix_partial(prefix_problem(a, r.k, r.v), a.dtype, g.pack, pre_o, pre_ml, stream);
+    if (rc != B200_SDPA_OK) return rc;
+  }
+  if (g.nsplit > 0) {
+    if (a.k_scales != nullptr) {
+      CacheScales sc = {};
+      sc.k = static_cast<const uint8_t*>(a.k_scales);
+      sc.v = static_cast<const uint8_t*>(a.v_scales);
+      for (int i = 0; i < 3; ++i) {
+        sc.ks[i] = a.k_scales_stride[i];
+        sc.vs[i] = a.v_scales_stride[i];
+      }
+      sc.n_pages = a.n_pages;
+      rc = launch_decode_partial_fp8(p, sc, a.dtype, g.chunk, g.nsplit, own_o, own_ml, stream);
+    } else {
+      rc = launch_decode_partial_mma(p, a.dtype, g.chunk, g.nsplit, own_o, own_ml, stream);
+    }
+    if (rc != B200_SDPA_OK) return rc;
+  }
+  const Partials own = {own_o, own_ml, g.nsplit}, prefix = {pre_o, pre_ml, g.pack.n_split};
+  return a.dtype == B200_SDPA_BF16 ? launch_combine<__nv_bfloat16>(p, g.chunk, own, prefix, stream)
+                                   : launch_combine<__half>(p, g.chunk, own, prefix, stream);
+}
+
+}  // namespace b200

@@ -1,0 +1,213 @@
+// Rows into and out of an 8-bit paged key/value cache.
+//
+// A cached row (one token, one head, D elements) is D e4m3 values and one power of two 2^e, kept as its biased exponent
+// (e8m0, one byte): the least e with amax <= 448 * 2^e, so the largest value uses the format's top binade.  A power of two
+// costs a float format nothing (only values 2^-15 below the row's largest lose bits they would keep under a finer scale)
+// and makes both directions exact where it matters: x * 2^-e is exact, so a value is rounded once, to e4m3; value * 2^e is
+// exact in bf16, so reading back rounds nothing (fp16: once, below 2^-14 and beyond 65504).  A row of zeros has e = 0; a
+// row with a NaN or an infinity has the scale NaN (255) and reads as NaN; e is at least -127.
+//
+// Bound by HBM.  Writing: a row is D / 8 lanes with 8 elements each (one 16-byte load, one 8-byte store), the maximum
+// meets over those lanes.  Reading: D / 16 lanes with 16 elements each (one 16-byte load, two 16-byte stores).
+// A page number outside the pool is reported through the status word and nothing is read or written there.
+#include "common.cuh"
+#include "debug.cuh"
+#include "fp8.cuh"
+
+namespace b200 {
+
+namespace {
+
+constexpr int kThreads = 256;
+
+// Pool row (page, row in page) of position `pos` of sequence b; false: outside the table or the pool.
+__device__ __forceinline__ bool locate(const B200CacheRowsParams& p, int page_shift, int b, int64_t pos, int64_t* page, int* row) {
+  const int64_t slot = pos >> page_shift;
+  if (pos < 0 || slot >= p.block_table_stride) return false;
+  *page = p.block_table[static_cast<int64_t>(b) * p.block_table_stride + slot];
+  *row = static_cast<int>(pos & ((1 << page_shift) - 1));
+  return *page >= 0 && *page < p.n_pages;
+}
+
+template <bool BF16, int LPR>   // LPR: lanes of a row, a power of two >= D / 8
+__global__ void __launch_bounds__(kThreads) cache_write_kernel(const B200CacheRowsParams p, const int page_shift, const int tokens,
+                                                               const int rows_16b) {
+  constexpr int kRows = kThreads / LPR;
+  const int b = blockIdx.y, i0 = blockIdx.x * tokens;
+  pdl_wait();
+  pdl_launch_dependents();
+  int n = p.lens != nullptr ? p.lens[b] : p.L;
+  n = n < p.L ? n : p.L;
+  const int n_tok = n - i0 < tokens ? n - i0 : tokens;
+  if (n_tok <= 0) return;
+  const int lane = threadIdx.x % LPR, c0 = lane * 8;
+  const int64_t start = p.start[b];
+  const int total = n_tok * 2 * p.Hkv;
+  for (int r = threadIdx.x / LPR; r < (total + kRows - 1) / kRows * kRows; r += kRows) {   // (whole warps: the maximum meets)
+    const int t = r / (2 * p.Hkv);
+    int h = r - t * 2 * p.Hkv;
+    const bool is_v = h >= p.Hkv;
+    h -= is_v ? p.Hkv : 0;
+    const int64_t* xs = is_v ? p.v_stride : p.k_stride;
+    const uint16_t* x = static_cast<const uint16_t*>(is_v ? p.v : p.k) + b * xs[0] + h * xs[1] + (i0 + t) * xs[2] + c0;
+    const bool on = r < total && c0 < p.D;
+    __align__(16) uint16_t e[8] = {};
+    if (on) {
+      if (rows_16b) *reinterpret_cast<uint4*>(e) = *reinterpret_cast<const uint4*>(x);
+      else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = x[i];
+      }
+    }
+    float f[8];
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      f[i] = half_to_f32<BF16>(e[i]);
+      const uint32_t m = __float_as_uint(f[i]) & 0x7fffffffu;
+      top = m > top ? m : top;
+    }
+#pragma unroll
+    for (int o = LPR / 2; o > 0; o >>= 1) {
+      const uint32_t m = __shfl_xor_sync(0xffffffffu, top, o);
+      top = m > top ? m : top;
+    }
+    if (!on) continue;
+    const int code = scale_code(top);
+    const float inv = scale_inverse(code);
+    uint2 w;
+    w.x = pack_e4m3(f[0] * inv, f[1] * inv) | pack_e4m3(f[2] * inv, f[3] * inv) << 16;
+    w.y = pack_e4m3(f[4] * inv, f[5] * inv) | pack_e4m3(f[6] * inv, f[7] * inv) << 16;
+    int64_t page;
+    int row;
+    if (!locate(p, page_shift, b, start + i0 + t, &page, &row)) {
+      const int64_t pos = start + i0 + t;
+      const bool full = pos >= (static_cast<int64_t>(p.block_table_stride) << page_shift);
+      report_page(p.status, full ? B200_SDPA_ERR_CACHE_FULL : B200_SDPA_ERR_PAGE, b, static_cast<int>(pos), p.n_pages);
+      continue;
+    }
+    const int64_t* ps = is_v ? p.v_pages_stride : p.k_pages_stride;
+    const int64_t* ss = is_v ? p.v_scales_stride : p.k_scales_stride;
+    uint8_t* dst = static_cast<uint8_t*>(is_v ? p.v_pages : p.k_pages) + page * ps[0] + h * ps[1] + row * ps[2] + c0;
+    *reinterpret_cast<uint2*>(dst) = w;
+    if (lane == 0) static_cast<uint8_t*>(is_v ? p.v_scales : p.k_scales)[page * ss[0] + h * ss[1] + row * ss[2]] = static_cast<uint8_t>(code);
+  }
+}
+
+// LPR: lanes of a row, a power of two >= D / 16.  QUANT false: the pools hold the rows' own 16-bit type (strides in
+// elements).  Without lens every row is there.
+template <bool BF16, int LPR, bool QUANT>
+__global__ void __launch_bounds__(kThreads) cache_read_kernel(const B200CacheRowsParams p, const int page_shift, const int tokens,
+                                                               const int rows_16b) {
+  constexpr int kRows = kThreads / LPR;
+  const int b = blockIdx.y, i0 = blockIdx.x * tokens;
+  pdl_wait();
+  pdl_launch_dependents();
+  int n = p.lens != nullptr ? p.lens[b] : p.L;
+  n = n < p.L ? n : p.L;
+  const int n_tok = p.L - i0 < tokens ? p.L - i0 : tokens;
+  const int lane = threadIdx.x % LPR, c0 = lane * 16;
+  if (c0 >= p.D) return;
+  const int total = n_tok * 2 * p.Hkv;
+  for (int r = threadIdx.x / LPR; r < total; r += kRows) {
+    const int hk = r / n_tok, t = r - hk * n_tok;   // neighbouring tokens of a head: neighbouring rows of the result
+    const bool is_v = hk >= p.Hkv;
+    const int h = hk - (is_v ? p.Hkv : 0);
+    const int64_t* xs = is_v ? p.v_stride : p.k_stride;
+    uint16_t* x = static_cast<uint16_t*>(const_cast<void*>(is_v ? p.v : p.k)) + b * xs[0] + h * xs[1] + (i0 + t) * xs[2] + c0;
+    __align__(16) uint32_t out[8] = {};
+    if (i0 + t < n) {
+      int64_t page;
+      int row;
+      if (locate(p, page_shift, b, i0 + t, &page, &row)) {
+        const int64_t* ps = is_v ? p.v_pages_stride : p.k_pages_stride;
+        const int64_t at = page * ps[0] + h * ps[1] + row * ps[2] + c0;
+        const void* pool = is_v ? p.v_pages : p.k_pages;
+        if constexpr (QUANT) {
+          const int64_t* ss = is_v ? p.v_scales_stride : p.k_scales_stride;
+          const uint4 w = ld_stream_16B(static_cast<const uint8_t*>(pool) + at);
+          const float scale = scale_value(static_cast<const uint8_t*>(is_v ? p.v_scales : p.k_scales)[page * ss[0] + h * ss[1] + row * ss[2]]);
+          const uint32_t in[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float f[4];
+            unpack_e4m3x4(in[i], f);
+            out[2 * i] = pack16<BF16>(f[0] * scale, f[1] * scale);
+            out[2 * i + 1] = pack16<BF16>(f[2] * scale, f[3] * scale);
+          }
+        } else {
+          *reinterpret_cast<uint4*>(out) = ld_stream_16B(static_cast<const uint16_t*>(pool) + at);
+          *reinterpret_cast<uint4*>(out + 4) = ld_stream_16B(static_cast<const uint16_t*>(pool) + at + 8);
+        }
+      } else {
+        report_page(p.status, B200_SDPA_ERR_PAGE, b, i0 + t, p.n_pages);
+      }
+    }
+    if (rows_16b) {
+      *reinterpret_cast<uint4*>(x) = make_uint4(out[0], out[1], out[2], out[3]);
+      *reinterpret_cast<uint4*>(x + 8) = make_uint4(out[4], out[5], out[6], out[7]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] = static_cast<uint16_t>(out[i / 2] >> (16 * (i & 1)));
+    }
+  }
+}
+
+// Tokens of one CTA: enough for a few rounds of its threads, fewer where there would not be several CTAs for every SM.
+int tokens_per_cta(const B200CacheRowsParams& p, int rows_per_round) {
+  int tokens = (4 * rows_per_round + 2 * p.Hkv - 1) / (2 * p.Hkv);
+  tokens = tokens < 1 ? 1 : tokens;
+  while (tokens > 1 && static_cast<int64_t>(p.B) * ((p.L + tokens - 1) / tokens) < 4 * 148) tokens = (tokens + 1) / 2;
+  return tokens;
+}
+
+int page_shift_of(int page_size) {
+  int s = 0;
+  while ((1 << s) < page_size) ++s;
+  return s;
+}
+
+// Whether every dense row starts on 16 bytes.
+bool rows_16b(const B200CacheRowsParams& p) {
+  if (reinterpret_cast<uintptr_t>(p.k) % 16 || reinterpret_cast<uintptr_t>(p.v) % 16) return false;
+  for (int i = 0; i < 3; ++i)
+    if (p.k_stride[i] % 8 || p.v_stride[i] % 8) return false;
+  return true;
+}
+
+enum Direction { WRITE, READ, GATHER };
+
+template <Direction DIR, bool BF16, int LPR> int launch_rows(const B200CacheRowsParams& p, cudaStream_t stream) {
+  const int tokens = tokens_per_cta(p, kThreads / LPR);
+  const dim3 grid((p.L + tokens - 1) / tokens, p.B);
+  const int shift = page_shift_of(p.page_size);
+  bool ok;
+  if constexpr (DIR == WRITE) ok = launch_pdl(cache_write_kernel<BF16, LPR>, grid, kThreads, 0, stream, p, shift, tokens, rows_16b(p) ? 1 : 0);
+  else ok = launch_pdl(cache_read_kernel<BF16, LPR, DIR == READ>, grid, kThreads, 0, stream, p, shift, tokens, rows_16b(p) ? 1 : 0);
+  if (!ok) return B200_SDPA_ERR_CUDA;
+  count_launch(DIR == WRITE ? KID_CACHE_WRITE : KID_CACHE_READ);
+  return B200_SDPA_OK;
+}
+
+template <Direction DIR, bool BF16> int launch_lanes(const B200CacheRowsParams& p, cudaStream_t stream) {
+  const int lanes = p.D / (DIR == WRITE ? 8 : 16);
+  if (lanes <= 4) return launch_rows<DIR, BF16, 4>(p, stream);
+  if (lanes <= 8) return launch_rows<DIR, BF16, 8>(p, stream);
+  if (lanes <= 16) return launch_rows<DIR, BF16, 16>(p, stream);
+  return launch_rows<DIR, BF16, 32>(p, stream);
+}
+
+}  // namespace
+
+int launch_cache_write(const B200CacheRowsParams& p, cudaStream_t stream) {
+  return p.dtype == B200_SDPA_BF16 ? launch_lanes<WRITE, true>(p, stream) : launch_lanes<WRITE, false>(p, stream);
+}
+int launch_cache_read(const B200CacheRowsParams& p, cudaStream_t stream) {
+  return p.dtype == B200_SDPA_BF16 ? launch_lanes<READ, true>(p, stream) : launch_lanes<READ, false>(p, stream);
+}
+int launch_cache_gather(const B200CacheRowsParams& p, cudaStream_t stream) {
+  if (p.k_scales != nullptr) return launch_cache_read(p, stream);
+  return launch_lanes<GATHER, true>(p, stream);   // (a copy: either 16-bit type)
+}
+
+}  // namespace b200

@@ -83,7 +83,10 @@ enum KernelId {
   KID_BWD_DQ = 5,
   KID_BWD_DKV = 6,
   KID_BWD_PREP = 7,
-  KID_COUNT = 8
+  KID_ROTARY = 8,
+  KID_CACHE_WRITE = 9,
+  KID_CACHE_READ = 10,
+  KID_COUNT = 11
 };
 
 // Host launchers implemented in the per-kernel translation units.  Each returns
@@ -129,6 +132,34 @@ int plan_prefill_wide(const Problem& p, int dtype, B200SdpaPlan* plan);
 int launch_prefill_wide(const Problem& p, int dtype, cudaStream_t stream);
 
 int launch_merge(const B200SdpaMergeParams& m, cudaStream_t stream);
+
+int launch_rotary(const B200RotaryParams& p, cudaStream_t stream);
+int launch_cache_write(const B200CacheRowsParams& p, cudaStream_t stream);
+int launch_cache_read(const B200CacheRowsParams& p, cudaStream_t stream);
+
+// The scales of an 8-bit paged cache beside a Problem whose k and v are its pools (strides in bytes = elements).
+struct CacheScales {
+  const uint8_t* k;
+  const uint8_t* v;
+  int64_t ks[3], vs[3];   // page, head, row in page
+  int n_pages;
+};
+int launch_decode_partial_fp8(const Problem& p, const CacheScales& sc, int dtype, int chunk, int nsplit, float* part_o,
+                              float* part_ml, cudaStream_t stream);
+int cache_decode_served(const B200CacheDecodeParams& a);   // a status
+int plan_cache_decode(const B200CacheDecodeParams& a, B200SdpaPlan* plan);
+int launch_cache_decode(const B200CacheDecodeParams& a, cudaStream_t stream);
+
+// The split form of the per-CTA prefill kernel (prefill_sm100.cu): the rows of a kv head's query heads packed into tiles,
+// the keys cut into ranges, fp32 partials [B][Hq][L][n_split][D] and (maximum in log2 units, sum) pairs.
+struct PackGeom {
+  int lb, n_pairs, dual, n_split, split_tiles;
+  long long grid;
+  uint64_t ws_bytes;
+};
+bool prefix_eligible(const Problem& p, int dtype);
+void prefix_geometry(const Problem& p, PackGeom* g);
+int launch_prefix_partial(const Problem& p, int dtype, const PackGeom& g, float* part_o, float* part_ml, cudaStream_t stream);
 
 int launch_bwd_generic(const BwdProblem& bp, int dtype, cudaStream_t stream);
 int plan_bwd_generic(const BwdProblem& bp, int dtype, B200SdpaPlan* plan);

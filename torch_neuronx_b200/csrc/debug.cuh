@@ -30,7 +30,10 @@ enum DebugFile {
   DBG_PREFILL_WIDE = 7,
   DBG_BWD_TC = 8,
   DBG_BWD_WIDE = 9,
-  DBG_FP32 = 10
+  DBG_FP32 = 10,
+  DBG_ROTARY = 11,
+  DBG_DECODE_FP8 = 12,
+  DBG_CACHE_DECODE = 13
 };
 
 __device__ __forceinline__ bool dbg_fail(int* status, int site, long long index, long long limit) {

@@ -974,12 +974,6 @@ __global__ void __launch_bounds__(256) prefill_combine_kernel(const Problem p, c
     p.lse[b * p.ls[0] + h * p.ls[1] + i * p.ls[2]] = lsum > 0.f ? fmaf(mx, kLn2, lg2(lsum) * kLn2) : -CUDART_INF_F;
 }
 
-struct PackGeom {
-  int lb, n_pairs, dual, n_split, split_tiles;
-  long long grid;
-  uint64_t ws_bytes;
-};
-
 // Whether the split form serves a request, and how.  The plain form gives every 128 (or 256) rows of a head a CTA
 // that walks all its keys: with a handful of rows, or few heads and sequences, that leaves most SMs without work and
 // most of every tile without rows.  The rule compares estimates of both, in cycles of one SM:
@@ -1064,7 +1058,7 @@ bool pack_geometry(const Problem& p, PackGeom* best) {
 }
 
 template <int D, bool BF16>
-int launch_packed(const Problem& p, const PackGeom& g, float* workspace, cudaStream_t stream) {
+int launch_pack_partial(const Problem& p, const PackGeom& g, float* part_o, float* part_ml, cudaStream_t stream) {
   using C = Cfg<D>;
   CUtensorMap tq, tk, tv;
   if (!make_map(&tq, p.q, BF16, D, p.L, p.Hq, p.B, p.qs, g.lb, p.group) || !make_map(&tk, p.k, BF16, D, p.S, p.Hkv, p.B, p.ks) ||
@@ -1075,28 +1069,78 @@ int launch_packed(const Problem& p, const PackGeom& g, float* workspace, cudaStr
     cudaGetLastError();
     return B200_SDPA_ERR_CUDA;
   }
-  const long long n_rows = static_cast<long long>(p.B) * p.Hq * p.L;
   PackArgs a;
   a.lb = g.lb;
   a.dual = g.dual;
   a.n_pairs = g.n_pairs;
   a.n_split = g.n_split;
   a.split_tiles = g.split_tiles;
-  a.part_o = workspace;
-  a.part_ml = workspace + n_rows * g.n_split * D;
+  a.part_o = part_o;
+  a.part_ml = part_ml;
   if (!launch_pdl(kern, dim3(static_cast<unsigned>(g.grid)), kThreads, C::kSmemBytes, stream, tq, tk, tv, tq, p, 0, 0, 1,
                   wait_limit_cycles(), a))
     return B200_SDPA_ERR_CUDA;
   count_launch(KID_PREFILL);
+  return B200_SDPA_OK;
+}
+
+template <int D, bool BF16>
+int launch_packed(const Problem& p, const PackGeom& g, float* workspace, cudaStream_t stream) {
+  const long long n_rows = static_cast<long long>(p.B) * p.Hq * p.L;
+  float* part_ml = workspace + n_rows * g.n_split * D;
+  const int rc = launch_pack_partial<D, BF16>(p, g, workspace, part_ml, stream);
+  if (rc != B200_SDPA_OK) return rc;
   using T = std::conditional_t<BF16, __nv_bfloat16, __half>;
   if (!launch_pdl(prefill_combine_kernel<T, D>, dim3(static_cast<unsigned>((n_rows + 7) / 8)), 256, 0, stream, p, g.n_split,
-                  a.part_o, a.part_ml))
+                  workspace, part_ml))
     return B200_SDPA_ERR_CUDA;
   count_launch(KID_COMBINE);
   return B200_SDPA_OK;
 }
 
 }  // namespace
+
+// A prefix that a batch shares: its sequences' query rows are the rows of one sequence (L = the batch, B = 1, no mask).
+bool prefix_eligible(const Problem& p, int dtype) {
+  if (dtype != B200_SDPA_F16 && dtype != B200_SDPA_BF16) return false;
+  if (!(p.scale > 0.f) || !(p.scale < 1e30f) || p.L < 1 || p.S < 1 || p.E != p.Dv || (p.E != 64 && p.E != 128) || p.group > kBlockM)
+    return false;
+  return strides_ok(p.q, p.qs, p.L, p.Hq, p.B) && strides_ok(p.k, p.ks, p.S, p.Hkv, p.B) && strides_ok(p.v, p.vs, p.S, p.Hkv, p.B);
+}
+
+void prefix_geometry(const Problem& p, PackGeom* best) {
+  constexpr long long kSms = 148, kTileCycles = 3500, kCtaCycles = 9000;
+  const long long streams = static_cast<long long>(p.Hkv) * p.B, tiles = (p.S + kBlockN - 1) / kBlockN;
+  const long long row_bytes = static_cast<long long>(p.B) * p.Hq * p.L * (p.Dv + 2) * 4;
+  PackGeom g;
+  g.lb = kBlockM / p.group < p.L ? kBlockM / p.group : p.L;
+  const int n_rt = (p.L + g.lb - 1) / g.lb;
+  g.n_pairs = (n_rt + 1) / 2;
+  g.dual = n_rt == 1 ? 1 : 0;
+  const int per_cta = g.dual ? 2 : 1;   // partials a CTA leaves for a row
+  long long best_cost = 1LL << 60;
+  for (long long n = 1; n <= tiles && n <= 2 * kSms; ++n) {
+    g.split_tiles = static_cast<int>((tiles + n - 1) / n);
+    if ((tiles + g.split_tiles - 1) / g.split_tiles != n) continue;
+    g.n_split = static_cast<int>(n) * per_cta;
+    g.grid = g.n_pairs * streams * n;
+    g.ws_bytes = static_cast<uint64_t>(row_bytes) * g.n_split;
+    const long long rounds = (g.grid + kSms - 1) / kSms, steps = (g.split_tiles + per_cta - 1) / per_cta;
+    const long long cost = rounds * (steps * kTileCycles + kCtaCycles) + 2 * row_bytes * g.n_split / 6000;
+    if (cost < best_cost) {
+      best_cost = cost;
+      *best = g;
+    }
+  }
+}
+
+int launch_prefix_partial(const Problem& p, int dtype, const PackGeom& g, float* part_o, float* part_ml, cudaStream_t stream) {
+  if (g.grid <= 0 || g.grid > 0x7fffffffLL) return B200_SDPA_ERR_UNSUPPORTED;
+  const bool bf16 = dtype == B200_SDPA_BF16;
+  if (p.E == 128)
+    return bf16 ? launch_pack_partial<128, true>(p, g, part_o, part_ml, stream) : launch_pack_partial<128, false>(p, g, part_o, part_ml, stream);
+  return bf16 ? launch_pack_partial<64, true>(p, g, part_o, part_ml, stream) : launch_pack_partial<64, false>(p, g, part_o, part_ml, stream);
+}
 
 bool prefill_eligible(const Problem& p, int dtype, bool* alignment_only_failure) {
   if (p.E > 128) return prefill_wide_eligible(p, dtype, alignment_only_failure);

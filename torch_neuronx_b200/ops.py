@@ -397,6 +397,8 @@ def paged_decode(
     rope_cos: Optional[torch.Tensor] = None,
     rope_sin: Optional[torch.Tensor] = None,
     rope_interleaved: bool = False,
+    k_scales: Optional[torch.Tensor] = None,
+    v_scales: Optional[torch.Tensor] = None,
 ):
     """One decode step against a paged key/value cache; returns ``(out, lse)`` -- or, with
     ``k_new`` / ``v_new`` (``(B, Hkv, D)``, the rows of the token being decoded),
@@ -410,7 +412,17 @@ def paged_decode(
     ``s % page_size`` of page ``block_table[b, s // page_size]``.  The split-KV decode
     kernel reads the pages in place -- no gather into a dense cache.  Upstream's decode
     runs the same op on a dense cache (``torch_mlir/ops/scaled_dot_product_attention.py:64-68``);
-    the paged layout is what a serving loop around that op keeps."""
+    the paged layout is what a serving loop around that op keeps.
+
+    With ``k_scales`` / ``v_scales`` the pools are an 8-bit cache (e4m3 values with a power of two for each row, as
+    :func:`paged_write` fills it); a row is appended to it with :func:`paged_write` before the call, not by ``k_new``."""
+    if k_scales is not None or v_scales is not None:
+        if k_new is not None or v_new is not None or rope_cos is not None or rope_sin is not None:
+            raise RuntimeError("paged_decode: a row is appended to an 8-bit cache by paged_write, before the call")
+        from . import cache
+
+        return cache.decode_8bit(query, k_pages, v_pages, k_scales, v_scales, block_table, kv_lens, scale=scale, layout=layout,
+                                 out=out, lse=lse, need_lse=need_lse, kv_chunk=kv_chunk)
     if _lib.native is not None and layout in ("NHD", "HND") and not torch.compiler.is_compiling():
         got = _lib.native.decode(query, k_pages, v_pages, block_table, kv_lens, scale, 1 if layout == "NHD" else 2, out, lse,
                                  need_lse, kv_chunk, k_new, v_new, rope_cos, rope_sin, rope_interleaved)
