@@ -108,7 +108,7 @@ def test_decode_refusals(change, code):
 def test_decode_plans():
     rc, plan = _plan(_decode())
     assert rc == _lib.OK and plan.launches == 2 and plan.kv_splits >= 1
-    assert plan.workspace_bytes >= 4 * 8 * plan.kv_splits * 130 * 4
+    assert plan.workspace_bytes >= 8 * plan.kv_splits * 130 * 4
     rc, shared = _plan(_decode(prefix_len=1000))
     assert rc == _lib.OK and shared.workspace_bytes > plan.workspace_bytes
     rc, only = _plan(_decode(prefix_len=1000, block_table_stride=0, block_table=None))

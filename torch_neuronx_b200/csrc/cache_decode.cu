@@ -21,16 +21,22 @@ namespace {
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kCombineWarps = 4;
 
-struct Partials {
-  const float* o;    // [row][n][D]
-  const float* ml;   // [row][n][2]
-  int n;
+// Rows of partials: o [row][D], ml [row][2]
+struct Rows {
+  const float* o;
+  const float* ml;
+};
+struct Merge {
+  Rows own, prefix;
+  int n_prefix;        // of a (query head, sequence)
+  int n_own, chunk;    // 16-bit cache: ranges of `chunk` keys, rows (sequence * Hq + head) * n_own + range
+  const int2* range;   // 8-bit cache (decode_fp8.cu)
+  int heads, units;
 };
 
-// One CTA per (sequence, query head): the prefix's partials (row h * B + b) and the own ones in use (row b * Hq + h).
+// One CTA per (sequence, query head): the prefix's partials (rows (h * B + b) * n ..) and the own ones in use.
 template <typename T, int D>
-__global__ void __launch_bounds__(kCombineWarps * 32)
-    cache_combine_kernel(const Problem p, const int chunk, const Partials own, const Partials prefix) {
+__global__ void __launch_bounds__(kCombineWarps * 32) cache_combine_kernel(const Problem p, const Merge a) {
   constexpr int C = D / 32;   // columns per lane
   __shared__ float sm_o[kCombineWarps][D];
   __shared__ float sm_l[kCombineWarps];
@@ -38,18 +44,28 @@ __global__ void __launch_bounds__(kCombineWarps * 32)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
   pdl_launch_dependents();
-  int used = 0;
-  if (own.n > 0) {
-    used = (valid_keys(p, b) + chunk - 1) / chunk;
-    used = used < 1 ? 1 : (used > own.n ? own.n : used);
+  // own partials: row own0 + s * step
+  int used = 0, step = 1;
+  int64_t own0 = 0;
+  if (a.range != nullptr) {
+    if (valid_keys(p, b) > 0) {
+      const int in_group = h % p.group;
+      const int2 r = a.range[static_cast<int64_t>(b) * a.units + in_group / a.heads * p.Hkv + h / p.group];
+      used = r.y - r.x + 1;
+      step = a.heads;
+      own0 = static_cast<int64_t>(r.x) * a.heads + in_group % a.heads;
+    }
+  } else if (a.n_own > 0) {
+    used = (valid_keys(p, b) + a.chunk - 1) / a.chunk;
+    used = used < 1 ? 1 : (used > a.n_own ? a.n_own : used);
+    own0 = (static_cast<int64_t>(b) * p.Hq + h) * a.n_own;
   }
-  const int64_t own0 = (static_cast<int64_t>(b) * p.Hq + h) * own.n, pre0 = (static_cast<int64_t>(h) * p.B + b) * prefix.n;
-  if (!dbg_range(p.status, DBG_CACHE_DECODE * 100 + 1, own0, used, static_cast<int64_t>(p.B) * p.Hq * own.n) ||
-      !dbg_bhrc(p.status, DBG_CACHE_DECODE * 100 + 2, b, p.B, h, p.Hq, 0, 1, lane * C, C, p.Dv))
-    return;
-  const int total = prefix.n + used;
+  const int64_t pre0 = (static_cast<int64_t>(h) * p.B + b) * a.n_prefix;
+  if (!dbg_bhrc(p.status, DBG_CACHE_DECODE * 100 + 1, b, p.B, h, p.Hq, 0, 1, lane * C, C, p.Dv)) return;
+  auto row_of = [&](int s) { return s < a.n_prefix ? pre0 + s : own0 + static_cast<int64_t>(s - a.n_prefix) * step; };
+  const int total = a.n_prefix + used;
   auto pair_of = [&](int s) {
-    return *reinterpret_cast<const float2*>(s < prefix.n ? prefix.ml + (pre0 + s) * 2 : own.ml + (own0 + s - prefix.n) * 2);
+    return *reinterpret_cast<const float2*>((s < a.n_prefix ? a.prefix.ml : a.own.ml) + row_of(s) * 2);
   };
   float mx = -CUDART_INF_F;
   for (int s = lane; s < total; s += 32) mx = fmaxf(mx, pair_of(s).x);
@@ -64,7 +80,7 @@ __global__ void __launch_bounds__(kCombineWarps * 32)
     const float2 ml = pair_of(s);
     // a range without a visible key has the sum 0, and the prefix kernel wrote nothing else for it (a NaN sum counts)
     if (ml.y == 0.f) continue;
-    const float* src = (s < prefix.n ? prefix.o + (pre0 + s) * D : own.o + (own0 + s - prefix.n) * D) + lane * C;
+    const float* src = (s < a.n_prefix ? a.prefix.o : a.own.o) + row_of(s) * D + lane * C;
     float v[C];
     if constexpr (C == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src);
     else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(src);
@@ -92,7 +108,8 @@ __global__ void __launch_bounds__(kCombineWarps * 32)
 }
 
 struct Geometry {
-  int chunk, nsplit;          // own keys; nsplit = 0: no table
+  int chunk, nsplit;          // own keys of a 16-bit cache; nsplit = 0: no table, or an 8-bit cache
+  Fp8Geometry fp8;            // own keys of an 8-bit cache
   PackGeom pack;              // prefix
   uint64_t own_bytes, prefix_bytes, dense_bytes;
   uint64_t total() const { return own_bytes + prefix_bytes + dense_bytes; }
@@ -151,18 +168,16 @@ Problem prefix_problem(const B200CacheDecodeParams& a, const void* k, const void
   return p;
 }
 
-// Keys of one CTA: enough CTAs for every slot of the GPU, ranges long enough to pay for a CTA's start and end.
+// Keys of one CTA of the 16-bit kernel: enough CTAs for every slot of the GPU, ranges long enough to pay for a CTA's start and end.
 int default_chunk(const Problem& p) {
-  const int heads = p.group <= 8 ? 8 : 16;
-  const int64_t units = static_cast<int64_t>(p.B) * p.Hkv * ((p.group + heads - 1) / heads);
-  const int64_t slots = heads == 8 ? 444 : 296;
+  const int64_t units = static_cast<int64_t>(p.B) * p.Hkv * ((p.group + 15) / 16);
   int best = 256;
   double best_us = 1e30;
-  for (int chunk = 64; chunk <= 4096; chunk += chunk < 512 ? 64 : 256) {
+  for (int chunk = 64; chunk <= 2048; chunk += chunk < 512 ? 64 : 256) {
     const int n = (p.S + chunk - 1) / chunk;
-    const double fill = static_cast<double>(units) * n / slots;
+    const double fill = static_cast<double>(units) * n / 444;
     const double rounds = fill < 1.0 ? 1.0 : fill + 0.35;
-    const double us = rounds * (3.5 + chunk / 64.0 * (0.5 + 0.8 * (fill < 1.0 ? fill : 1.0))) * (1.0 + 0.002 * n);
+    const double us = rounds * (3.5 + chunk / 64.0 * (1.1 + 1.6 * (fill < 1.0 ? fill : 1.0))) * (1.0 + 0.002 * n);
     if (us < best_us) {
       best_us = us;
       best = chunk;
@@ -190,10 +205,13 @@ int geometry(const B200CacheDecodeParams& a, Geometry* g) {
   const Problem p = own_problem(a);
   *g = {};
   const int64_t rows = static_cast<int64_t>(a.B) * a.Hq;
-  if (p.S > 0) {
+  if (p.S > 0 && a.k_scales != nullptr) {
+    if (!decode_fp8_geometry(p, a.kv_chunk, &g->fp8)) return B200_SDPA_ERR_UNSUPPORTED;
+    g->own_bytes = aligned(g->fp8.bytes);
+  } else if (p.S > 0) {
     g->chunk = a.kv_chunk > 0 ? (a.kv_chunk + 31) / 32 * 32 : default_chunk(p);
     g->nsplit = (p.S + g->chunk - 1) / g->chunk;
-    if (g->nsplit > 65535 || static_cast<int64_t>(p.Hkv) * ((p.group + 7) / 8) > 65535) return B200_SDPA_ERR_UNSUPPORTED;
+    if (g->nsplit > 65535 || static_cast<int64_t>(p.Hkv) * ((p.group + 15) / 16) > 65535) return B200_SDPA_ERR_UNSUPPORTED;
     g->own_bytes = aligned(static_cast<uint64_t>(rows) * g->nsplit * (a.D + 2) * sizeof(float));
   }
   if (a.prefix_len > 0) {
@@ -205,10 +223,9 @@ int geometry(const B200CacheDecodeParams& a, Geometry* g) {
   return B200_SDPA_OK;
 }
 
-template <typename T>
-int launch_combine(const Problem& p, int chunk, const Partials& own, const Partials& prefix, cudaStream_t stream) {
+template <typename T> int launch_combine(const Problem& p, const Merge& a, cudaStream_t stream) {
   auto kern = p.E == 128 ? cache_combine_kernel<T, 128> : cache_combine_kernel<T, 64>;
-  if (!launch_pdl(kern, dim3(p.B * p.Hq), kCombineWarps * 32, 0, stream, p, chunk, own, prefix)) return B200_SDPA_ERR_CUDA;
+  if (!launch_pdl(kern, dim3(p.B * p.Hq), kCombineWarps * 32, 0, stream, p, a)) return B200_SDPA_ERR_CUDA;
   count_launch(KID_COMBINE);
   return B200_SDPA_OK;
 }
@@ -219,17 +236,17 @@ int plan_cache_decode(const B200CacheDecodeParams& a, B200SdpaPlan* plan) {
   Geometry g;
   const int rc = geometry(a, &g);
   if (rc != B200_SDPA_OK) return rc;
-  const int heads = a.Hq / a.Hkv <= 8 && a.k_scales != nullptr ? 8 : 16;
+  const bool fp8 = g.fp8.grid > 0;
   plan->path = B200_SDPA_PATH_DECODE;
   plan->block_m = 1;
-  plan->block_n = g.chunk;
-  plan->grid_x = a.Hkv * ((a.Hq / a.Hkv + heads - 1) / heads);
-  plan->grid_y = a.B;
-  plan->grid_z = g.nsplit;
-  plan->threads = 128;
+  plan->block_n = fp8 ? 128 : g.chunk;
+  plan->grid_x = fp8 ? g.fp8.grid : a.Hkv * ((a.Hq / a.Hkv + 15) / 16);
+  plan->grid_y = fp8 ? 1 : a.B;
+  plan->grid_z = fp8 ? 1 : g.nsplit;
+  plan->threads = fp8 ? 192 : 128;
   plan->smem_bytes = 0;
-  plan->kv_splits = g.nsplit;
-  plan->launches = 1 + (g.nsplit > 0 ? 1 : 0) + (a.prefix_len > 0 ? 2 : 0);
+  plan->kv_splits = fp8 ? g.fp8.grid : g.nsplit;
+  plan->launches = 1 + (plan->kv_splits > 0 ? 1 : 0) + (a.prefix_len > 0 ? 2 : 0);
   plan->workspace_bytes = g.total();
   return B200_SDPA_OK;
 }
@@ -243,8 +260,6 @@ int launch_cache_decode(const B200CacheDecodeParams& a, cudaStream_t stream) {
   const Problem p = own_problem(a);
   const int64_t rows = static_cast<int64_t>(a.B) * a.Hq;
   char* ws = static_cast<char*>(a.workspace);
-  float* own_o = reinterpret_cast<float*>(ws);
-  float* own_ml = own_o + rows * g.nsplit * a.D;
   float* pre_o = reinterpret_cast<float*>(ws + g.own_bytes);
   float* pre_ml = pre_o + rows * g.pack.n_split * a.D;
   if (a.prefix_len > 0) {
@@ -279,25 +294,38 @@ int launch_cache_decode(const B200CacheDecodeParams& a, cudaStream_t stream) {
     rc = launch_prefix_partial(prefix_problem(a, r.k, r.v), a.dtype, g.pack, pre_o, pre_ml, stream);
     if (rc != B200_SDPA_OK) return rc;
   }
-  if (g.nsplit > 0) {
-    if (a.k_scales != nullptr) {
-      CacheScales sc = {};
-      sc.k = static_cast<const uint8_t*>(a.k_scales);
-      sc.v = static_cast<const uint8_t*>(a.v_scales);
-      for (int i = 0; i < 3; ++i) {
-        sc.ks[i] = a.k_scales_stride[i];
-        sc.vs[i] = a.v_scales_stride[i];
-      }
-      sc.n_pages = a.n_pages;
-      rc = launch_decode_partial_fp8(p, sc, a.dtype, g.chunk, g.nsplit, own_o, own_ml, stream);
-    } else {
-      rc = launch_decode_partial_mma(p, a.dtype, g.chunk, g.nsplit, own_o, own_ml, stream);
+  Merge m = {};
+  m.prefix = {pre_o, pre_ml};
+  m.n_prefix = g.pack.n_split;
+  if (g.fp8.grid > 0) {
+    CacheScales sc = {};
+    sc.k = static_cast<const uint8_t*>(a.k_scales);
+    sc.v = static_cast<const uint8_t*>(a.v_scales);
+    for (int i = 0; i < 3; ++i) {
+      sc.ks[i] = a.k_scales_stride[i];
+      sc.vs[i] = a.v_scales_stride[i];
     }
-    if (rc != B200_SDPA_OK) return rc;
+    sc.n_pages = a.n_pages;
+    OwnPartials part;
+    part.slots = g.fp8.slots;
+    part.o = reinterpret_cast<float*>(ws);
+    part.ml = part.o + g.fp8.slots * g.fp8.heads * a.D;
+    part.range = reinterpret_cast<int2*>(part.ml + g.fp8.slots * g.fp8.heads * 2);
+    m.own = {part.o, part.ml};
+    m.range = part.range;
+    m.heads = g.fp8.heads;
+    m.units = g.fp8.units;
+    rc = launch_decode_partial_fp8(p, sc, a.dtype, g.fp8, part, stream);
+  } else if (g.nsplit > 0) {
+    float* own_o = reinterpret_cast<float*>(ws);
+    float* own_ml = own_o + rows * g.nsplit * a.D;
+    m.own = {own_o, own_ml};
+    m.n_own = g.nsplit;
+    m.chunk = g.chunk;
+    rc = launch_decode_partial_mma(p, a.dtype, g.chunk, g.nsplit, own_o, own_ml, stream);
   }
-  const Partials own = {own_o, own_ml, g.nsplit}, prefix = {pre_o, pre_ml, g.pack.n_split};
-  return a.dtype == B200_SDPA_BF16 ? launch_combine<__nv_bfloat16>(p, g.chunk, own, prefix, stream)
-                                   : launch_combine<__half>(p, g.chunk, own, prefix, stream);
+  if (rc != B200_SDPA_OK) return rc;
+  return a.dtype == B200_SDPA_BF16 ? launch_combine<__nv_bfloat16>(p, m, stream) : launch_combine<__half>(p, m, stream);
 }
 
 }  // namespace b200

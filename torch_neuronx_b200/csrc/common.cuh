@@ -144,8 +144,22 @@ struct CacheScales {
   int64_t ks[3], vs[3];   // page, head, row in page
   int n_pages;
 };
-int launch_decode_partial_fp8(const Problem& p, const CacheScales& sc, int dtype, int chunk, int nsplit, float* part_o,
-                              float* part_ml, cudaStream_t stream);
+// Partials of the own keys of an 8-bit cache (decode_fp8.cu): slots of `heads` rows; a pair (sequence, unit) has the slots
+// range[pair].x to range[pair].y, all written, unless its sequence is empty.
+struct OwnPartials {
+  float* o;      // [slot][heads][D]
+  float* ml;     // [slot][heads][2]: maximum in log2 units, sum
+  int2* range;   // [pair]
+  int64_t slots;
+};
+struct Fp8Geometry {
+  int heads, units, grid, fixed_blocks;   // units: kv heads x blocks of query heads
+  int64_t slots;
+  uint64_t bytes;
+};
+bool decode_fp8_geometry(const Problem& p, int kv_chunk, Fp8Geometry* g);
+int launch_decode_partial_fp8(const Problem& p, const CacheScales& sc, int dtype, const Fp8Geometry& g, const OwnPartials& part,
+                              cudaStream_t stream);
 int cache_decode_served(const B200CacheDecodeParams& a);   // a status
 int plan_cache_decode(const B200CacheDecodeParams& a, B200SdpaPlan* plan);
 int launch_cache_decode(const B200CacheDecodeParams& a, cudaStream_t stream);

@@ -1,53 +1,79 @@
-// Split-KV flash decoding against an 8-bit paged cache (cache_rows.cu has the format), products on tensor cores.
+// Flash decoding against an 8-bit paged cache (cache_rows.cu has the format), products on tensor cores.
 //
-// The partial kernel of decode_mma.cu with half the bytes: grid (kv head and block of query heads, sequence, key split), the
-// cache read once for all query heads of a block, fp32 partials (o, m, l) merged by the same second launch.
+// The cache is read once for all query heads of a kv head.  Its blocks of 128 keys, over all sequences and kv heads, are one
+// list that is cut into equal ranges, one for each CTA the GPU holds at a time: the lengths are read on the device, so ragged
+// batches leave no SM without work and no CTA starts twice.  A CTA leaves one fp32 partial (o, m, l) for each (sequence, kv head)
+// that its range touches, in slot `CTA + number of the pair` (both only ever grow along the list, so no slot is used twice),
+// and whoever has a pair's first or last block notes the slot; a second launch merges (cache_decode.cu).
 // What the format changes:
-//   * e4m3 is exact in fp16, so both products are fp16 m16n8k16 MMAs with the bytes expanded in registers: a fragment word
-//     of K holds four consecutive elements of one key, and the order inside a k-step is free as long as the query
-//     fragments use it too; a transposed fragment word of V holds two keys x two columns, one byte permutation makes it
-//     an operand for each column.  (8-bit MMAs would need P and Q in 8 bits.)
+//   * e4m3 is exact in fp16, so both products are fp16 m16n8k16 MMAs with the bytes expanded in registers (8-bit MMAs would
+//     need P and Q in 8 bits).  Both are taken transposed, S^T = K Q^T and O^T = V^T P^T: the keys, then the columns of V,
+//     fill the sixteen rows of an MMA and the query heads its eight columns, so that no row is empty and O of 8 heads
+//     needs D / 4 registers.  A fragment word of K holds four consecutive elements of one key, and the order inside a
+//     k-step is free as long as the query fragments use it too; a transposed fragment word of V holds two keys x two
+//     columns, which one byte permutation makes rows 2 i and 2 i + 1 of V^T.  movmatrix turns the probabilities round.
 //   * scores: s = (q . k8) * 2^e_k, the row's power of two applied to the finished fp32 score.  A query row is brought to
 //     a maximum in [2^14, 2^15) by a power of two first (bf16; fp16 keeps its own scale unless it has room above), so
 //     fp16 holds it exactly but for elements 2^-28 below the row's largest, which round at 2^-39 of it.
 //   * values: o += (p 2^(e_v - r + 9)) v8 with r the largest e_v the warp has met (o is rescaled when it grows), so the
 //     probability stays inside fp16; it enters as hi + lo, two fp16 operands: 22 bits, and never coarser than 2^-34 of
-//     the largest value row the warp has met.  With up to 8 query heads the low parts ride in the eight rows of the
-//     MMA that would be empty; with up to 16 they cost a second MMA.
+//     the largest value row the warp has met.
+// One warp brings the rows into a ring of blocks by tensor copies, one for each page and operand, and another the scales; four
+// warps compute, 32 keys of a block each, and wait for nothing but their block.  (With plain copies and one barrier a block of 64
+// keys, as decode_mma.cu has them, the address arithmetic and the latency of table and scales stood in the way: 64 x 512..8192
+// keys, 32/8 heads of 128, 194 us.)
 // Softmax in the exp2 domain on raw scores, statistics fp32, the running maximum raised lazily (2^6).
-#include "common.cuh"
 #include "debug.cuh"
 #include "fp8.cuh"
+#include "tc_common.cuh"
 
 namespace b200 {
 
 namespace {
 
-constexpr int kWarps = 4;
-constexpr int kThreads = kWarps * 32;
-constexpr int kBlockKeys = 64;
-constexpr int kStages = 4;
-constexpr float kLog2e = 1.4426950408889634f;
+using namespace ptx;
+using namespace tc;
+
+constexpr int kWarps = 4;                         // that compute; one more brings the rows, one the scales
+constexpr int kThreads = (kWarps + 2) * 32;
+constexpr int kBlockKeys = 128;
+constexpr int kWarpKeys = kBlockKeys / kWarps;
 constexpr float kRescaleThreshold = 6.0f;
 constexpr float kProbShift = 9.0f;   // p <= 2^6, p 2^9 <= 2^15 in fp16
 
-template <int D> struct Geo {
-  static constexpr int kRowBytes = D + 16;                     // padded row: conflict-free ldmatrix
-  static constexpr int kTileBytes = kBlockKeys * kRowBytes;    // one K or V block
+// A block of the ring: its rows of K, then of V, swizzled in 16-byte pieces as a tensor copy leaves them (128-byte pattern for
+// D = 128, 64-byte for D = 64), so that ldmatrix meets no bank twice.
+template <int D, int HEADS> struct Geo {
+  static constexpr int kTileBytes = kBlockKeys * D;
   static constexpr int kStageBytes = 2 * kTileBytes;
+  static constexpr int kStages = D == 128 && HEADS == 16 ? 2 : 3;
   static constexpr int kRingBytes = kStages * kStageBytes;
   static constexpr int kChunksPerRow = D / 16;
-  static constexpr int kScaleBytes = 2 * 2 * kBlockKeys * 4;   // [parity][K, V][key]
-  static constexpr int kSmemBytes = kRingBytes + kScaleBytes;
+  static constexpr int kCtas = D == 128 || HEADS == 16 ? 2 : 3;             // of an SM
+  static constexpr int kState = D / 4 * (HEADS / 8) + 4 * (HEADS / 8);      // registers of a warp's state: o, m, l
+  static __device__ __forceinline__ int swizzle(int row) { return D == 128 ? row & 7 : (row >> 1) & 3; }
 };
 
-__device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
-__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, bool valid) {
-  const int n = valid ? 16 : 0;   // 0 source bytes: the 16 destination bytes are zero-filled
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+template <int D, int HEADS> struct Sync {
+  static constexpr int kStages = Geo<D, HEADS>::kStages;
+  uint64_t full[kStages];                  // the copies' arrivals and the scales' one
+  uint64_t empty[kStages];                 // the computing warps
+  float scale[kStages][2][kBlockKeys];     // of the keys: 2^e; of the values: e (NaN for a NaN scale)
+  float top[kStages];                      // the block's largest e of a value
+  int abort_flag;
+  float meet[2][Geo<D, HEADS>::kState][32];   // two warps' states on their way to another
+};
+template <int D, int HEADS> constexpr int smem_bytes() {
+  return Geo<D, HEADS>::kRingBytes + 1024 + static_cast<int>(sizeof(Sync<D, HEADS>));
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// One of the barrier's counted arrivals, when this thread's copies so far have landed.
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
 __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -59,15 +85,10 @@ __device__ __forceinline__ void ldsm_x4_trans(uint32_t addr, uint32_t (&r)[4]) {
                : "r"(addr));
 }
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ float ex2f(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 // (lo, hi) as an fp16 pair, and what the rounding left over as another.
 __device__ __forceinline__ void split_f16(float lo, float hi, uint32_t& head, uint32_t& rest) {
@@ -75,384 +96,644 @@ __device__ __forceinline__ void split_f16(float lo, float hi, uint32_t& head, ui
   const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&head));
   rest = pack16<false>(lo - h.x, hi - h.y);
 }
-__device__ __forceinline__ float quad_max(float x) {
-  x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-  return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-}
-__device__ __forceinline__ float quad_sum(float x) {
-  x += __shfl_xor_sync(0xffffffffu, x, 1);
-  return x + __shfl_xor_sync(0xffffffffu, x, 2);
+// The transpose of an 8 x 8 matrix of 16-bit elements: lane 4 i + j holds elements 2 j, 2 j + 1 of row i.
+__device__ __forceinline__ uint32_t turn8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 
-// HEADS: query heads of a CTA, 8 or 16.  ROWS = accumulator rows with a query head in them (g, and g + 8 of 16).
-template <int D, bool BF16, int HEADS>
-__global__ void __launch_bounds__(kThreads, HEADS == 8 ? 3 : 2)
-    decode_fp8_kernel(const Problem p, const CacheScales sc, const int chunk, const int nsplit, float* __restrict__ part_o,
-                      float* __restrict__ part_ml) {
-  using G = Geo<D>;
-  constexpr int KS = D / 16;            // k-steps of the first product
-  constexpr bool kTwo = HEADS == 16;    // rows g + 8 are heads too (else they carry the low parts of P)
-  extern __shared__ __align__(16) uint8_t smem[];
+// The list of blocks: for each sequence and unit (a kv head and a block of its query heads) the blocks of its keys.
+struct List {
+  const Problem& p;
+  const int units;
+  __device__ __forceinline__ int blocks(int b) const { return (valid_keys(p, b) + kBlockKeys - 1) / kBlockKeys; }
+};
 
-  const int split = blockIdx.z;   // slowest: the launch ends on the last (short or empty) chunks
-  const int hk = blockIdx.x % p.Hkv;
-  const int gsub = blockIdx.x / p.Hkv;
-  const int b = blockIdx.y;
-  pdl_wait();
-  const int n_keys = valid_keys(p, b);
-  const int s0 = split * chunk;
-  if (s0 >= n_keys && split != 0) return;   // split 0 still writes an (empty) partial
-  const int s1 = (s0 + chunk < n_keys) ? s0 + chunk : n_keys;
-  const int n_blocks = s1 > s0 ? (s1 - s0 + kBlockKeys - 1) / kBlockKeys : 0;
+// A place in the list and the number of blocks behind it that the CTA still has to do; every role walks on its own.
+struct Cursor {
+  int b, unit, blk;     // sequence, unit, block of the sequence
+  int n_keys, n_blk;    // of the sequence
+  int left;
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int g = lane >> 2, tq = lane & 3;
-  const int h0 = hk * p.group + gsub * HEADS;
-  const int n_heads = (p.group - gsub * HEADS) < HEADS ? (p.group - gsub * HEADS) : HEADS;
+  __device__ __forceinline__ void enter(const List& l) {
+    n_keys = valid_keys(l.p, b);
+    n_blk = (n_keys + kBlockKeys - 1) / kBlockKeys;
+  }
+  // The next block; `left` reaches 0 at the end of the range.
+  __device__ __forceinline__ void step(const List& l) {
+    if (--left <= 0) return;
+    if (++blk < n_blk) return;
+    next_pair(l);
+  }
+  // The first block of the next pair that has one.
+  __device__ __forceinline__ void next_pair(const List& l) {
+    blk = 0;
+    if (++unit < l.units) return;
+    unit = 0;
+    do {
+      ++b;
+      enter(l);
+    } while (n_blk == 0 && b + 1 < l.p.B);
+  }
+};
 
-  const uint8_t* kbase = static_cast<const uint8_t*>(p.k) + hk * p.ks[1];
-  const uint8_t* vbase = static_cast<const uint8_t*>(p.v) + hk * p.vs[1];
-  const int* table = p.block_table + static_cast<int64_t>(b) * p.table_stride;
+// The first place of this CTA's range.  Whole warp; lens are read 32 at a time, twice.
+__device__ __forceinline__ Cursor first_place(const List& l, int fixed_blocks, int lane) {
+  int64_t sum = 0;
+  for (int b0 = 0; b0 < l.p.B; b0 += 32) sum += __reduce_add_sync(0xffffffffu, b0 + lane < l.p.B ? l.blocks(b0 + lane) : 0);
+  const int64_t total = sum * l.units;
+  int64_t per = fixed_blocks;
+  if (per == 0) per = (total + gridDim.x - 1) / gridDim.x;
+  const int64_t start = blockIdx.x * per;
+  Cursor c = {0, 0, 0, 0, 0, 0};
+  if (start >= total) return c;
+  c.left = static_cast<int>(total - start < per ? total - start : per);
+  int64_t before = 0;
+  for (int b0 = 0; b0 < l.p.B; b0 += 32) {
+    const int mine = b0 + lane < l.p.B ? l.blocks(b0 + lane) : 0;
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const int x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
+    }
+    const unsigned here = __ballot_sync(0xffffffffu, start < (before + upto) * l.units);
+    if (here != 0u) {
+      const int at = __ffs(here) - 1;
+      c.b = b0 + at;
+      const int64_t off = start - (before + __shfl_sync(0xffffffffu, upto - mine, at)) * l.units;
+      c.enter(l);
+      c.unit = static_cast<int>(off / c.n_blk);
+      c.blk = static_cast<int>(off % c.n_blk);
+      return c;
+    }
+    before += __shfl_sync(0xffffffffu, upto, 31);
+  }
+  return c;   // (not reached: start < total)
+}
+
+// Table entry of a key position; -1 behind the end.  Looked at where it is used: a look here would wait for the load.
+__device__ __forceinline__ int entry_of(const Problem& p, const Cursor& c, int row) {
+  int page = -1;
+  if (c.left > 0 && row < c.n_keys) page = p.block_table[static_cast<int64_t>(c.b) * p.table_stride + (row >> p.page_shift)];
+  return page;
+}
+// A number outside the pool is reported, and page 0 read in its place.
+__device__ __forceinline__ int page_of(const Problem& p, const CacheScales& sc, const Cursor& c, int entry, int row) {
+  if (row >= c.n_keys) return -1;
+  if (static_cast<unsigned>(entry) < static_cast<unsigned>(sc.n_pages)) return entry;
+  report_page(p.status, B200_SDPA_ERR_PAGE, c.b, row, sc.n_pages);
+  return 0;
+}
+
+// The n-th block's stage is free: the warps that compute have read the block before it there.
+template <typename S>
+__device__ __forceinline__ bool wait_read(const Problem& p, S* sync, int n, int role, int lane, long long wait_limit) {
+  const int s = n % S::kStages, round = n / S::kStages;
+  if (round == 0) return true;
+  const bool ok = __all_sync(0xffffffffu, wait_clocked(smem_u32(&sync->empty[s]), (round - 1) & 1, &sync->abort_flag, wait_limit));
+  if (!ok && lane == 0) report(p.status, role, n, s);
+  return ok;
+}
+
+// The warp that brings the rows.  Lane l looks up the pages of keys l, l + 32, ... of a block, kStages blocks ahead.  TMA: pages of 8
+// rows or more, one tensor copy for each page and operand.  Smaller pages: 16-byte copies of single rows.
+template <int D, int HEADS, bool TMA>
+__device__ __forceinline__ void bring_rows(const List& l, const CacheScales& sc, const CUtensorMap* tm_k, const CUtensorMap* tm_v,
+                                           Sync<D, HEADS>* sync, uint32_t ring, Cursor c, int lane, long long wait_limit) {
+  using G = Geo<D, HEADS>;
+  constexpr int kStages = G::kStages, kLook = kBlockKeys / 32;
+  const Problem& p = l.p;
   const int page_mask = (1 << p.page_shift) - 1;
-  const uint32_t smem_base = smem_addr(smem);
-  float* scales = reinterpret_cast<float*>(smem + G::kRingBytes);
-
-  // Page of a key position of this chunk; -1 where there is none (behind the end, or a number outside the pool).
-  auto page_of = [&](int row) -> int {
-    if (row >= s1) return -1;
-    const int page = table[row >> p.page_shift];
-    if (static_cast<unsigned>(page) < static_cast<unsigned>(sc.n_pages)) return page;
-    report_page(p.status, B200_SDPA_ERR_PAGE, b, row, sc.n_pages);
-    return -1;
-  };
-  constexpr int kCopies = kBlockKeys * G::kChunksPerRow / kThreads;
-  int pages[kCopies];
-  auto fetch_pages = [&](int blk) {
+  int entries[kStages][kLook];
+  Cursor ahead = c;
+  auto look_up = [&](int (&e)[kLook]) {
 #pragma unroll
-    for (int i = 0; i < kCopies; ++i) pages[i] = page_of(s0 + blk * kBlockKeys + (tid + i * kThreads) / G::kChunksPerRow);
+    for (int i = 0; i < kLook; ++i) e[i] = entry_of(p, ahead, ahead.blk * kBlockKeys + lane + 32 * i);
+    ahead.step(l);
   };
-  auto load_block = [&](int blk) {
-    const uint32_t stage = smem_base + (blk % kStages) * G::kStageBytes;
-    const int key0 = s0 + blk * kBlockKeys;
 #pragma unroll
-    for (int i = 0; i < kCopies; ++i) {
-      const int c = tid + i * kThreads;
-      const int row = c / G::kChunksPerRow, ch = c % G::kChunksPerRow;
-      const bool ok = pages[i] >= 0;
-      const int64_t page = ok ? pages[i] : 0;
-      const int in_page = (key0 + row) & page_mask;
-      cp_async_16(stage + row * G::kRowBytes + ch * 16, kbase + page * p.ks[0] + in_page * p.ks[2] + ch * 16, ok);
-      cp_async_16(stage + G::kTileBytes + row * G::kRowBytes + ch * 16, vbase + page * p.vs[0] + in_page * p.vs[2] + ch * 16, ok);
-    }
-  };
-  // Thread t < 64 brings the key scale of key t of a block, thread 64 + t the value scale.
-  auto fetch_scale = [&](int blk) -> int {
-    const int key = s0 + blk * kBlockKeys + (tid & 63);
-    const int page = page_of(key);
-    if (page < 0) return -1;
-    const int64_t* ss = tid < 64 ? sc.ks : sc.vs;
-    return (tid < 64 ? sc.k : sc.v)[page * ss[0] + hk * ss[1] + (key & page_mask) * ss[2]];
-  };
-  // Keys: the scale itself.  Values: its exponent (NaN for a NaN scale; -inf where there is no key).
-  auto store_scale = [&](int blk, int code) {
-    float x;
-    if (tid < 64) x = code < 0 ? 0.f : scale_value(code);
-    else x = code < 0 ? -CUDART_INF_F : (code == 255 ? CUDART_NAN_F : static_cast<float>(code - 127));
-    scales[(blk & 1) * 2 * kBlockKeys + tid] = x;
-  };
-
-  if (n_blocks > 0) {
-    store_scale(0, fetch_scale(0));
+  for (int s = 0; s < kStages; ++s) look_up(entries[s]);
+  bool alive = true;
+  int n = 0;
+  while (c.left > 0 && alive) {
 #pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) {
-      if (i < n_blocks) {
-        fetch_pages(i);
-        load_block(i);
+    for (int s = 0; s < kStages; ++s) {
+      if (c.left <= 0 || !alive) break;
+      alive = wait_read(p, sync, n, 1, lane, wait_limit);
+      if (!alive) break;
+      const int hk = c.unit % p.Hkv;
+      const uint32_t stage = ring + s * G::kStageBytes, bar = smem_u32(&sync->full[s]);
+      const int key0 = c.blk * kBlockKeys;
+      if constexpr (TMA) {
+        const int rows = page_mask + 1 < kBlockKeys ? page_mask + 1 : kBlockKeys;   // of one copy
+        const int first = (lane >> 1) * rows;                  // lanes 2 i and 2 i + 1: keys and values of copy i
+        int entry = 0;
+#pragma unroll
+        for (int i = 0; i < kLook; ++i) {
+          const int e = __shfl_sync(0xffffffffu, entries[s][i], first & 31);
+          entry = (first >> 5) == i ? e : entry;
+        }
+        const int page = first < kBlockKeys ? page_of(p, sc, c, entry, key0 + first) : -1;
+        const bool mine = page >= 0;
+        const unsigned copies = __popc(__ballot_sync(0xffffffffu, mine));
+        if (lane == 0) mbar_arrive_expect_tx(bar, copies * rows * D);
+        __syncwarp();
+        if (mine)
+          tma_load_4d(stage + (lane & 1) * G::kTileBytes + first * D, (lane & 1) ? tm_v : tm_k, bar, 0, (key0 + first) & page_mask, hk, page);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kLook; ++i)
+#pragma unroll 4
+          for (int x = lane; x < 32 * G::kChunksPerRow; x += 32) {
+            const int row = 32 * i + x / G::kChunksPerRow, ch = x % G::kChunksPerRow;
+            const int64_t page = page_of(p, sc, c, __shfl_sync(0xffffffffu, entries[s][i], row & 31), key0 + row);
+            if (page < 0) continue;
+            const int in_page = (key0 + row) & page_mask;
+            const uint32_t dst = stage + row * D + ((ch ^ G::swizzle(row)) << 4);
+            cp_async_16(dst, static_cast<const uint8_t*>(p.k) + hk * p.ks[1] + page * p.ks[0] + in_page * p.ks[2] + ch * 16);
+            cp_async_16(dst + G::kTileBytes, static_cast<const uint8_t*>(p.v) + hk * p.vs[1] + page * p.vs[0] + in_page * p.vs[2] + ch * 16);
+          }
+        cp_async_arrive(bar);   // (every lane's copies; the barrier counts the 32 lanes)
       }
-      cp_async_commit();
+      ++n;
+      c.step(l);
+      look_up(entries[s]);
     }
-    if (kStages - 1 < n_blocks) fetch_pages(kStages - 1);
   }
-
-  // ---- query rows: through the last stage as fp16, scaled by a power of two
-  uint32_t qf[KS][kTwo ? 4 : 2];
-  float sl2[2];   // score to exp2 units, of rows g and g + 8
-  {
-    const uint16_t* q16 = reinterpret_cast<const uint16_t*>(p.q) + b * p.qs[0];
-    constexpr int kPitch = 2 * D + 16;
-    uint8_t* stage = smem + (kStages - 1) * G::kStageBytes;
-    float* q_scale = reinterpret_cast<float*>(stage + HEADS * kPitch);
-    static_assert(HEADS * kPitch + HEADS * 4 <= G::kStageBytes, "the query rows fit in a stage");
-    for (int row = warp; row < HEADS; row += kWarps) {
-      float x[D / 32];
-      uint32_t top = 0;
-#pragma unroll
-      for (int i = 0; i < D / 32; ++i) {
-        x[i] = row < n_heads ? half_to_f32<BF16>(q16[(h0 + row) * p.qs[1] + (lane + 32 * i) * p.qs[3]]) : 0.f;
-        const uint32_t m = __float_as_uint(x[i]) & 0x7fffffffu;
-        top = m > top ? m : top;
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        const uint32_t m = __shfl_xor_sync(0xffffffffu, top, o);
-        top = m > top ? m : top;
-      }
-      // largest element into [2^14, 2^15); zeros, infinities and NaN stay as they are
-      int up = top == 0u || top >= 0x7f800000u ? 0 : 127 + 14 - static_cast<int>(top >> 23);
-      if (!BF16 && up < 0) up = 0;
-      if (up > 126) up = 126;
-      const float f = __int_as_float((127 + up) << 23);   // up >= -113
-#pragma unroll
-      for (int i = 0; i < D / 32; ++i)
-        *reinterpret_cast<__half*>(stage + row * kPitch + (lane + 32 * i) * 2) = __float2half_rn(x[i] * f);
-      if (lane == 0) q_scale[row] = p.scale * kLog2e * __int_as_float((127 - up) << 23);
-    }
-    __syncthreads();
-    // k-step s of a fragment: elements 16 s + 4 tq .. + 3 of a row, as the bytes of a key's fragment word
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      const uint2 lo = *reinterpret_cast<const uint2*>(stage + g * kPitch + (16 * s + 4 * tq) * 2);
-      qf[s][0] = lo.x;
-      qf[s][1] = lo.y;
-      if constexpr (kTwo) {
-        const uint2 hi = *reinterpret_cast<const uint2*>(stage + (g + 8) * kPitch + (16 * s + 4 * tq) * 2);
-        qf[s][2] = hi.x;
-        qf[s][3] = hi.y;
-      }
-    }
-    sl2[0] = q_scale[g];
-    sl2[1] = kTwo ? q_scale[g + 8] : 0.f;
-    __syncthreads();
+  if (*static_cast<volatile int*>(&sync->abort_flag) != 0 && lane == 0) {
+    // what was issued has to land before the CTA lets go of its memory
+    for (int s = 0; s < kStages && s < n; ++s) wait_drain(smem_u32(&sync->full[s]), ((n - 1 - s) / kStages) & 1);
   }
+}
 
-  constexpr int kRows = kTwo ? 2 : 1;
-  float o_acc[D / 8][4];   // block 2 j: columns 16 j + 4 tq, + 2; block 2 j + 1: + 1, + 3
+// The warp that brings the scales of a block's keys l, l + 32, ... and of their values, asked for a block ahead.
+template <int D, int HEADS>
+__device__ __forceinline__ void bring_scales(const List& l, const CacheScales& sc, Sync<D, HEADS>* sync, Cursor c, int lane,
+                                             long long wait_limit) {
+  constexpr int kStages = Geo<D, HEADS>::kStages, kLook = kBlockKeys / 32;
+  const Problem& p = l.p;
+  const int page_mask = (1 << p.page_shift) - 1;
+  int entries[kLook], codes[2][kLook];   // of the block after the next, of the next; codes: -1 where there is no key
+  Cursor next = c, ahead = c;
+  auto look_up = [&]() {
 #pragma unroll
-  for (int n = 0; n < D / 8; ++n)
+    for (int i = 0; i < kLook; ++i) entries[i] = entry_of(p, ahead, ahead.blk * kBlockKeys + lane + 32 * i);
+    ahead.step(l);
+  };
+  auto ask = [&]() {
+    const int hk = next.unit % p.Hkv;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) o_acc[n][r] = 0.f;
-  float m[kRows], l[kRows], r_exp = -CUDART_INF_F;
+    for (int i = 0; i < kLook; ++i) {
+      codes[0][i] = codes[1][i] = -1;
+      if (next.left <= 0) continue;
+      const int row = next.blk * kBlockKeys + lane + 32 * i;
+      const int64_t page = page_of(p, sc, next, entries[i], row);
+      if (page < 0) continue;
+      codes[0][i] = sc.k[page * sc.ks[0] + hk * sc.ks[1] + (row & page_mask) * sc.ks[2]];
+      codes[1][i] = sc.v[page * sc.vs[0] + hk * sc.vs[1] + (row & page_mask) * sc.vs[2]];
+    }
+    next.step(l);
+  };
+  look_up();
+  ask();
+  look_up();
+  for (int n = 0; n < c.left; ++n) {
+    const int s = n % kStages;
+    if (!wait_read(p, sync, n, 3, lane, wait_limit)) break;
+    int top = -1;
 #pragma unroll
-  for (int r = 0; r < kRows; ++r) {
-    m[r] = -CUDART_INF_F;
-    l[r] = 0.f;
+    for (int i = 0; i < kLook; ++i) {
+      sync->scale[s][0][lane + 32 * i] = codes[0][i] < 0 ? 0.f : scale_value(codes[0][i]);
+      const int x = codes[1][i];
+      sync->scale[s][1][lane + 32 * i] = x < 0 ? -CUDART_INF_F : (x == 255 ? CUDART_NAN_F : static_cast<float>(x - 127));
+      if (x < 255 && x > top) top = x;
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (lane == 0) sync->top[s] = top < 0 ? -CUDART_INF_F : static_cast<float>(top - 127);
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&sync->full[s]));
+    ask();
+    look_up();
   }
+}
 
-  for (int blk = 0; blk < n_blocks; ++blk) {
-    if (blk + kStages - 1 < n_blocks) load_block(blk + kStages - 1);
-    cp_async_commit();
-    if (blk + kStages < n_blocks) fetch_pages(blk + kStages);
-    const int next_scale = blk + 1 < n_blocks ? fetch_scale(blk + 1) : -1;
-    cp_async_wait<kStages - 1>();
-    __syncthreads();
+// The state of a warp for one pair.  Lane 4 g + tq: heads 2 tq, 2 tq + 1 of every eight; o: rows 16 j + 2 g, + 1 of O^T.
+template <int D, int NB> struct State {
+  float o[D / 16][NB][4];
+  float m[NB][2], l[NB][2];   // maximum of the raw scores (for `merge`: in log2 units), this lane's share of the sum
 
-    const uint32_t kt = smem_base + (blk % kStages) * G::kStageBytes;
-    const uint32_t vt = kt + G::kTileBytes;
-    const int key_w = s0 + blk * kBlockKeys + warp * 16;   // first key of this warp's 16
-    if (key_w < s1) {
-      const float* ksc = scales + (blk & 1) * 2 * kBlockKeys + warp * 16;
-      const float* vsc = ksc + kBlockKeys;
-      // ---- S = Q K^T for 16 keys: two n-blocks of 8 keys
-      float sv[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-      {
-        // matrices = (keys 0-7, bytes 0-15), (keys 8-15, 0-15), (keys 0-7, 16-31), (keys 8-15, 16-31)
-        const uint32_t a0 = kt + (warp * 16 + ((lane >> 3) & 1) * 8 + (lane & 7)) * G::kRowBytes + (lane >> 4) * 16;
+  __device__ __forceinline__ void put(float (*to)[32], int lane) const {
+    int i = 0;
 #pragma unroll
-        for (int s = 0; s < KS; s += 2) {
-          uint32_t kf[4];
-          ldsm_x4(a0 + s * 16, kf);
+    for (int j = 0; j < D / 16; ++j)
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            uint32_t b0, b1;
-            unpack_e4m3_f16(kf[u], b0, b1);
-            const int ks = s + (u >> 1);
-            mma_f16(sv[u & 1], qf[ks][0], kTwo ? qf[ks][kTwo ? 2 : 0] : 0u, qf[ks][1], kTwo ? qf[ks][kTwo ? 3 : 0] : 0u, b0, b1);
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) to[i++][lane] = o[j][n][r];
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        to[i++][lane] = m[n][e];
+        to[i++][lane] = l[n][e];
+      }
+  }
+  __device__ __forceinline__ void merge(const float (*from)[32], int lane) {
+    float mine[NB][2], theirs[NB][2];
+    int i = D / 4 * NB;
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float om = from[i++][lane], ol = from[i++][lane];
+        const float mx = fmaxf(m[n][e], om), ref = mx == -CUDART_INF_F ? 0.f : mx;
+        mine[n][e] = ex2(m[n][e] - ref);
+        theirs[n][e] = ex2(om - ref);
+        m[n][e] = mx;
+        l[n][e] = fmaf(l[n][e], mine[n][e], ol * theirs[n][e]);
+      }
+    i = 0;
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[j][n][r] = fmaf(o[j][n][r], mine[n][r & 1], from[i++][lane] * theirs[n][r & 1]);
+  }
+};
+
+__device__ __forceinline__ void computing_warps_meet() { asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory"); }
+
+// HEADS: query heads of a CTA, 8 or 16.
+template <int D, bool BF16, int HEADS, bool TMA>
+__global__ void __launch_bounds__(kThreads, Geo<D, HEADS>::kCtas)
+    decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const Problem p, const CacheScales sc,
+                      const OwnPartials part, const int fixed_blocks, const long long wait_limit) {
+  using G = Geo<D, HEADS>;
+  constexpr int KS = D / 16, NB = HEADS / 8;
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw), ring = (raw + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (ring - raw);
+  auto* sync = reinterpret_cast<Sync<D, HEADS>*>(smem + G::kRingBytes);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int s = 0; s < G::kStages; ++s) {
+      mbar_init(smem_u32(&sync->full[s]), TMA ? 2 : 33);
+      mbar_init(smem_u32(&sync->empty[s]), kWarps);
+    }
+    sync->abort_flag = 0;
+    mbar_fence_init();
+  }
+  __syncthreads();
+  pdl_wait();
+  const List list = {p, p.Hkv * ((p.group + HEADS - 1) / HEADS)};
+  Cursor c = first_place(list, fixed_blocks, lane);
+
+  if (warp == kWarps) {
+    bring_rows<D, HEADS, TMA>(list, sc, &tm_k, &tm_v, sync, ring, c, lane, wait_limit);
+  } else if (warp == kWarps + 1) {
+    bring_scales<D, HEADS>(list, sc, sync, c, lane, wait_limit);
+  } else {
+    const int g = lane >> 2, tq = lane & 3;
+    bool ok = true;
+    int n = 0;   // blocks so far
+    while (c.left > 0) {
+      // ---- one pair: `todo` blocks of it
+      const int b = c.b, gsub = c.unit / p.Hkv, hk = c.unit % p.Hkv;
+      const int h0 = hk * p.group + gsub * HEADS;
+      const int n_heads = (p.group - gsub * HEADS) < HEADS ? (p.group - gsub * HEADS) : HEADS;
+      const int first = c.blk, todo = c.n_blk - c.blk < c.left ? c.n_blk - c.blk : c.left, n_keys = c.n_keys;
+      const int64_t pair = static_cast<int64_t>(b) * list.units + c.unit, slot = pair + blockIdx.x;
+      if (tid == 0) {
+        if (first == 0) part.range[pair].x = static_cast<int>(slot);
+        if (first + todo == c.n_blk) part.range[pair].y = static_cast<int>(slot);
+      }
+      // query fragments: k-step s holds elements 16 s + 4 tq .. + 3 of head g, as the bytes of a key's fragment word; a head's
+      // quad has all of it
+      uint32_t qf[NB][KS][2];
+      float sl2[NB][2];   // score to exp2 units, of heads 2 tq, 2 tq + 1
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const int head = 8 * i + g;
+        const uint16_t* q16 = reinterpret_cast<const uint16_t*>(p.q) + b * p.qs[0] + (h0 + (head < n_heads ? head : 0)) * p.qs[1];
+        const bool vec = p.qs[3] == 1 && reinterpret_cast<uintptr_t>(q16) % 8 == 0;
+        uint2 x[KS];
+        uint32_t top = 0;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          const int at = 16 * s + 4 * tq;
+          if (vec) {
+            x[s] = *reinterpret_cast<const uint2*>(q16 + at);
+          } else {
+            x[s].x = q16[at * p.qs[3]] | static_cast<uint32_t>(q16[(at + 1) * p.qs[3]]) << 16;
+            x[s].y = q16[(at + 2) * p.qs[3]] | static_cast<uint32_t>(q16[(at + 3) * p.qs[3]]) << 16;
           }
         }
-      }
-      float kx[2][2], ev[2][2];
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        *reinterpret_cast<float2*>(kx[n]) = *reinterpret_cast<const float2*>(ksc + n * 8 + tq * 2);
-        *reinterpret_cast<float2*>(ev[n]) = *reinterpret_cast<const float2*>(vsc + n * 8 + tq * 2);
-      }
-      const bool tail = key_w + 16 > s1;
+        for (int s = 0; s < KS; ++s)   // (magnitudes of either type order like their bits)
+          top = max(max(top, max(x[s].x & 0x7fffu, (x[s].x >> 16) & 0x7fffu)), max(x[s].y & 0x7fffu, (x[s].y >> 16) & 0x7fffu));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        top = __float_as_uint(half_to_f32<BF16>(static_cast<uint16_t>(top)));
+        // largest element into [2^14, 2^15); zeros, infinities and NaN stay as they are
+        int up = top == 0u || top >= 0x7f800000u ? 0 : 127 + 14 - static_cast<int>(top >> 23);
+        if (!BF16 && up < 0) up = 0;
+        if (up > 126) up = 126;
+        const float f = __int_as_float((127 + up) << 23);   // up >= -113
+        const float mine = p.scale * kLog2e * __int_as_float((127 - up) << 23);
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+        for (int e = 0; e < 2; ++e) sl2[i][e] = __shfl_sync(0xffffffffu, mine, (2 * tq + e) * 4);
 #pragma unroll
-        for (int r = 0; r < 2 * kRows; ++r) {
-          sv[n][r] *= kx[n][r & 1];
-          if (tail && key_w + n * 8 + tq * 2 + (r & 1) >= s1) sv[n][r] = -CUDART_INF_F;
-        }
-      // ---- the largest value exponent, and the row maxima; o is rescaled when either reference grows
-      const float e_top = quad_max(fmaxf(fmaxf(ev[0][0], ev[0][1]), fmaxf(ev[1][0], ev[1][1])));
-      float mn[kRows];
-      bool grow = e_top > r_exp;
-#pragma unroll
-      for (int r = 0; r < kRows; ++r) {
-        mn[r] = fmaxf(m[r], quad_max(fmaxf(fmaxf(sv[0][2 * r], sv[0][2 * r + 1]), fmaxf(sv[1][2 * r], sv[1][2 * r + 1]))));
-        grow |= (mn[r] - m[r]) * sl2[r] > kRescaleThreshold;
-      }
-      if (__any_sync(0xffffffffu, grow)) {
-        const float re = fmaxf(r_exp, e_top);
-        const float down = re == r_exp ? 1.f : ex2f(r_exp - re);   // -inf -> 0
-        r_exp = re;
-        float a[2];
-#pragma unroll
-        for (int r = 0; r < kRows; ++r) {
-          a[r] = mn[r] == m[r] ? 1.f : ex2f((m[r] - mn[r]) * sl2[r]);
-          m[r] = mn[r];
-          l[r] *= a[r];
-          a[r] *= down;
-        }
-        if (!kTwo) a[1] = a[0];
-#pragma unroll
-        for (int n = 0; n < D / 8; ++n) {
-          o_acc[n][0] *= a[0];
-          o_acc[n][1] *= a[0];
-          o_acc[n][2] *= a[1];
-          o_acc[n][3] *= a[1];
+        for (int s = 0; s < KS; ++s) {
+          const float e0 = half_to_f32<BF16>(static_cast<uint16_t>(x[s].x)), e1 = half_to_f32<BF16>(static_cast<uint16_t>(x[s].x >> 16));
+          const float e2 = half_to_f32<BF16>(static_cast<uint16_t>(x[s].y)), e3 = half_to_f32<BF16>(static_cast<uint16_t>(x[s].y >> 16));
+          qf[i][s][0] = head < n_heads ? pack16<false>(e0 * f, e1 * f) : 0u;
+          qf[i][s][1] = head < n_heads ? pack16<false>(e2 * f, e3 * f) : 0u;
         }
       }
-      // ---- probabilities, times the value scale relative to r
-      float w[2][2];
+      State<D, NB> a;
+      float r_exp = -CUDART_INF_F;
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int i = 0; i < NB; ++i) {
 #pragma unroll
-        for (int e = 0; e < 2; ++e) w[n][e] = ev[n][e] == -CUDART_INF_F ? 0.f : ex2f(ev[n][e] - r_exp + kProbShift);
-      uint32_t ph[kRows][2], pl[kRows][2];   // [row][n-block]: hi and lo parts of two keys
+        for (int j = 0; j < D / 16; ++j)
 #pragma unroll
-      for (int r = 0; r < kRows; ++r) {
-        const float nm = (m[r] == -CUDART_INF_F) ? 0.f : -m[r] * sl2[r];
-        float sum = 0.f;
+          for (int r = 0; r < 4; ++r) a.o[j][i][r] = 0.f;
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const float p0 = ex2f(fmaf(sv[n][2 * r], sl2[r], nm)), p1 = ex2f(fmaf(sv[n][2 * r + 1], sl2[r], nm));
-          sum += p0 + p1;
-          split_f16(p0 * w[n][0], p1 * w[n][1], ph[r][n], pl[r][n]);
+        for (int e = 0; e < 2; ++e) {
+          a.m[i][e] = -CUDART_INF_F;
+          a.l[i][e] = 0.f;
         }
-        l[r] += sum;
       }
-      // ---- O += P V: sixteen columns at a time
-      {
-        // matrices = (keys 0-7, bytes 0-15), (keys 8-15, 0-15), (keys 0-7, 16-31), (keys 8-15, 16-31), transposed
-        const uint32_t v0 = vt + (warp * 16 + ((lane >> 3) & 1) * 8 + (lane & 7)) * G::kRowBytes + (lane >> 4) * 16;
+
+      for (int blk = first; blk < first + todo; ++blk, ++n) {
+        const int st = n % G::kStages;
+        ok = ok && wait_clocked(smem_u32(&sync->full[st]), (n / G::kStages) & 1, &sync->abort_flag, wait_limit);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) {   // (the CTA gives up: what is merged and stored from here on means nothing)
+          if (lane == 0) report(p.status, 2, n, warp);
+          continue;
+        }
+        const int key_w = blk * kBlockKeys + warp * kWarpKeys;   // first key of this warp's 32
+        if (key_w < n_keys) {
+          // the rows in matrices of 8 rows x 16 bytes: rows 0-7 and 8-15 of one piece, then of the next
+          const int row = warp * kWarpKeys + ((lane >> 3) & 1) * 8 + (lane & 7);
+          const uint32_t k_row = ring + st * G::kStageBytes + row * D, v_row = k_row + G::kTileBytes;
+          auto piece = [&](int x) { return static_cast<uint32_t>(((x + (lane >> 4)) ^ G::swizzle(lane & 7)) << 4); };
+          float kx[2][2], ev[2][2];
+          uint32_t kf[2][KS / 2][4];
 #pragma unroll
-        for (int j = 0; j < D / 32; ++j) {
-          uint32_t vf[4];
-          ldsm_x4_trans(v0 + j * 32, vf);
+          for (int t = 0; t < 2; ++t) {
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            uint32_t even0, odd0, even1, odd1;   // keys 0-7 and 8-15 of an even and an odd column
-            unpack_e4m3_f16(__byte_perm(vf[2 * u], 0, 0x3120), even0, odd0);
-            unpack_e4m3_f16(__byte_perm(vf[2 * u + 1], 0, 0x3120), even1, odd1);
-            float(&oe)[4] = o_acc[4 * j + 2 * u];
-            float(&oo)[4] = o_acc[4 * j + 2 * u + 1];
-            if constexpr (kTwo) {
-              mma_f16(oe, ph[0][0], ph[kRows - 1][0], ph[0][1], ph[kRows - 1][1], even0, even1);
-              mma_f16(oo, ph[0][0], ph[kRows - 1][0], ph[0][1], ph[kRows - 1][1], odd0, odd1);
-              mma_f16(oe, pl[0][0], pl[kRows - 1][0], pl[0][1], pl[kRows - 1][1], even0, even1);
-              mma_f16(oo, pl[0][0], pl[kRows - 1][0], pl[0][1], pl[kRows - 1][1], odd0, odd1);
-            } else {
-              mma_f16(oe, ph[0][0], pl[0][0], ph[0][1], pl[0][1], even0, even1);
-              mma_f16(oo, ph[0][0], pl[0][0], ph[0][1], pl[0][1], odd0, odd1);
+            for (int s = 0; s < KS; s += 2) ldsm_x4(k_row + t * 16 * D + piece(s), kf[t][s / 2]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              kx[t][i] = sync->scale[st][0][warp * kWarpKeys + 16 * t + g + 8 * i];
+              ev[t][i] = sync->scale[st][1][warp * kWarpKeys + 16 * t + g + 8 * i];
             }
           }
+          const float e_top = sync->top[st];
+          const bool tail = key_w + kWarpKeys > n_keys;
+          if (tail) {
+            // what lies behind the end is anything: its weight is 0, and 0 times a NaN is not
+            for (int i = lane; i < kWarpKeys * G::kChunksPerRow; i += 32)
+              if (key_w + i / G::kChunksPerRow >= n_keys)
+                *reinterpret_cast<uint4*>(smem + st * G::kStageBytes + G::kTileBytes + warp * kWarpKeys * D + i * 16) = make_uint4(0, 0, 0, 0);
+            fence_proxy_async_smem();   // (the stage's next block comes by tensor copies)
+            __syncwarp();
+          }
+          // ---- S^T = K Q^T: keys 16 t + g, + 8 x heads 2 tq, 2 tq + 1
+          constexpr int kChains = NB == 1 ? 2 : 1;   // even and odd k-steps apart
+          float sv[2][NB][4], part_s[2][NB][kChains][4];
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+#pragma unroll
+              for (int x = 0; x < kChains; ++x)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) part_s[t][i][x][r] = 0.f;
+#pragma unroll
+          for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              uint32_t a0, a1, a2, a3;
+              unpack_e4m3_f16(kf[t][s / 2][2 * (s & 1)], a0, a2);
+              unpack_e4m3_f16(kf[t][s / 2][2 * (s & 1) + 1], a1, a3);
+#pragma unroll
+              for (int i = 0; i < NB; ++i) mma_f16(part_s[t][i][s % kChains], a0, a1, a2, a3, qf[i][s][0], qf[i][s][1]);
+            }
+          float mn[NB][2];
+          bool grow = e_top > r_exp;
+#pragma unroll
+          for (int i = 0; i < NB; ++i) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) {
+                sv[t][i][r] = (kChains == 2 ? part_s[t][i][0][r] + part_s[t][i][kChains - 1][r] : part_s[t][i][0][r]) * kx[t][r >> 1];
+                if (tail && key_w + 16 * t + g + 8 * (r >> 1) >= n_keys) sv[t][i][r] = -CUDART_INF_F;
+              }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float x = fmaxf(fmaxf(sv[0][i][e], sv[0][i][2 + e]), fmaxf(sv[1][i][e], sv[1][i][2 + e]));
+#pragma unroll
+              for (int o = 4; o < 32; o *= 2) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+              mn[i][e] = fmaxf(a.m[i][e], x);
+              grow |= (mn[i][e] - a.m[i][e]) * sl2[i][e] > kRescaleThreshold;
+            }
+          }
+          // ---- o is rescaled when the largest value exponent or a row maximum grows
+          if (__any_sync(0xffffffffu, grow)) {
+            const float re = fmaxf(r_exp, e_top);
+            const float down = re == r_exp ? 1.f : ex2(r_exp - re);   // -inf -> 0
+            r_exp = re;
+#pragma unroll
+            for (int i = 0; i < NB; ++i) {
+              float f[2];
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                f[e] = mn[i][e] == a.m[i][e] ? 1.f : ex2((a.m[i][e] - mn[i][e]) * sl2[i][e]);
+                a.m[i][e] = mn[i][e];
+                a.l[i][e] *= f[e];
+                f[e] *= down;
+              }
+#pragma unroll
+              for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) a.o[j][i][r] *= f[r & 1];
+            }
+          }
+          // ---- probabilities; times the value scale relative to r, hi and lo, turned round: heads g x keys 2 tq, 2 tq + 1
+          uint32_t ph[2][NB][2], pl[2][NB][2];
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            float w[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) w[i] = ev[t][i] == -CUDART_INF_F ? 0.f : ex2(ev[t][i] - r_exp + kProbShift);
+#pragma unroll
+            for (int i = 0; i < NB; ++i) {
+              float x[4];
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const float nm = (a.m[i][e] == -CUDART_INF_F) ? 0.f : -a.m[i][e] * sl2[i][e];
+                x[e] = ex2(fmaf(sv[t][i][e], sl2[i][e], nm));
+                x[2 + e] = ex2(fmaf(sv[t][i][2 + e], sl2[i][e], nm));
+                a.l[i][e] += x[e] + x[2 + e];
+              }
+#pragma unroll
+              for (int y = 0; y < 2; ++y) {
+                split_f16(x[2 * y] * w[y], x[2 * y + 1] * w[y], ph[t][i][y], pl[t][i][y]);
+                ph[t][i][y] = turn8x8(ph[t][i][y]);
+                pl[t][i][y] = turn8x8(pl[t][i][y]);
+              }
+            }
+          }
+          // ---- O^T += V^T P^T, sixteen columns of V at a time
+#pragma unroll
+          for (int j = 0; j < D / 16; j += 2)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              uint32_t vf[4];
+              ldsm_x4_trans(v_row + t * 16 * D + piece(j), vf);
+#pragma unroll
+              for (int u = 0; u < 2; ++u) {
+                uint32_t a0, a1, a2, a3;   // even and odd columns of keys 0-7, then of keys 8-15
+                unpack_e4m3_f16(__byte_perm(vf[2 * u], 0, 0x3120), a0, a1);
+                unpack_e4m3_f16(__byte_perm(vf[2 * u + 1], 0, 0x3120), a2, a3);
+#pragma unroll
+                for (int i = 0; i < NB; ++i) {
+                  mma_f16(a.o[j + u][i], a0, a1, a2, a3, ph[t][i][0], ph[t][i][1]);
+                  mma_f16(a.o[j + u][i], a0, a1, a2, a3, pl[t][i][0], pl[t][i][1]);
+                }
+              }
+            }
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sync->empty[st]));
       }
-    }
-    store_scale(blk + 1, next_scale);   // the other parity
-    __syncthreads();   // the stage may be refilled, and the scales read, from here on
-  }
-  cp_async_wait<0>();
-  pdl_launch_dependents();
 
-  // ---- the four warps' states meet in shared memory
-  float* sm_o = reinterpret_cast<float*>(smem);               // [warp][HEADS][D]
-  float* sm_ml = sm_o + kWarps * HEADS * D;                   // [warp][HEADS][2] (max in log2 units, sum)
-  static_assert(kWarps * HEADS * (D + 2) * 4 <= G::kSmemBytes, "merge buffer must fit");
-  __syncthreads();
-  const float back = r_exp == -CUDART_INF_F ? 0.f : ex2f(0.5f * (r_exp - kProbShift));   // 2^(r - 9), in two factors
+      // ---- the four warps' states meet: 2 and 3 with 0 and 1, then 1 with 0, which stores
+      const float back = r_exp == -CUDART_INF_F ? 0.f : ex2(0.5f * (r_exp - kProbShift));   // 2^(r - 9), in two factors
 #pragma unroll
-  for (int j = 0; j < D / 16; ++j) {
-    float(&oe)[4] = o_acc[2 * j];
-    float(&oo)[4] = o_acc[2 * j + 1];
-    if constexpr (!kTwo) {
+      for (int i = 0; i < NB; ++i) {
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        oe[r] += oe[r + 2];
-        oo[r] += oo[r + 2];
+        for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) a.o[j][i][r] *= back * back;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) a.m[i][e] = a.m[i][e] == -CUDART_INF_F ? -CUDART_INF_F : a.m[i][e] * sl2[i][e];
       }
-    }
+      if (warp >= 2) a.put(sync->meet[warp - 2], lane);
+      computing_warps_meet();
+      if (warp < 2) a.merge(sync->meet[warp], lane);
+      if (warp == 1) {
+        __syncwarp();
+        a.put(sync->meet[1], lane);
+      }
+      computing_warps_meet();
+      if (warp == 0) {
+        a.merge(sync->meet[1], lane);
 #pragma unroll
-    for (int r = 0; r < kRows; ++r)
-      *reinterpret_cast<float4*>(&sm_o[(warp * HEADS + g + 8 * r) * D + j * 16 + tq * 4]) =
-          make_float4(oe[2 * r] * back * back, oo[2 * r] * back * back, oe[2 * r + 1] * back * back, oo[2 * r + 1] * back * back);
-  }
+        for (int i = 0; i < NB; ++i)
 #pragma unroll
-  for (int r = 0; r < kRows; ++r) {
-    const float sum = quad_sum(l[r]);
-    if (tq == 0) {
-      sm_ml[(warp * HEADS + g + 8 * r) * 2] = m[r] == -CUDART_INF_F ? -CUDART_INF_F : m[r] * sl2[r];
-      sm_ml[(warp * HEADS + g + 8 * r) * 2 + 1] = sum;
-    }
-  }
-  __syncthreads();
-  for (int idx = tid; idx < n_heads * D; idx += kThreads) {
-    const int row = idx / D, d = idx - row * D;
-    float mx = -CUDART_INF_F;
+          for (int e = 0; e < 2; ++e) {
+            float sum = a.l[i][e];
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, sm_ml[(w * HEADS + row) * 2]);
-    const float ms = (mx == -CUDART_INF_F) ? 0.f : mx;
-    float o = 0.f, lsum = 0.f;
+            for (int o = 4; o < 32; o *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            const int head = 8 * i + 2 * tq + e;
+            if (head >= n_heads || !dbg_range(p.status, DBG_DECODE_FP8 * 100 + 1, slot, 1, part.slots)) continue;
+            float* to = part.o + (slot * HEADS + head) * D;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      const float wgt = ex2f(sm_ml[(w * HEADS + row) * 2] - ms);
-      o = fmaf(sm_o[(w * HEADS + row) * D + d], wgt, o);
-      lsum = fmaf(sm_ml[(w * HEADS + row) * 2 + 1], wgt, lsum);
-    }
-    const int64_t slot = (static_cast<int64_t>(b) * p.Hq + (h0 + row)) * nsplit + split;
-    if (!dbg_range(p.status, DBG_DECODE_FP8 * 100 + 1, slot, 1, static_cast<int64_t>(p.B) * p.Hq * nsplit) ||
-        !dbg_range(p.status, DBG_DECODE_FP8 * 100 + 2, h0 + row, 1, p.Hq))
-      continue;
-    part_o[slot * D + d] = o;
-    if (d == 0) {
-      part_ml[slot * 2] = mx;
-      part_ml[slot * 2 + 1] = lsum;
+            for (int j = 0; j < D / 16; ++j) *reinterpret_cast<float2*>(to + 16 * j + 2 * g) = make_float2(a.o[j][i][e], a.o[j][i][2 + e]);
+            if (g == 0) *reinterpret_cast<float2*>(part.ml + (slot * HEADS + head) * 2) = make_float2(a.m[i][e], sum);
+          }
+      }
+      computing_warps_meet();   // (the next pair's states go where warp 0 has just read)
+      // on to the next pair
+      c.left -= todo;
+      if (c.left > 0) c.next_pair(list);
     }
   }
+  pdl_launch_dependents();
+  __syncthreads();   // (the warp that brings rows leaves last when the CTA gave up: the ring is its copies' until they have landed)
 }
 
-template <int D, bool BF16, int HEADS>
-int launch_one(const Problem& p, const CacheScales& sc, int chunk, int nsplit, float* po, float* pml, cudaStream_t stream) {
-  using G = Geo<D>;
-  auto kern = decode_fp8_kernel<D, BF16, HEADS>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, G::kSmemBytes) != cudaSuccess) {
+// Pages of the pool as (bytes of a row, rows, heads, pages); one copy takes up to a block's rows of a page.
+bool make_page_map(CUtensorMap* map, const void* pool, int d, int page, int heads, int pages, const int64_t* stride) {
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) return false;
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(d), static_cast<cuuint64_t>(page), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(pages)};
+  auto fix = [&](int64_t s, int n) -> cuuint64_t { return static_cast<cuuint64_t>(n == 1 ? d : s); };   // (never stepped)
+  const cuuint64_t strides[3] = {fix(stride[2], page), fix(stride[1], heads), fix(stride[0], pages)};
+  const cuuint32_t box[4] = {static_cast<cuuint32_t>(d), static_cast<cuuint32_t>(page < kBlockKeys ? page : kBlockKeys), 1, 1};
+  const cuuint32_t elem[4] = {1, 1, 1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(pool), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            d == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// A tensor copy wants positive strides below 2^40 (the rows are on 16 bytes already) and whole swizzle patterns: 8 rows.
+bool tma_pages(const Problem& p, int pages) {
+  const int page = 1 << p.page_shift, n[3] = {pages, p.Hkv, page};
+  if (page < 8) return false;
+  for (int i = 0; i < 3; ++i)
+    if (n[i] > 1 && (p.ks[i] <= 0 || p.vs[i] <= 0 || p.ks[i] >= (1LL << 40) || p.vs[i] >= (1LL << 40))) return false;
+  return true;
+}
+
+template <int D, bool BF16, int HEADS, bool TMA>
+int launch_one(const Problem& p, const CacheScales& sc, const Fp8Geometry& g, const OwnPartials& part, cudaStream_t stream) {
+  CUtensorMap tk = {}, tv = {};
+  if (TMA && (!make_page_map(&tk, p.k, D, 1 << p.page_shift, p.Hkv, sc.n_pages, p.ks) ||
+              !make_page_map(&tv, p.v, D, 1 << p.page_shift, p.Hkv, sc.n_pages, p.vs)))
+    return B200_SDPA_ERR_CUDA;
+  auto kern = decode_fp8_kernel<D, BF16, HEADS, TMA>;
+  constexpr int smem = smem_bytes<D, HEADS>();
+  static_assert(Geo<D, HEADS>::kCtas * (smem + 1024) <= 228 * 1024, "the CTAs of an SM share its memory");
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
     cudaGetLastError();
     return B200_SDPA_ERR_CUDA;
   }
-  dim3 grid(p.Hkv * ((p.group + HEADS - 1) / HEADS), p.B, nsplit);
-  if (!launch_pdl(kern, grid, kThreads, G::kSmemBytes, stream, p, sc, chunk, nsplit, po, pml)) return B200_SDPA_ERR_CUDA;
+  if (!launch_pdl(kern, dim3(g.grid), kThreads, smem, stream, tk, tv, p, sc, part, g.fixed_blocks, wait_limit_cycles())) return B200_SDPA_ERR_CUDA;
   count_launch(KID_DECODE);
   return B200_SDPA_OK;
 }
 
 template <int D, bool BF16>
-int launch_heads(const Problem& p, const CacheScales& sc, int chunk, int nsplit, float* po, float* pml, cudaStream_t stream) {
-  return p.group <= 8 ? launch_one<D, BF16, 8>(p, sc, chunk, nsplit, po, pml, stream)
-                      : launch_one<D, BF16, 16>(p, sc, chunk, nsplit, po, pml, stream);
+int launch_heads(const Problem& p, const CacheScales& sc, const Fp8Geometry& g, const OwnPartials& part, cudaStream_t stream) {
+  const bool tma = tma_pages(p, sc.n_pages);
+  if (g.heads == 8) return tma ? launch_one<D, BF16, 8, true>(p, sc, g, part, stream) : launch_one<D, BF16, 8, false>(p, sc, g, part, stream);
+  return tma ? launch_one<D, BF16, 16, true>(p, sc, g, part, stream) : launch_one<D, BF16, 16, false>(p, sc, g, part, stream);
 }
 
 }  // namespace
 
-int launch_decode_partial_fp8(const Problem& p, const CacheScales& sc, int dtype, int chunk, int nsplit, float* po, float* pml,
-                              cudaStream_t stream) {
+bool decode_fp8_geometry(const Problem& p, int kv_chunk, Fp8Geometry* g) {
+  constexpr int64_t kSms = 148;
+  g->heads = p.group <= 8 ? 8 : 16;
+  g->units = p.Hkv * ((p.group + g->heads - 1) / g->heads);
+  const int64_t pairs = static_cast<int64_t>(p.B) * g->units, most = pairs * ((p.S + kBlockKeys - 1) / kBlockKeys);
+  int64_t grid = kSms * (p.E == 128 || g->heads == 16 ? 2 : 3);
+  static_assert(Geo<128, 8>::kCtas == 2 && Geo<128, 16>::kCtas == 2 && Geo<64, 16>::kCtas == 2 && Geo<64, 8>::kCtas == 3, "as above");
+  g->fixed_blocks = 0;
+  if (kv_chunk > 0) {
+    g->fixed_blocks = (kv_chunk + kBlockKeys - 1) / kBlockKeys;
+    grid = (most + g->fixed_blocks - 1) / g->fixed_blocks;
+  }
+  if (grid > most) grid = most;
+  if (grid + pairs > 0x7fffffffLL) return false;
+  g->grid = static_cast<int>(grid);
+  g->slots = grid + pairs;
+  g->bytes = static_cast<uint64_t>(g->slots) * g->heads * (p.E + 2) * sizeof(float) + static_cast<uint64_t>(pairs) * sizeof(int2);
+  return true;
+}
+
+int launch_decode_partial_fp8(const Problem& p, const CacheScales& sc, int dtype, const Fp8Geometry& g, const OwnPartials& part, cudaStream_t stream) {
   const bool bf16 = dtype == B200_SDPA_BF16;
-  if (p.E == 128)
-    return bf16 ? launch_heads<128, true>(p, sc, chunk, nsplit, po, pml, stream)
-                : launch_heads<128, false>(p, sc, chunk, nsplit, po, pml, stream);
-  return bf16 ? launch_heads<64, true>(p, sc, chunk, nsplit, po, pml, stream)
-              : launch_heads<64, false>(p, sc, chunk, nsplit, po, pml, stream);
+  if (p.E == 128) return bf16 ? launch_heads<128, true>(p, sc, g, part, stream) : launch_heads<128, false>(p, sc, g, part, stream);
+  return bf16 ? launch_heads<64, true>(p, sc, g, part, stream) : launch_heads<64, false>(p, sc, g, part, stream);
 }
 
 }  // namespace b200
