@@ -190,6 +190,9 @@ int default_chunk(const Problem& p) {
 }  // namespace
 
 int cache_decode_served(const B200CacheDecodeParams& a) {
+  for (int i = 0; i < 3 && a.k_scales != nullptr; ++i)   // (the kernels multiply page and row by 32 bits)
+    if (a.k_scales_stride[i] < 0 || a.k_scales_stride[i] > 0x7fffffffLL || a.v_scales_stride[i] < 0 || a.v_scales_stride[i] > 0x7fffffffLL)
+      return B200_SDPA_ERR_UNSUPPORTED;
   if (static_cast<int64_t>(a.B) * a.Hq > 0x7fffffffLL) return B200_SDPA_ERR_UNSUPPORTED;
   if (a.prefix_len == 0) return a.k_scales != nullptr ? B200_SDPA_OK : B200_SDPA_ERR_UNSUPPORTED;
   const Problem f = prefix_problem(a, reinterpret_cast<void*>(256), reinterpret_cast<void*>(256));

@@ -58,7 +58,7 @@ template <int D, int HEADS> struct Sync {
   static constexpr int kStages = Geo<D, HEADS>::kStages;
   uint64_t full[kStages];                  // the copies' arrivals and the scales' one
   uint64_t empty[kStages];                 // the computing warps
-  float scale[kStages][2][kBlockKeys];     // of the keys: 2^e; of the values: e (NaN for a NaN scale)
+  float scale[kStages][2][kBlockKeys];     // of the keys: 2^e; of the values: e (NaN for a NaN scale); anything behind the end
   float top[kStages];                      // the block's largest e of a value
   int abort_flag;
   float meet[2][Geo<D, HEADS>::kState][32];   // two warps' states on their way to another
@@ -268,54 +268,90 @@ __device__ __forceinline__ void bring_rows(const List& l, const CacheScales& sc,
   }
 }
 
-// The warp that brings the scales of a block's keys l, l + 32, ... and of their values, asked for a block ahead.
+// The warp that brings the scales of a block's keys l, l + 32, ... and of their values.  Scales are asked for two blocks ahead and
+// pages looked up four blocks ahead, since under load each takes about as long as a block.  One warp does this for four that
+// compute, so every instruction of it counts: one multiply-add for an address, one look at all pages of a block.
 template <int D, int HEADS>
 __device__ __forceinline__ void bring_scales(const List& l, const CacheScales& sc, Sync<D, HEADS>* sync, Cursor c, int lane,
                                              long long wait_limit) {
-  constexpr int kStages = Geo<D, HEADS>::kStages, kLook = kBlockKeys / 32;
+  constexpr int kStages = Geo<D, HEADS>::kStages, kLook = kBlockKeys / 32, kDepth = 2;
   const Problem& p = l.p;
   const int page_mask = (1 << p.page_shift) - 1;
-  int entries[kLook], codes[2][kLook];   // of the block after the next, of the next; codes: -1 where there is no key
+  const uint32_t k_page = static_cast<uint32_t>(sc.ks[0]), v_page = static_cast<uint32_t>(sc.vs[0]);
+  int entries[kDepth][kLook];
+  uint32_t codes[kDepth][2][kLook];
   Cursor next = c, ahead = c;
-  auto look_up = [&]() {
-#pragma unroll
-    for (int i = 0; i < kLook; ++i) entries[i] = entry_of(p, ahead, ahead.blk * kBlockKeys + lane + 32 * i);
-    ahead.step(l);
-  };
-  auto ask = [&]() {
-    const int hk = next.unit % p.Hkv;
+  const int blocks = c.left;
+  auto look_up = [&](int (&e)[kLook]) {
+    const int* table = p.block_table + static_cast<int64_t>(ahead.b) * p.table_stride;
+    const int key0 = ahead.blk * kBlockKeys + lane;
 #pragma unroll
     for (int i = 0; i < kLook; ++i) {
-      codes[0][i] = codes[1][i] = -1;
-      if (next.left <= 0) continue;
-      const int row = next.blk * kBlockKeys + lane + 32 * i;
-      const int64_t page = page_of(p, sc, next, entries[i], row);
-      if (page < 0) continue;
-      codes[0][i] = sc.k[page * sc.ks[0] + hk * sc.ks[1] + (row & page_mask) * sc.ks[2]];
-      codes[1][i] = sc.v[page * sc.vs[0] + hk * sc.vs[1] + (row & page_mask) * sc.vs[2]];
+      e[i] = 0;   // (behind the end: a page that is there; what it says is not used)
+      if (ahead.left > 0 && key0 + 32 * i < ahead.n_keys) e[i] = table[(key0 + 32 * i) >> p.page_shift];
+    }
+    ahead.step(l);
+  };
+  auto ask = [&](int (&e)[kLook], uint32_t (&cd)[2][kLook]) {
+    if (next.left <= 0) return;
+    unsigned worst = 0;
+#pragma unroll
+    for (int i = 0; i < kLook; ++i) worst = max(worst, static_cast<unsigned>(e[i]));
+    if (__any_sync(0xffffffffu, worst >= static_cast<unsigned>(sc.n_pages))) {
+#pragma unroll
+      for (int i = 0; i < kLook; ++i)
+        if (static_cast<unsigned>(e[i]) >= static_cast<unsigned>(sc.n_pages)) {
+          report_page(p.status, B200_SDPA_ERR_PAGE, next.b, next.blk * kBlockKeys + lane + 32 * i, sc.n_pages);
+          e[i] = 0;
+        }
+    }
+    const int hk = next.unit % p.Hkv;
+    const uint8_t* k = sc.k + hk * sc.ks[1];
+    const uint8_t* v = sc.v + hk * sc.vs[1];
+    const uint32_t k_row = static_cast<uint32_t>(sc.ks[2]), v_row = static_cast<uint32_t>(sc.vs[2]);
+#pragma unroll
+    for (int i = 0; i < kLook; ++i) {
+      const uint32_t row = static_cast<uint32_t>((next.blk * kBlockKeys + lane + 32 * i) & page_mask);
+      cd[0][i] = k[static_cast<uint64_t>(static_cast<uint32_t>(e[i])) * k_page + static_cast<uint64_t>(row) * k_row];
+      cd[1][i] = v[static_cast<uint64_t>(static_cast<uint32_t>(e[i])) * v_page + static_cast<uint64_t>(row) * v_row];
     }
     next.step(l);
   };
-  look_up();
-  ask();
-  look_up();
-  for (int n = 0; n < c.left; ++n) {
-    const int s = n % kStages;
-    if (!wait_read(p, sync, n, 3, lane, wait_limit)) break;
-    int top = -1;
 #pragma unroll
-    for (int i = 0; i < kLook; ++i) {
-      sync->scale[s][0][lane + 32 * i] = codes[0][i] < 0 ? 0.f : scale_value(codes[0][i]);
-      const int x = codes[1][i];
-      sync->scale[s][1][lane + 32 * i] = x < 0 ? -CUDART_INF_F : (x == 255 ? CUDART_NAN_F : static_cast<float>(x - 127));
-      if (x < 255 && x > top) top = x;
+  for (int d = 0; d < kDepth; ++d) look_up(entries[d]);
+#pragma unroll
+  for (int d = 0; d < kDepth; ++d) {
+    ask(entries[d], codes[d]);
+    look_up(entries[d]);
+  }
+  bool alive = true;
+  for (int n0 = 0; n0 < blocks && alive; n0 += kDepth) {
+#pragma unroll
+    for (int d = 0; d < kDepth; ++d) {
+      const int n = n0 + d;
+      if (n >= blocks || !alive) break;
+      alive = wait_read(p, sync, n, 3, lane, wait_limit);
+      if (!alive) break;
+      const int s = n % kStages;
+      float* to = &sync->scale[s][0][lane];
+      const int key0 = c.blk * kBlockKeys + lane, n_keys = c.n_keys;
+      int top = -1;
+#pragma unroll
+      for (int i = 0; i < kLook; ++i) {
+        // 2^e as bits (2^-127 as 0: beside such a key every score is 0 in fp32), and e as a number, by way of 2^23 + code
+        const uint32_t k = codes[d][0][i], v = codes[d][1][i];
+        to[32 * i] = __uint_as_float(k == 255u ? 0x7fffffffu : k << 23);
+        to[kBlockKeys + 32 * i] = v == 255u ? CUDART_NAN_F : __uint_as_float(0x4b000000u | v) - (8388608.f + 127.f);
+        if (v < 255u && key0 + 32 * i < n_keys) top = max(top, static_cast<int>(v));
+      }
+      top = __reduce_max_sync(0xffffffffu, top);
+      if (lane == 0) sync->top[s] = top < 0 ? -CUDART_INF_F : static_cast<float>(top - 127);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&sync->full[s]));
+      c.step(l);
+      ask(entries[d], codes[d]);
+      look_up(entries[d]);
     }
-    top = __reduce_max_sync(0xffffffffu, top);
-    if (lane == 0) sync->top[s] = top < 0 ? -CUDART_INF_F : static_cast<float>(top - 127);
-    __syncwarp();
-    if (lane == 0) mbar_arrive(smem_u32(&sync->full[s]));
-    ask();
-    look_up();
   }
 }
 
@@ -503,6 +539,11 @@ __global__ void __launch_bounds__(kThreads, Geo<D, HEADS>::kCtas)
                 *reinterpret_cast<uint4*>(smem + st * G::kStageBytes + G::kTileBytes + warp * kWarpKeys * D + i * 16) = make_uint4(0, 0, 0, 0);
             fence_proxy_async_smem();   // (the stage's next block comes by tensor copies)
             __syncwarp();
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+              for (int i = 0; i < 2; ++i)
+                if (key_w + 16 * t + g + 8 * i >= n_keys) ev[t][i] = -CUDART_INF_F;
           }
           // ---- S^T = K Q^T: keys 16 t + g, + 8 x heads 2 tq, 2 tq + 1
           constexpr int kChains = NB == 1 ? 2 : 1;   // even and odd k-steps apart
