@@ -34,26 +34,31 @@ struct Merge {
   int heads, units;
 };
 
-// One CTA per (sequence, query head): the prefix's partials (rows (h * B + b) * n ..) and the own ones in use.
-template <typename T, int D>
+// WARPS warps for each (sequence, query head), 4 / WARPS rows in a CTA: the prefix's partials (rows (h * B + b) * n ..) and the own
+// ones in use.  Bound by latency: the (maximum, sum) pairs are read at once, one a lane, then the rows eight at a time.  One warp where
+// there are rows enough to fill the GPU, four where the ranges are many and the rows few.
+template <typename T, int D, int WARPS>
 __global__ void __launch_bounds__(kCombineWarps * 32) cache_combine_kernel(const Problem p, const Merge a) {
-  constexpr int C = D / 32;   // columns per lane
-  __shared__ float sm_o[kCombineWarps][D];
-  __shared__ float sm_l[kCombineWarps];
-  const int h = blockIdx.x % p.Hq, b = blockIdx.x / p.Hq;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int C = D / 32, kChunk = 32 * WARPS;   // columns per lane, ranges whose weights are held at a time
+  __shared__ float sm_w[kCombineWarps / WARPS][kChunk];
+  __shared__ float sm_o[WARPS > 1 ? kCombineWarps : 1][D], sm_x[kCombineWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = warp % WARPS, lane_w = sub * 32 + lane;
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * (kCombineWarps / WARPS) + warp / WARPS;
   pdl_wait();
   pdl_launch_dependents();
+  if (id >= static_cast<int64_t>(p.B) * p.Hq) return;   // (whole warps; with four to a row the grid is exact)
+  const int h = static_cast<int>(id % p.Hq), b = static_cast<int>(id / p.Hq);
   // own partials: row own0 + s * step
   int used = 0, step = 1;
   int64_t own0 = 0;
   if (a.range != nullptr) {
+    const int in_group = h % p.group;
+    const int64_t pair = static_cast<int64_t>(b) * a.units + in_group / a.heads * p.Hkv + h / p.group;
     if (valid_keys(p, b) > 0) {
-      const int in_group = h % p.group;
-      const int2 r = a.range[static_cast<int64_t>(b) * a.units + in_group / a.heads * p.Hkv + h / p.group];
-      used = r.y - r.x + 1;
+      const int2 r = a.range[pair];
+      used = (r.y - r.x + 1) * kFp8Parts;
       step = a.heads;
-      own0 = static_cast<int64_t>(r.x) * a.heads + in_group % a.heads;
+      own0 = static_cast<int64_t>(r.x) * kFp8Parts * a.heads + in_group % a.heads;
     }
   } else if (a.n_own > 0) {
     used = (valid_keys(p, b) + a.chunk - 1) / a.chunk;
@@ -64,47 +69,92 @@ __global__ void __launch_bounds__(kCombineWarps * 32) cache_combine_kernel(const
   if (!dbg_bhrc(p.status, DBG_CACHE_DECODE * 100 + 1, b, p.B, h, p.Hq, 0, 1, lane * C, C, p.Dv)) return;
   auto row_of = [&](int s) { return s < a.n_prefix ? pre0 + s : own0 + static_cast<int64_t>(s - a.n_prefix) * step; };
   const int total = a.n_prefix + used;
-  auto pair_of = [&](int s) {
-    return *reinterpret_cast<const float2*>((s < a.n_prefix ? a.prefix.ml : a.own.ml) + row_of(s) * 2);
+  auto pair_of = [&](int s) { return *reinterpret_cast<const float2*>((s < a.n_prefix ? a.prefix.ml : a.own.ml) + row_of(s) * 2); };
+  auto together = [&]() {
+    if constexpr (WARPS > 1) __syncthreads();
+    else __syncwarp();
   };
   float mx = -CUDART_INF_F;
-  for (int s = lane; s < total; s += 32) mx = fmaxf(mx, pair_of(s).x);
+  float2 mine = make_float2(-CUDART_INF_F, 0.f);   // of the first chunk
+  for (int s = lane_w; s < total; s += kChunk) {
+    const float2 ml = pair_of(s);
+    if (s == lane_w) mine = ml;
+    mx = fmaxf(mx, ml.x);
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  if constexpr (WARPS > 1) {
+    if (lane == 0) sm_x[warp] = mx;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) mx = fmaxf(mx, sm_x[w]);
+  }
   const float ms = (mx == -CUDART_INF_F) ? 0.f : mx;
   float acc[C], lsum = 0.f;
 #pragma unroll
   for (int c = 0; c < C; ++c) acc[c] = 0.f;
-#pragma unroll 4
-  for (int s = warp; s < total; s += kCombineWarps) {
-    const float2 ml = pair_of(s);
-    // a range without a visible key has the sum 0, and the prefix kernel wrote nothing else for it (a NaN sum counts)
-    if (ml.y == 0.f) continue;
-    const float* src = (s < a.n_prefix ? a.prefix.o : a.own.o) + row_of(s) * D + lane * C;
-    float v[C];
-    if constexpr (C == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src);
-    else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(src);
-    const float w = exp2f(ml.x - ms);
-    lsum = fmaf(ml.y, w, lsum);
+  for (int s0 = 0; s0 < total; s0 += kChunk) {
+    if (s0 > 0) {
+      together();   // (the weights before have been used)
+      mine = s0 + lane_w < total ? pair_of(s0 + lane_w) : make_float2(-CUDART_INF_F, 0.f);
+    }
+    // a range without a visible key has the sum 0, and nothing else of it may have been written (a NaN sum counts)
+    const float wgt = mine.y != 0.f ? exp2f(mine.x - ms) : 0.f;
+    lsum += mine.y != 0.f ? wgt * mine.y : 0.f;
+    sm_w[warp / WARPS][lane_w] = wgt;
+    together();
+    const int n = total - s0 < kChunk ? total - s0 : kChunk;
+    for (int s1 = sub; s1 < n; s1 += 8 * WARPS) {
+      float v[8][C], w[8];
 #pragma unroll
-    for (int c = 0; c < C; ++c) acc[c] = fmaf(v[c], w, acc[c]);
+      for (int i = 0; i < 8; ++i) {
+        const int s = s1 + i * WARPS;
+        w[i] = s < n ? sm_w[warp / WARPS][s] : 0.f;
+#pragma unroll
+        for (int c = 0; c < C; ++c) v[i][c] = 0.f;
+        if (w[i] != 0.f) {
+          const float* src = (s0 + s < a.n_prefix ? a.prefix.o : a.own.o) + row_of(s0 + s) * D + lane * C;
+          if constexpr (C == 4) *reinterpret_cast<float4*>(v[i]) = *reinterpret_cast<const float4*>(src);
+          else *reinterpret_cast<float2*>(v[i]) = *reinterpret_cast<const float2*>(src);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int c = 0; c < C; ++c) acc[c] = fmaf(v[i][c], w[i], acc[c]);
+    }
   }
 #pragma unroll
-  for (int c = 0; c < C; ++c) sm_o[warp][lane * C + c] = acc[c];
-  if (lane == 0) sm_l[warp] = lsum;
-  __syncthreads();
-  float l = 0.f;
+  for (int o = 16; o > 0; o >>= 1) lsum += __shfl_xor_sync(0xffffffffu, lsum, o);
+  if constexpr (WARPS > 1) {
+    __syncthreads();   // (sm_x has been read)
 #pragma unroll
-  for (int w = 0; w < kCombineWarps; ++w) l += sm_l[w];
-  const float inv = l != 0.f ? 1.f / l : 0.f;
-  for (int d = threadIdx.x; d < D; d += kCombineWarps * 32) {
-    float o = 0.f;
+    for (int c = 0; c < C; ++c) sm_o[warp][lane * C + c] = acc[c];
+    if (lane == 0) sm_x[warp] = lsum;
+    __syncthreads();
+    if (warp != 0) return;
+    lsum = 0.f;
 #pragma unroll
-    for (int w = 0; w < kCombineWarps; ++w) o += sm_o[w][d];
-    reinterpret_cast<T*>(p.out)[b * p.os[0] + h * p.os[1] + d * p.os[3]] = from_f32<T>(o * inv);
+    for (int w = 0; w < WARPS; ++w) {
+      lsum += sm_x[w];
+#pragma unroll
+      for (int c = 0; c < C; ++c) acc[c] = w == 0 ? sm_o[0][lane * C + c] : acc[c] + sm_o[w][lane * C + c];
+    }
   }
-  if (p.lse != nullptr && threadIdx.x == 0)
-    p.lse[b * p.ls[0] + h * p.ls[1]] = l == 0.f ? -CUDART_INF_F : fmaf(mx, kLn2, logf(l));
+  const float inv = lsum != 0.f ? 1.f / lsum : 0.f;
+  T* out = reinterpret_cast<T*>(p.out) + b * p.os[0] + h * p.os[1];
+  __align__(8) T r[C];
+#pragma unroll
+  for (int c = 0; c < C; ++c) r[c] = from_f32<T>(acc[c] * inv);
+  T* to = out + lane * C;
+  if (p.os[3] == 1 && reinterpret_cast<uintptr_t>(to) % (2 * C) == 0) {
+    if constexpr (C == 4) *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(r);
+    else *reinterpret_cast<uint32_t*>(to) = *reinterpret_cast<const uint32_t*>(r);
+  } else {
+#pragma unroll
+    for (int c = 0; c < C; ++c) out[(lane * C + c) * p.os[3]] = r[c];
+  }
+  if (p.lse != nullptr && lane == 0) p.lse[b * p.ls[0] + h * p.ls[1]] = lsum == 0.f ? -CUDART_INF_F : fmaf(mx, kLn2, logf(lsum));
 }
 
 struct Geometry {
@@ -226,11 +276,15 @@ int geometry(const B200CacheDecodeParams& a, Geometry* g) {
   return B200_SDPA_OK;
 }
 
-template <typename T> int launch_combine(const Problem& p, const Merge& a, cudaStream_t stream) {
-  auto kern = p.E == 128 ? cache_combine_kernel<T, 128> : cache_combine_kernel<T, 64>;
-  if (!launch_pdl(kern, dim3(p.B * p.Hq), kCombineWarps * 32, 0, stream, p, a)) return B200_SDPA_ERR_CUDA;
+template <typename T, int WARPS> int launch_combine_warps(const Problem& p, const Merge& a, cudaStream_t stream) {
+  auto kern = p.E == 128 ? cache_combine_kernel<T, 128, WARPS> : cache_combine_kernel<T, 64, WARPS>;
+  const unsigned grid = static_cast<unsigned>((static_cast<int64_t>(p.B) * p.Hq * WARPS + kCombineWarps - 1) / kCombineWarps);
+  if (!launch_pdl(kern, dim3(grid), kCombineWarps * 32, 0, stream, p, a)) return B200_SDPA_ERR_CUDA;
   count_launch(KID_COMBINE);
   return B200_SDPA_OK;
+}
+template <typename T> int launch_combine(const Problem& p, const Merge& a, cudaStream_t stream) {
+  return static_cast<int64_t>(p.B) * p.Hq >= 1024 ? launch_combine_warps<T, 1>(p, a, stream) : launch_combine_warps<T, 4>(p, a, stream);
 }
 
 }  // namespace
@@ -312,8 +366,8 @@ int launch_cache_decode(const B200CacheDecodeParams& a, cudaStream_t stream) {
     OwnPartials part;
     part.slots = g.fp8.slots;
     part.o = reinterpret_cast<float*>(ws);
-    part.ml = part.o + g.fp8.slots * g.fp8.heads * a.D;
-    part.range = reinterpret_cast<int2*>(part.ml + g.fp8.slots * g.fp8.heads * 2);
+    part.ml = part.o + g.fp8.slots * kFp8Parts * g.fp8.heads * a.D;
+    part.range = reinterpret_cast<int2*>(part.ml + g.fp8.slots * kFp8Parts * g.fp8.heads * 2);
     m.own = {part.o, part.ml};
     m.range = part.range;
     m.heads = g.fp8.heads;

@@ -144,11 +144,12 @@ struct CacheScales {
   int64_t ks[3], vs[3];   // page, head, row in page
   int n_pages;
 };
-// Partials of the own keys of an 8-bit cache (decode_fp8.cu): slots of `heads` rows; a pair (sequence, unit) has the slots
+// Partials of the own keys of an 8-bit cache (decode_fp8.cu): slots of kFp8Parts x `heads` rows; a pair (sequence, unit) has the slots
 // range[pair].x to range[pair].y, all written, unless its sequence is empty.
+constexpr int kFp8Parts = 4;
 struct OwnPartials {
-  float* o;      // [slot][heads][D]
-  float* ml;     // [slot][heads][2]: maximum in log2 units, sum
+  float* o;      // [slot][part][heads][D]
+  float* ml;     // [slot][part][heads][2]: maximum in log2 units, sum
   int2* range;   // [pair]
   int64_t slots;
 };

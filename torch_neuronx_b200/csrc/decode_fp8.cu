@@ -2,8 +2,8 @@
 //
 // The cache is read once for all query heads of a kv head.  Its blocks of 128 keys, over all sequences and kv heads, are one
 // list that is cut into equal ranges, one for each CTA the GPU holds at a time: the lengths are read on the device, so ragged
-// batches leave no SM without work and no CTA starts twice.  A CTA leaves one fp32 partial (o, m, l) for each (sequence, kv head)
-// that its range touches, in slot `CTA + number of the pair` (both only ever grow along the list, so no slot is used twice),
+// batches leave no SM without work and no CTA starts twice.  A CTA leaves fp32 partials (o, m, l), one of each computing warp, for
+// each (sequence, kv head) that its range touches, in slot `CTA + number of the pair` (both only ever grow along the list, so no slot is used twice),
 // and whoever has a pair's first or last block notes the slot; a second launch merges (cache_decode.cu).
 // What the format changes:
 //   * e4m3 is exact in fp16, so both products are fp16 m16n8k16 MMAs with the bytes expanded in registers (8-bit MMAs would
@@ -34,7 +34,7 @@ namespace {
 using namespace ptx;
 using namespace tc;
 
-constexpr int kWarps = 4;                         // that compute; one more brings the rows, one the scales
+constexpr int kWarps = kFp8Parts;                         // that compute; one more brings the rows, one the scales
 constexpr int kThreads = (kWarps + 2) * 32;
 constexpr int kBlockKeys = 128;
 constexpr int kWarpKeys = kBlockKeys / kWarps;
@@ -50,18 +50,25 @@ template <int D, int HEADS> struct Geo {
   static constexpr int kRingBytes = kStages * kStageBytes;
   static constexpr int kChunksPerRow = D / 16;
   static constexpr int kCtas = D == 128 || HEADS == 16 ? 2 : 3;             // of an SM
-  static constexpr int kState = D / 4 * (HEADS / 8) + 4 * (HEADS / 8);      // registers of a warp's state: o, m, l
   static __device__ __forceinline__ int swizzle(int row) { return D == 128 ? row & 7 : (row >> 1) & 3; }
+};
+
+// What the warps that compute have to know of a block, left beside it by the warp that brings the rows: they walk through the list
+// without reading a length.
+struct __align__(16) Block {
+  int blk, n_keys, last, next_unit;   // last: of this CTA's blocks of the pair; the pair behind it (next_unit -1: none)
+  int next_b, pad[3];
 };
 
 template <int D, int HEADS> struct Sync {
   static constexpr int kStages = Geo<D, HEADS>::kStages;
-  uint64_t full[kStages];                  // the copies' arrivals and the scales' one
+  uint64_t full[kStages];                  // the copies' arrivals and those of the warps that start them
   uint64_t empty[kStages];                 // the computing warps
-  float scale[kStages][2][kBlockKeys];     // of the keys: 2^e; of the values: e (NaN for a NaN scale); anything behind the end
-  float top[kStages];                      // the block's largest e of a value
+  Block block[kStages];
+  alignas(16) uint16_t query[kStages][HEADS][D + 16];   // with a pair's first block: its query rows (padded: fragments meet no bank twice)
+  uint32_t scale[kStages][2][kBlockKeys];  // of the keys and of the values: the four bytes around a scale
+  uint8_t shift[kStages][2][kBlockKeys];   // ... and the bit at which it starts
   int abort_flag;
-  float meet[2][Geo<D, HEADS>::kState][32];   // two warps' states on their way to another
 };
 template <int D, int HEADS> constexpr int smem_bytes() {
   return Geo<D, HEADS>::kRingBytes + 1024 + static_cast<int>(sizeof(Sync<D, HEADS>));
@@ -70,6 +77,10 @@ template <int D, int HEADS> constexpr int smem_bytes() {
 __device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
+__device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 // One of the barrier's counted arrivals, when this thread's copies so far have landed.
 __device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
@@ -226,6 +237,17 @@ __device__ __forceinline__ void bring_rows(const List& l, const CacheScales& sc,
       const int hk = c.unit % p.Hkv;
       const uint32_t stage = ring + s * G::kStageBytes, bar = smem_u32(&sync->full[s]);
       const int key0 = c.blk * kBlockKeys;
+      Cursor after = c;
+      after.step(l);
+      if (lane == 0) {
+        const bool more = after.left > 0;
+        Block& k = sync->block[s];
+        k.blk = c.blk;
+        k.n_keys = c.n_keys;
+        k.last = !more || after.b != c.b || after.unit != c.unit;
+        k.next_unit = more ? after.unit : -1;
+        k.next_b = after.b;
+      }
       if constexpr (TMA) {
         const int rows = page_mask + 1 < kBlockKeys ? page_mask + 1 : kBlockKeys;   // of one copy
         const int first = (lane >> 1) * rows;                  // lanes 2 i and 2 i + 1: keys and values of copy i
@@ -256,32 +278,37 @@ __device__ __forceinline__ void bring_rows(const List& l, const CacheScales& sc,
             cp_async_16(dst + G::kTileBytes, static_cast<const uint8_t*>(p.v) + hk * p.vs[1] + page * p.vs[0] + in_page * p.vs[2] + ch * 16);
           }
         cp_async_arrive(bar);   // (every lane's copies; the barrier counts the 32 lanes)
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar);   // (the block's record)
       }
       ++n;
-      c.step(l);
+      c = after;
       look_up(entries[s]);
     }
   }
+  if constexpr (!TMA) cp_async_wait_all();
   if (*static_cast<volatile int*>(&sync->abort_flag) != 0 && lane == 0) {
     // what was issued has to land before the CTA lets go of its memory
     for (int s = 0; s < kStages && s < n; ++s) wait_drain(smem_u32(&sync->full[s]), ((n - 1 - s) / kStages) & 1);
   }
 }
 
-// The warp that brings the scales of a block's keys l, l + 32, ... and of their values.  Scales are asked for two blocks ahead and
-// pages looked up four blocks ahead, since under load each takes about as long as a block.  One warp does this for four that
-// compute, so every instruction of it counts: one multiply-add for an address, one look at all pages of a block.
+// The warp that brings the scales of a block's keys l, l + 32, ... and of their values, and with the first block of a pair its query
+// rows.  All by asynchronous copies: a value that passes through a register would be waited for, and under load each takes as
+// long as a block.  (Scales are single bytes at any stride, so the four bytes around one are copied.)  Pages are looked up two blocks ahead.
 template <int D, int HEADS>
 __device__ __forceinline__ void bring_scales(const List& l, const CacheScales& sc, Sync<D, HEADS>* sync, Cursor c, int lane,
                                              long long wait_limit) {
-  constexpr int kStages = Geo<D, HEADS>::kStages, kLook = kBlockKeys / 32, kDepth = 2;
+  constexpr int kStages = Geo<D, HEADS>::kStages, kLook = kBlockKeys / 32, kAhead = 2;
   const Problem& p = l.p;
   const int page_mask = (1 << p.page_shift) - 1;
   const uint32_t k_page = static_cast<uint32_t>(sc.ks[0]), v_page = static_cast<uint32_t>(sc.vs[0]);
-  int entries[kDepth][kLook];
-  uint32_t codes[kDepth][2][kLook];
-  Cursor next = c, ahead = c;
+  const uint32_t k_row = static_cast<uint32_t>(sc.ks[2]), v_row = static_cast<uint32_t>(sc.vs[2]);
+  int entries[kAhead][kLook];
+  Cursor ahead = c;
   const int blocks = c.left;
+  int b = -1, unit = -1;   // whose queries were brought last
+  const uint8_t *k_base = nullptr, *v_base = nullptr;
   auto look_up = [&](int (&e)[kLook]) {
     const int* table = p.block_table + static_cast<int64_t>(ahead.b) * p.table_stride;
     const int key0 = ahead.blk * kBlockKeys + lane;
@@ -292,115 +319,63 @@ __device__ __forceinline__ void bring_scales(const List& l, const CacheScales& s
     }
     ahead.step(l);
   };
-  auto ask = [&](int (&e)[kLook], uint32_t (&cd)[2][kLook]) {
-    if (next.left <= 0) return;
-    unsigned worst = 0;
 #pragma unroll
-    for (int i = 0; i < kLook; ++i) worst = max(worst, static_cast<unsigned>(e[i]));
-    if (__any_sync(0xffffffffu, worst >= static_cast<unsigned>(sc.n_pages))) {
-#pragma unroll
-      for (int i = 0; i < kLook; ++i)
-        if (static_cast<unsigned>(e[i]) >= static_cast<unsigned>(sc.n_pages)) {
-          report_page(p.status, B200_SDPA_ERR_PAGE, next.b, next.blk * kBlockKeys + lane + 32 * i, sc.n_pages);
-          e[i] = 0;
-        }
-    }
-    const int hk = next.unit % p.Hkv;
-    const uint8_t* k = sc.k + hk * sc.ks[1];
-    const uint8_t* v = sc.v + hk * sc.vs[1];
-    const uint32_t k_row = static_cast<uint32_t>(sc.ks[2]), v_row = static_cast<uint32_t>(sc.vs[2]);
-#pragma unroll
-    for (int i = 0; i < kLook; ++i) {
-      const uint32_t row = static_cast<uint32_t>((next.blk * kBlockKeys + lane + 32 * i) & page_mask);
-      cd[0][i] = k[static_cast<uint64_t>(static_cast<uint32_t>(e[i])) * k_page + static_cast<uint64_t>(row) * k_row];
-      cd[1][i] = v[static_cast<uint64_t>(static_cast<uint32_t>(e[i])) * v_page + static_cast<uint64_t>(row) * v_row];
-    }
-    next.step(l);
-  };
-#pragma unroll
-  for (int d = 0; d < kDepth; ++d) look_up(entries[d]);
-#pragma unroll
-  for (int d = 0; d < kDepth; ++d) {
-    ask(entries[d], codes[d]);
-    look_up(entries[d]);
-  }
+  for (int d = 0; d < kAhead; ++d) look_up(entries[d]);
   bool alive = true;
-  for (int n0 = 0; n0 < blocks && alive; n0 += kDepth) {
+  for (int n0 = 0; n0 < blocks && alive; n0 += kAhead) {
 #pragma unroll
-    for (int d = 0; d < kDepth; ++d) {
+    for (int d = 0; d < kAhead; ++d) {
       const int n = n0 + d;
       if (n >= blocks || !alive) break;
       alive = wait_read(p, sync, n, 3, lane, wait_limit);
       if (!alive) break;
       const int s = n % kStages;
-      float* to = &sync->scale[s][0][lane];
-      const int key0 = c.blk * kBlockKeys + lane, n_keys = c.n_keys;
-      int top = -1;
+      if (c.unit != unit || c.b != b) {
+        b = c.b;
+        unit = c.unit;
+        const int hk = unit % p.Hkv, h0 = unit / p.Hkv * HEADS, heads = p.group - h0 < HEADS ? p.group - h0 : HEADS;
+        k_base = sc.k + hk * sc.ks[1];
+        v_base = sc.v + hk * sc.vs[1];
+        const uint16_t* q = reinterpret_cast<const uint16_t*>(p.q) + b * p.qs[0] + static_cast<int64_t>(hk * p.group + h0) * p.qs[1];
+        if (p.qs[3] == 1 && ((reinterpret_cast<uintptr_t>(q) | static_cast<uint64_t>(p.qs[1] * 2)) & 15) == 0) {
+          for (int i = lane; i < heads * (D / 8); i += 32)
+            cp_async_16(smem_u32(&sync->query[s][i / (D / 8)][i % (D / 8) * 8]), q + i / (D / 8) * p.qs[1] + i % (D / 8) * 8);
+        } else {
+          for (int i = lane; i < heads * D; i += 32) sync->query[s][i / D][i % D] = q[i / D * p.qs[1] + i % D * p.qs[3]];
+        }
+      }
+      int(&e)[kLook] = entries[d];
+      unsigned worst = 0;
+#pragma unroll
+      for (int i = 0; i < kLook; ++i) worst = max(worst, static_cast<unsigned>(e[i]));
+      if (__any_sync(0xffffffffu, worst >= static_cast<unsigned>(sc.n_pages))) {
+#pragma unroll
+        for (int i = 0; i < kLook; ++i)
+          if (static_cast<unsigned>(e[i]) >= static_cast<unsigned>(sc.n_pages)) {
+            report_page(p.status, B200_SDPA_ERR_PAGE, b, c.blk * kBlockKeys + lane + 32 * i, sc.n_pages);
+            e[i] = 0;
+          }
+      }
 #pragma unroll
       for (int i = 0; i < kLook; ++i) {
-        // 2^e as bits (2^-127 as 0: beside such a key every score is 0 in fp32), and e as a number, by way of 2^23 + code
-        const uint32_t k = codes[d][0][i], v = codes[d][1][i];
-        to[32 * i] = __uint_as_float(k == 255u ? 0x7fffffffu : k << 23);
-        to[kBlockKeys + 32 * i] = v == 255u ? CUDART_NAN_F : __uint_as_float(0x4b000000u | v) - (8388608.f + 127.f);
-        if (v < 255u && key0 + 32 * i < n_keys) top = max(top, static_cast<int>(v));
+        const uint32_t row = static_cast<uint32_t>((c.blk * kBlockKeys + lane + 32 * i) & page_mask);
+        const uint64_t page = static_cast<uint32_t>(e[i]);
+        const uintptr_t k = reinterpret_cast<uintptr_t>(k_base) + page * k_page + static_cast<uint64_t>(row) * k_row;
+        const uintptr_t v = reinterpret_cast<uintptr_t>(v_base) + page * v_page + static_cast<uint64_t>(row) * v_row;
+        cp_async_4(smem_u32(&sync->scale[s][0][lane + 32 * i]), reinterpret_cast<const void*>(k & ~static_cast<uintptr_t>(3)));
+        cp_async_4(smem_u32(&sync->scale[s][1][lane + 32 * i]), reinterpret_cast<const void*>(v & ~static_cast<uintptr_t>(3)));
+        sync->shift[s][0][lane + 32 * i] = static_cast<uint8_t>((k & 3) * 8);
+        sync->shift[s][1][lane + 32 * i] = static_cast<uint8_t>((v & 3) * 8);
       }
-      top = __reduce_max_sync(0xffffffffu, top);
-      if (lane == 0) sync->top[s] = top < 0 ? -CUDART_INF_F : static_cast<float>(top - 127);
+      cp_async_arrive(smem_u32(&sync->full[s]));
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&sync->full[s]));
       c.step(l);
-      ask(entries[d], codes[d]);
-      look_up(entries[d]);
+      look_up(e);
     }
   }
+  cp_async_wait_all();   // (before the CTA lets go of its memory, should it give up)
 }
-
-// The state of a warp for one pair.  Lane 4 g + tq: heads 2 tq, 2 tq + 1 of every eight; o: rows 16 j + 2 g, + 1 of O^T.
-template <int D, int NB> struct State {
-  float o[D / 16][NB][4];
-  float m[NB][2], l[NB][2];   // maximum of the raw scores (for `merge`: in log2 units), this lane's share of the sum
-
-  __device__ __forceinline__ void put(float (*to)[32], int lane) const {
-    int i = 0;
-#pragma unroll
-    for (int j = 0; j < D / 16; ++j)
-#pragma unroll
-      for (int n = 0; n < NB; ++n)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) to[i++][lane] = o[j][n][r];
-#pragma unroll
-    for (int n = 0; n < NB; ++n)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        to[i++][lane] = m[n][e];
-        to[i++][lane] = l[n][e];
-      }
-  }
-  __device__ __forceinline__ void merge(const float (*from)[32], int lane) {
-    float mine[NB][2], theirs[NB][2];
-    int i = D / 4 * NB;
-#pragma unroll
-    for (int n = 0; n < NB; ++n)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float om = from[i++][lane], ol = from[i++][lane];
-        const float mx = fmaxf(m[n][e], om), ref = mx == -CUDART_INF_F ? 0.f : mx;
-        mine[n][e] = ex2(m[n][e] - ref);
-        theirs[n][e] = ex2(om - ref);
-        m[n][e] = mx;
-        l[n][e] = fmaf(l[n][e], mine[n][e], ol * theirs[n][e]);
-      }
-    i = 0;
-#pragma unroll
-    for (int j = 0; j < D / 16; ++j)
-#pragma unroll
-      for (int n = 0; n < NB; ++n)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) o[j][n][r] = fmaf(o[j][n][r], mine[n][r & 1], from[i++][lane] * theirs[n][r & 1]);
-  }
-};
-
-__device__ __forceinline__ void computing_warps_meet() { asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory"); }
 
 // HEADS: query heads of a CTA, 8 or 16.
 template <int D, bool BF16, int HEADS, bool TMA>
@@ -416,7 +391,7 @@ __global__ void __launch_bounds__(kThreads, Geo<D, HEADS>::kCtas)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     for (int s = 0; s < G::kStages; ++s) {
-      mbar_init(smem_u32(&sync->full[s]), TMA ? 2 : 33);
+      mbar_init(smem_u32(&sync->full[s]), TMA ? 1 + 33 : 33 + 33);
       mbar_init(smem_u32(&sync->empty[s]), kWarps);
     }
     sync->abort_flag = 0;
@@ -433,84 +408,63 @@ __global__ void __launch_bounds__(kThreads, Geo<D, HEADS>::kCtas)
     bring_scales<D, HEADS>(list, sc, sync, c, lane, wait_limit);
   } else {
     const int g = lane >> 2, tq = lane & 3;
-    bool ok = true;
-    int n = 0;   // blocks so far
-    while (c.left > 0) {
-      // ---- one pair: `todo` blocks of it
-      const int b = c.b, gsub = c.unit / p.Hkv, hk = c.unit % p.Hkv;
-      const int h0 = hk * p.group + gsub * HEADS;
-      const int n_heads = (p.group - gsub * HEADS) < HEADS ? (p.group - gsub * HEADS) : HEADS;
-      const int first = c.blk, todo = c.n_blk - c.blk < c.left ? c.n_blk - c.blk : c.left, n_keys = c.n_keys;
-      const int64_t pair = static_cast<int64_t>(b) * list.units + c.unit, slot = pair + blockIdx.x;
-      if (tid == 0) {
-        if (first == 0) part.range[pair].x = static_cast<int>(slot);
-        if (first + todo == c.n_blk) part.range[pair].y = static_cast<int>(slot);
-      }
-      // query fragments: k-step s holds elements 16 s + 4 tq .. + 3 of head g, as the bytes of a key's fragment word; a head's
-      // quad has all of it
-      uint32_t qf[NB][KS][2];
-      float sl2[NB][2];   // score to exp2 units, of heads 2 tq, 2 tq + 1
-#pragma unroll
-      for (int i = 0; i < NB; ++i) {
-        const int head = 8 * i + g;
-        const uint16_t* q16 = reinterpret_cast<const uint16_t*>(p.q) + b * p.qs[0] + (h0 + (head < n_heads ? head : 0)) * p.qs[1];
-        const bool vec = p.qs[3] == 1 && reinterpret_cast<uintptr_t>(q16) % 8 == 0;
-        uint2 x[KS];
-        uint32_t top = 0;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          const int at = 16 * s + 4 * tq;
-          if (vec) {
-            x[s] = *reinterpret_cast<const uint2*>(q16 + at);
-          } else {
-            x[s].x = q16[at * p.qs[3]] | static_cast<uint32_t>(q16[(at + 1) * p.qs[3]]) << 16;
-            x[s].y = q16[(at + 2) * p.qs[3]] | static_cast<uint32_t>(q16[(at + 3) * p.qs[3]]) << 16;
-          }
-        }
-#pragma unroll
-        for (int s = 0; s < KS; ++s)   // (magnitudes of either type order like their bits)
-          top = max(max(top, max(x[s].x & 0x7fffu, (x[s].x >> 16) & 0x7fffu)), max(x[s].y & 0x7fffu, (x[s].y >> 16) & 0x7fffu));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        top = __float_as_uint(half_to_f32<BF16>(static_cast<uint16_t>(top)));
-        // largest element into [2^14, 2^15); zeros, infinities and NaN stay as they are
-        int up = top == 0u || top >= 0x7f800000u ? 0 : 127 + 14 - static_cast<int>(top >> 23);
-        if (!BF16 && up < 0) up = 0;
-        if (up > 126) up = 126;
-        const float f = __int_as_float((127 + up) << 23);   // up >= -113
-        const float mine = p.scale * kLog2e * __int_as_float((127 - up) << 23);
-#pragma unroll
-        for (int e = 0; e < 2; ++e) sl2[i][e] = __shfl_sync(0xffffffffu, mine, (2 * tq + e) * 4);
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          const float e0 = half_to_f32<BF16>(static_cast<uint16_t>(x[s].x)), e1 = half_to_f32<BF16>(static_cast<uint16_t>(x[s].x >> 16));
-          const float e2 = half_to_f32<BF16>(static_cast<uint16_t>(x[s].y)), e3 = half_to_f32<BF16>(static_cast<uint16_t>(x[s].y >> 16));
-          qf[i][s][0] = head < n_heads ? pack16<false>(e0 * f, e1 * f) : 0u;
-          qf[i][s][1] = head < n_heads ? pack16<false>(e2 * f, e3 * f) : 0u;
-        }
-      }
-      State<D, NB> a;
-      float r_exp = -CUDART_INF_F;
-#pragma unroll
-      for (int i = 0; i < NB; ++i) {
-#pragma unroll
-        for (int j = 0; j < D / 16; ++j)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) a.o[j][i][r] = 0.f;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          a.m[i][e] = -CUDART_INF_F;
-          a.l[i][e] = 0.f;
-        }
-      }
-
-      for (int blk = first; blk < first + todo; ++blk, ++n) {
+    uint2 q[NB][KS];
+    float o[D / 16][NB][4];     // O^T: rows 2 g, 2 g + 1 of sixteen columns of V; heads 2 tq, 2 tq + 1 of eight
+    float m[NB][2], lsum[NB][2], sl2[NB][2];   // of heads 2 tq, 2 tq + 1: maximum raw score, this lane's share of the sum, score to exp2 units
+    float r_exp = -CUDART_INF_F;
+    int b = c.b, unit = c.unit, first = 0;     // the pair, and its first block here
+    const int blocks = c.left;
+    bool fresh = true, ok = true;
+    for (int n = 0; n < blocks; ++n) {
+      {
         const int st = n % G::kStages;
-        ok = ok && wait_clocked(smem_u32(&sync->full[st]), (n / G::kStages) & 1, &sync->abort_flag, wait_limit);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) {   // (the CTA gives up: what is merged and stored from here on means nothing)
+        ok = __all_sync(0xffffffffu, wait_clocked(smem_u32(&sync->full[st]), (n / G::kStages) & 1, &sync->abort_flag, wait_limit));
+        if (!ok) {   // the CTA gives up
           if (lane == 0) report(p.status, 2, n, warp);
-          continue;
+          break;
+        }
+        const int blk = sync->block[st].blk, n_keys = sync->block[st].n_keys;
+        if (fresh) {
+          fresh = false;
+          first = blk;
+          r_exp = -CUDART_INF_F;
+#pragma unroll
+          for (int i = 0; i < NB; ++i) {
+            // fragments: k-step s holds elements 16 s + 4 tq .. + 3 of head g, as the bytes of a key's fragment word; a head's
+            // quad has all of it
+            uint32_t top = 0;   // (magnitudes of either type order like their bits)
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+              q[i][s] = *reinterpret_cast<const uint2*>(&sync->query[st][8 * i + g][16 * s + 4 * tq]);
+              top = max(max(top, max(q[i][s].x & 0x7fffu, (q[i][s].x >> 16) & 0x7fffu)), max(q[i][s].y & 0x7fffu, (q[i][s].y >> 16) & 0x7fffu));
+            }
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            top = __float_as_uint(half_to_f32<BF16>(static_cast<uint16_t>(top)));
+            // largest element into [2^14, 2^15); zeros, infinities and NaN stay as they are
+            int up = top == 0u || top >= 0x7f800000u ? 0 : 127 + 14 - static_cast<int>(top >> 23);
+            if (!BF16 && up < 0) up = 0;
+            if (up > 126) up = 126;
+            const bool here = unit / p.Hkv * HEADS + 8 * i + g < p.group;   // (else the row is whatever was there)
+            const float f = __int_as_float((127 + up) << 23);               // up >= -113
+            const float factor = p.scale * kLog2e * __int_as_float((127 - up) << 23);
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+              const uint2 v = q[i][s];
+              q[i][s].x = here ? pack16<false>(half_to_f32<BF16>(static_cast<uint16_t>(v.x)) * f, half_to_f32<BF16>(static_cast<uint16_t>(v.x >> 16)) * f) : 0u;
+              q[i][s].y = here ? pack16<false>(half_to_f32<BF16>(static_cast<uint16_t>(v.y)) * f, half_to_f32<BF16>(static_cast<uint16_t>(v.y >> 16)) * f) : 0u;
+            }
+#pragma unroll
+            for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) o[j][i][r] = 0.f;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              sl2[i][e] = __shfl_sync(0xffffffffu, here ? factor : 0.f, (2 * tq + e) * 4);
+              m[i][e] = -CUDART_INF_F;
+              lsum[i][e] = 0.f;
+            }
+          }
         }
         const int key_w = blk * kBlockKeys + warp * kWarpKeys;   // first key of this warp's 32
         if (key_w < n_keys) {
@@ -519,6 +473,7 @@ __global__ void __launch_bounds__(kThreads, Geo<D, HEADS>::kCtas)
           const uint32_t k_row = ring + st * G::kStageBytes + row * D, v_row = k_row + G::kTileBytes;
           auto piece = [&](int x) { return static_cast<uint32_t>(((x + (lane >> 4)) ^ G::swizzle(lane & 7)) << 4); };
           float kx[2][2], ev[2][2];
+          int e_max = -1;
           uint32_t kf[2][KS / 2][4];
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
@@ -526,11 +481,16 @@ __global__ void __launch_bounds__(kThreads, Geo<D, HEADS>::kCtas)
             for (int s = 0; s < KS; s += 2) ldsm_x4(k_row + t * 16 * D + piece(s), kf[t][s / 2]);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              kx[t][i] = sync->scale[st][0][warp * kWarpKeys + 16 * t + g + 8 * i];
-              ev[t][i] = sync->scale[st][1][warp * kWarpKeys + 16 * t + g + 8 * i];
+              const int at = warp * kWarpKeys + 16 * t + g + 8 * i;
+              const uint32_t k = (sync->scale[st][0][at] >> sync->shift[st][0][at]) & 255u, v = (sync->scale[st][1][at] >> sync->shift[st][1][at]) & 255u;
+              // 2^e as bits (2^-127 as 0: beside such a key every score is 0 in fp32), and e as a number, by way of 2^23 + code
+              kx[t][i] = __uint_as_float(k == 255u ? 0x7fffffffu : k << 23);
+              ev[t][i] = v == 255u ? CUDART_NAN_F : __uint_as_float(0x4b000000u | v) - (8388608.f + 127.f);
+              if (v < 255u && key_w + 16 * t + g + 8 * i < n_keys) e_max = max(e_max, static_cast<int>(v));
             }
           }
-          const float e_top = sync->top[st];
+          e_max = __reduce_max_sync(0xffffffffu, e_max);
+          const float e_top = e_max < 0 ? -CUDART_INF_F : static_cast<float>(e_max - 127);   // the largest e of a value here
           const bool tail = key_w + kWarpKeys > n_keys;
           if (tail) {
             // what lies behind the end is anything: its weight is 0, and 0 times a NaN is not
@@ -564,7 +524,7 @@ __global__ void __launch_bounds__(kThreads, Geo<D, HEADS>::kCtas)
               unpack_e4m3_f16(kf[t][s / 2][2 * (s & 1)], a0, a2);
               unpack_e4m3_f16(kf[t][s / 2][2 * (s & 1) + 1], a1, a3);
 #pragma unroll
-              for (int i = 0; i < NB; ++i) mma_f16(part_s[t][i][s % kChains], a0, a1, a2, a3, qf[i][s][0], qf[i][s][1]);
+              for (int i = 0; i < NB; ++i) mma_f16(part_s[t][i][s % kChains], a0, a1, a2, a3, q[i][s].x, q[i][s].y);
             }
           float mn[NB][2];
           bool grow = e_top > r_exp;
@@ -581,9 +541,9 @@ __global__ void __launch_bounds__(kThreads, Geo<D, HEADS>::kCtas)
             for (int e = 0; e < 2; ++e) {
               float x = fmaxf(fmaxf(sv[0][i][e], sv[0][i][2 + e]), fmaxf(sv[1][i][e], sv[1][i][2 + e]));
 #pragma unroll
-              for (int o = 4; o < 32; o *= 2) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
-              mn[i][e] = fmaxf(a.m[i][e], x);
-              grow |= (mn[i][e] - a.m[i][e]) * sl2[i][e] > kRescaleThreshold;
+              for (int d = 4; d < 32; d *= 2) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+              mn[i][e] = fmaxf(m[i][e], x);
+              grow |= (mn[i][e] - m[i][e]) * sl2[i][e] > kRescaleThreshold;
             }
           }
           // ---- o is rescaled when the largest value exponent or a row maximum grows
@@ -596,15 +556,15 @@ __global__ void __launch_bounds__(kThreads, Geo<D, HEADS>::kCtas)
               float f[2];
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
-                f[e] = mn[i][e] == a.m[i][e] ? 1.f : ex2((a.m[i][e] - mn[i][e]) * sl2[i][e]);
-                a.m[i][e] = mn[i][e];
-                a.l[i][e] *= f[e];
+                f[e] = mn[i][e] == m[i][e] ? 1.f : ex2((m[i][e] - mn[i][e]) * sl2[i][e]);
+                m[i][e] = mn[i][e];
+                lsum[i][e] *= f[e];
                 f[e] *= down;
               }
 #pragma unroll
               for (int j = 0; j < D / 16; ++j)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) a.o[j][i][r] *= f[r & 1];
+                for (int r = 0; r < 4; ++r) o[j][i][r] *= f[r & 1];
             }
           }
           // ---- probabilities; times the value scale relative to r, hi and lo, turned round: heads g x keys 2 tq, 2 tq + 1
@@ -619,10 +579,10 @@ __global__ void __launch_bounds__(kThreads, Geo<D, HEADS>::kCtas)
               float x[4];
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
-                const float nm = (a.m[i][e] == -CUDART_INF_F) ? 0.f : -a.m[i][e] * sl2[i][e];
+                const float nm = (m[i][e] == -CUDART_INF_F) ? 0.f : -m[i][e] * sl2[i][e];
                 x[e] = ex2(fmaf(sv[t][i][e], sl2[i][e], nm));
                 x[2 + e] = ex2(fmaf(sv[t][i][2 + e], sl2[i][e], nm));
-                a.l[i][e] += x[e] + x[2 + e];
+                lsum[i][e] += x[e] + x[2 + e];
               }
 #pragma unroll
               for (int y = 0; y < 2; ++y) {
@@ -646,56 +606,47 @@ __global__ void __launch_bounds__(kThreads, Geo<D, HEADS>::kCtas)
                 unpack_e4m3_f16(__byte_perm(vf[2 * u + 1], 0, 0x3120), a2, a3);
 #pragma unroll
                 for (int i = 0; i < NB; ++i) {
-                  mma_f16(a.o[j + u][i], a0, a1, a2, a3, ph[t][i][0], ph[t][i][1]);
-                  mma_f16(a.o[j + u][i], a0, a1, a2, a3, pl[t][i][0], pl[t][i][1]);
+                  mma_f16(o[j + u][i], a0, a1, a2, a3, ph[t][i][0], ph[t][i][1]);
+                  mma_f16(o[j + u][i], a0, a1, a2, a3, pl[t][i][0], pl[t][i][1]);
                 }
               }
             }
         }
+        const int last = sync->block[st].last, next_unit = sync->block[st].next_unit, next_b = sync->block[st].next_b;
+        const bool ends = blk + 1 == (n_keys + kBlockKeys - 1) / kBlockKeys;
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&sync->empty[st]));
-      }
+        if (last == 0) continue;
 
-      // ---- the four warps' states meet: 2 and 3 with 0 and 1, then 1 with 0, which stores
-      const float back = r_exp == -CUDART_INF_F ? 0.f : ex2(0.5f * (r_exp - kProbShift));   // 2^(r - 9), in two factors
-#pragma unroll
-      for (int i = 0; i < NB; ++i) {
-#pragma unroll
-        for (int j = 0; j < D / 16; ++j)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) a.o[j][i][r] *= back * back;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) a.m[i][e] = a.m[i][e] == -CUDART_INF_F ? -CUDART_INF_F : a.m[i][e] * sl2[i][e];
-      }
-      if (warp >= 2) a.put(sync->meet[warp - 2], lane);
-      computing_warps_meet();
-      if (warp < 2) a.merge(sync->meet[warp], lane);
-      if (warp == 1) {
-        __syncwarp();
-        a.put(sync->meet[1], lane);
-      }
-      computing_warps_meet();
-      if (warp == 0) {
-        a.merge(sync->meet[1], lane);
+        // ---- the pair's last block here: every warp leaves its partial, the merge is the second launch's.  (A merge of the
+        // four in shared memory took longer than the few bytes more.)
+        const int64_t pair = static_cast<int64_t>(b) * list.units + unit;
+        const int64_t slot = pair + blockIdx.x;
+        if (tid == 0) {
+          if (first == 0) part.range[pair].x = static_cast<int>(slot);
+          if (ends) part.range[pair].y = static_cast<int>(slot);
+        }
+        const float back = r_exp == -CUDART_INF_F ? 0.f : ex2(0.5f * (r_exp - kProbShift));   // 2^(r - 9), in two factors
 #pragma unroll
         for (int i = 0; i < NB; ++i)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float sum = a.l[i][e];
+            float sum = lsum[i][e];
 #pragma unroll
-            for (int o = 4; o < 32; o *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            for (int d = 4; d < 32; d *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
             const int head = 8 * i + 2 * tq + e;
-            if (head >= n_heads || !dbg_range(p.status, DBG_DECODE_FP8 * 100 + 1, slot, 1, part.slots)) continue;
-            float* to = part.o + (slot * HEADS + head) * D;
+            if (unit / p.Hkv * HEADS + head >= p.group || !dbg_range(p.status, DBG_DECODE_FP8 * 100 + 1, slot, 1, part.slots)) continue;
+            const int64_t row = (slot * kWarps + warp) * HEADS + head;
 #pragma unroll
-            for (int j = 0; j < D / 16; ++j) *reinterpret_cast<float2*>(to + 16 * j + 2 * g) = make_float2(a.o[j][i][e], a.o[j][i][2 + e]);
-            if (g == 0) *reinterpret_cast<float2*>(part.ml + (slot * HEADS + head) * 2) = make_float2(a.m[i][e], sum);
+            for (int j = 0; j < D / 16; ++j)
+              *reinterpret_cast<float2*>(part.o + row * D + 16 * j + 2 * g) = make_float2(o[j][i][e] * back * back, o[j][i][2 + e] * back * back);
+            if (g == 0)
+              *reinterpret_cast<float2*>(part.ml + row * 2) = make_float2(m[i][e] == -CUDART_INF_F ? -CUDART_INF_F : m[i][e] * sl2[i][e], sum);
           }
+        b = next_b;
+        unit = next_unit;
+        fresh = true;
       }
-      computing_warps_meet();   // (the next pair's states go where warp 0 has just read)
-      // on to the next pair
-      c.left -= todo;
-      if (c.left > 0) c.next_pair(list);
     }
   }
   pdl_launch_dependents();
@@ -767,7 +718,7 @@ bool decode_fp8_geometry(const Problem& p, int kv_chunk, Fp8Geometry* g) {
   if (grid + pairs > 0x7fffffffLL) return false;
   g->grid = static_cast<int>(grid);
   g->slots = grid + pairs;
-  g->bytes = static_cast<uint64_t>(g->slots) * g->heads * (p.E + 2) * sizeof(float) + static_cast<uint64_t>(pairs) * sizeof(int2);
+  g->bytes = static_cast<uint64_t>(g->slots) * kWarps * g->heads * (p.E + 2) * sizeof(float) + static_cast<uint64_t>(pairs) * sizeof(int2);
   return true;
 }
 
