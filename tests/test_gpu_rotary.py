@@ -97,8 +97,17 @@ def test_gradient_against_differences():
         assert abs(slope.item() - (d.double() * step).sum().item()) <= x.numel() * 2.0**-22
     # twice differentiable: the gradient of the gradient is the rotation again
     y, _ = T.rotary_embedding(q, k, pos, freq, sections=(5, 7))
-    (d,) = torch.autograd.grad((wq * y).sum(), q, create_graph=True)
-    assert not d.requires_grad or d.grad_fn is not None
+    g1 = torch.randn(y.shape, generator=g).cuda().requires_grad_()
+    (d,) = torch.autograd.grad(y, q, g1, create_graph=True)
+    (again,) = torch.autograd.grad(d, g1, wq)
+    _check(again.cpu(), _want(wq.cpu(), pos.cpu(), freq.cpu(), (5, 7), False))
+    # the query alone, and only the keys' gradient
+    y, _ = T.rotary_embedding(q, None, pos, freq, sections=(5, 7))
+    (d,) = torch.autograd.grad(y, q, wq)
+    _check(d.cpu(), _want(wq.cpu(), pos.cpu(), freq.cpu(), (5, 7), False, -1.0))
+    _, z = T.rotary_embedding(q.detach(), k, pos, freq, sections=(5, 7))
+    (d,) = torch.autograd.grad(z, k, wk)
+    _check(d.cpu(), _want(wk.cpu(), pos.cpu(), freq.cpu(), (5, 7), False, -1.0))
 
 
 def test_strides_broadcasts_and_single_gradients():

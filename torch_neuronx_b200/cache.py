@@ -21,6 +21,14 @@ _HALF = (torch.float16, torch.bfloat16)
 _SCALE_DTYPES = (torch.float8_e8m0fnu, torch.uint8)
 
 
+_LAYOUTS = {"NHD": 1, "HND": 2}
+
+
+def _native():
+    """The direct entry points, where nothing is tracing."""
+    return None if _lib.native is None or torch.compiler.is_compiling() else _lib.native
+
+
 def _dims(layout: str):
     """(head dimension, row dimension) of a pool."""
     if layout not in ("NHD", "HND"):
@@ -117,6 +125,10 @@ def paged_write(
     for a row of zeros); its values are rounded once, to e4m3.  A row with a NaN or an infinity reads back as NaN.  A position
     behind the table's last page, or a page number outside the pool, drops the row and is reported by
     :func:`ops.check_device_status`.  Two rows of one call must not have the same place."""
+    native = _native()
+    if native is not None and layout in _LAYOUTS and native.paged_write(
+            key, value, k_pages, v_pages, k_scales, v_scales, block_table, start, lens, _LAYOUTS[layout]):
+        return
     if key.dim() != 4 or value.shape != key.shape:
         raise RuntimeError("paged_write: key and value must be 4-D (B, Hkv, L, D) and of the same shape")
     if key.dtype not in _HALF or value.dtype != key.dtype or value.device != key.device:
@@ -154,6 +166,11 @@ def paged_read(
     bf16 -- what :func:`ops.sdpa_forward` takes for the next chunk of a prompt.  Rows at or behind ``kv_lens[b]`` are zeros.
     ``max_len`` is the table's capacity by default.  bf16 holds every cached value exactly; fp16 rounds those below ``2^-14`` and
     overflows beyond 65504.  ``out`` is a pair of tensors to write into (any strides with a unit inner stride)."""
+    native = _native()
+    if native is not None and layout in _LAYOUTS and out is None and dtype in _HALF:
+        got = native.paged_read(k_pages, v_pages, k_scales, v_scales, block_table, kv_lens, max_len, dtype == torch.bfloat16, _LAYOUTS[layout])
+        if got is not None:
+            return got
     hd, rd = _dims(layout)
     if dtype not in _HALF:
         raise RuntimeError("paged_read: dtype must be float16 or bfloat16")
@@ -227,6 +244,12 @@ def decode_8bit(query, k_pages, v_pages, k_scales, v_scales, block_table, kv_len
 
 def _decode(op, query, k_pages, v_pages, k_scales, v_scales, block_table, kv_lens, scale, layout, out, lse, need_lse, kv_chunk,
             prefix_table, prefix_len):
+    native = _native()
+    if native is not None and layout in _LAYOUTS:
+        got = native.cache_decode(query, k_pages, v_pages, k_scales, v_scales, prefix_table, prefix_len, block_table, kv_lens, scale,
+                                  _LAYOUTS[layout], out, lse, need_lse, kv_chunk)
+        if got is not None:
+            return got
     hd, rd = _dims(layout)
     if query.dim() != 4 or query.shape[2] != 1:
         raise RuntimeError(f"{op}: query must be (B, Hq, 1, D) and the page pools 4-D")

@@ -34,6 +34,10 @@ def rotary_embedding(
     says how many consecutive pairs belong to each axis (their sum is ``R / 2``).  Pair ``i`` is elements ``(i, i + R / 2)``, or
     ``(2 i, 2 i + 1)`` when ``interleaved``, and is turned by ``positions[axis of i] * inv_freq[i]``, an angle that is formed in
     64 bits; the rest is computed in 32 and rounded once.  Gradients flow to ``query`` and ``key``."""
+    if _lib.native is not None and not torch.compiler.is_compiling():
+        got = _lib.native.rotary(query, key, positions, inv_freq, sections, interleaved)
+        if got is not None:
+            return got
     args = _check(query, key, positions, inv_freq, sections)
     wants = torch.is_grad_enabled() and (query.requires_grad or (key is not None and key.requires_grad))
     if wants:
