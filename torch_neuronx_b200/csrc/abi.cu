@@ -344,6 +344,10 @@ int validate_rows(const B200CacheRowsParams* a) {
       a->v_scales == nullptr || a->block_table == nullptr)
     return B200_SDPA_ERR_NULL;
   if (!pool_aligned(a->k_pages, a->k_pages_stride, 1) || !pool_aligned(a->v_pages, a->v_pages_stride, 1)) return B200_SDPA_ERR_ALIGNMENT;
+  for (int i = 0; i < 3; ++i)   // (but for the batch's, strides are multiplied in 32 bits)
+    for (int64_t s : {a->k_pages_stride[i], a->v_pages_stride[i], a->k_scales_stride[i], a->v_scales_stride[i], i > 0 ? a->k_stride[i] : 0,
+                      i > 0 ? a->v_stride[i] : 0})
+      if (s < 0 || s > 0x7fffffffLL) return B200_SDPA_ERR_UNSUPPORTED;
   return B200_SDPA_OK;
 }
 

@@ -29,7 +29,13 @@ __device__ __forceinline__ bool locate(const B200CacheRowsParams& p, int page_sh
   return *page >= 0 && *page < p.n_pages;
 }
 
-template <bool BF16, int LPR>   // LPR: lanes of a row, a power of two >= D / 8
+// The largest magnitude of eight 16-bit elements, as bits of their type: both types order like their bits without the sign.
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) { return __vmaxu2(a, b); }
+
+// LPR: lanes of a row, a power of two >= D / 8.  One CTA: `tokens` tokens of the keys or of the values of one sequence.  A thread's place
+// (token, head) moves on by fixed steps and offsets are 32 x 32 bits: in the first form, which divided for each row and chose between
+// keys and values in the loop, instructions and not bytes were the bound (16 prompts of 512..4096 tokens, 8 heads of 128: 82 us).
+template <bool BF16, int LPR>
 __global__ void __launch_bounds__(kThreads) cache_write_kernel(const B200CacheRowsParams p, const int page_shift, const int tokens,
                                                                const int rows_16b) {
   constexpr int kRows = kThreads / LPR;
@@ -40,57 +46,62 @@ __global__ void __launch_bounds__(kThreads) cache_write_kernel(const B200CacheRo
   n = n < p.L ? n : p.L;
   const int n_tok = n - i0 < tokens ? n - i0 : tokens;
   if (n_tok <= 0) return;
+  const bool is_v = blockIdx.z != 0;
+  const uint32_t x_head = static_cast<uint32_t>(is_v ? p.v_stride[1] : p.k_stride[1]), x_row = static_cast<uint32_t>(is_v ? p.v_stride[2] : p.k_stride[2]);
+  const uint32_t y_page = static_cast<uint32_t>(is_v ? p.v_pages_stride[0] : p.k_pages_stride[0]);
+  const uint32_t y_head = static_cast<uint32_t>(is_v ? p.v_pages_stride[1] : p.k_pages_stride[1]), y_row = static_cast<uint32_t>(is_v ? p.v_pages_stride[2] : p.k_pages_stride[2]);
+  const uint32_t s_page = static_cast<uint32_t>(is_v ? p.v_scales_stride[0] : p.k_scales_stride[0]);
+  const uint32_t s_head = static_cast<uint32_t>(is_v ? p.v_scales_stride[1] : p.k_scales_stride[1]), s_row = static_cast<uint32_t>(is_v ? p.v_scales_stride[2] : p.k_scales_stride[2]);
   const int lane = threadIdx.x % LPR, c0 = lane * 8;
+  const uint16_t* x = static_cast<const uint16_t*>(is_v ? p.v : p.k) + b * (is_v ? p.v_stride[0] : p.k_stride[0]) +
+                      static_cast<int64_t>(i0) * x_row + c0;
+  uint8_t* pages = static_cast<uint8_t*>(is_v ? p.v_pages : p.k_pages) + c0;
+  uint8_t* scales = static_cast<uint8_t*>(is_v ? p.v_scales : p.k_scales);
+  const int* table = p.block_table + static_cast<int64_t>(b) * p.block_table_stride;
   const int64_t start = p.start[b];
-  const int total = n_tok * 2 * p.Hkv;
-  for (int r = threadIdx.x / LPR; r < (total + kRows - 1) / kRows * kRows; r += kRows) {   // (whole warps: the maximum meets)
-    const int t = r / (2 * p.Hkv);
-    int h = r - t * 2 * p.Hkv;
-    const bool is_v = h >= p.Hkv;
-    h -= is_v ? p.Hkv : 0;
-    const int64_t* xs = is_v ? p.v_stride : p.k_stride;
-    const uint16_t* x = static_cast<const uint16_t*>(is_v ? p.v : p.k) + b * xs[0] + h * xs[1] + (i0 + t) * xs[2] + c0;
-    const bool on = r < total && c0 < p.D;
-    __align__(16) uint16_t e[8] = {};
+  const int first = threadIdx.x / LPR, d_h = kRows % p.Hkv, d_t = kRows / p.Hkv;
+  int h = first % p.Hkv, t = first / p.Hkv;
+  const int rounds = (n_tok * p.Hkv + kRows - 1) / kRows;   // (whole warps walk on together: the maximum meets over a row's lanes)
+  for (int i = 0; i < rounds; ++i) {
+    const bool on = t < n_tok && c0 < p.D;
+    __align__(16) uint32_t e[4] = {0u, 0u, 0u, 0u};
+    int entry = -1;
+    const int64_t pos = start + i0 + t;
     if (on) {
-      if (rows_16b) *reinterpret_cast<uint4*>(e) = *reinterpret_cast<const uint4*>(x);
+      const uint16_t* from = x + static_cast<uint64_t>(static_cast<uint32_t>(h)) * x_head + static_cast<uint64_t>(static_cast<uint32_t>(t)) * x_row;
+      if (rows_16b) *reinterpret_cast<uint4*>(e) = ld_stream_16B(from);
       else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) e[i] = x[i];
+        for (int k = 0; k < 4; ++k) e[k] = from[2 * k] | static_cast<uint32_t>(from[2 * k + 1]) << 16;
+      }
+      if (pos >= 0 && (pos >> page_shift) < p.block_table_stride) entry = table[pos >> page_shift];
+    }
+    uint32_t top2 = max_u16x2(max_u16x2(e[0] & 0x7fff7fffu, e[1] & 0x7fff7fffu), max_u16x2(e[2] & 0x7fff7fffu, e[3] & 0x7fff7fffu));
+#pragma unroll
+    for (int o = LPR / 2; o > 0; o >>= 1) top2 = max_u16x2(top2, __shfl_xor_sync(0xffffffffu, top2, o));
+    if (on) {
+      const uint32_t top = top2 >> 16 > (top2 & 0xffffu) ? top2 >> 16 : top2 & 0xffffu;
+      const int code = scale_code(__float_as_uint(half_to_f32<BF16>(static_cast<uint16_t>(top))));
+      if (static_cast<unsigned>(entry) < static_cast<unsigned>(p.n_pages)) {
+        const float inv = scale_inverse(code);
+        uint32_t w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          w[k] = pack_e4m3(half_to_f32<BF16>(static_cast<uint16_t>(e[k])) * inv, half_to_f32<BF16>(static_cast<uint16_t>(e[k] >> 16)) * inv);
+        const uint64_t page = static_cast<uint32_t>(entry), row = static_cast<uint32_t>(pos) & ((1u << page_shift) - 1), head = static_cast<uint32_t>(h);
+        *reinterpret_cast<uint2*>(pages + page * y_page + head * y_head + row * y_row) = make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
+        if (lane == 0) scales[page * s_page + head * s_head + row * s_row] = static_cast<uint8_t>(code);
+      } else {
+        const bool full = pos >= (static_cast<int64_t>(p.block_table_stride) << page_shift);
+        report_page(p.status, full ? B200_SDPA_ERR_CACHE_FULL : B200_SDPA_ERR_PAGE, b, static_cast<int>(pos), p.n_pages);
       }
     }
-    float f[8];
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      f[i] = half_to_f32<BF16>(e[i]);
-      const uint32_t m = __float_as_uint(f[i]) & 0x7fffffffu;
-      top = m > top ? m : top;
+    h += d_h;
+    t += d_t;
+    if (h >= p.Hkv) {
+      h -= p.Hkv;
+      ++t;
     }
-#pragma unroll
-    for (int o = LPR / 2; o > 0; o >>= 1) {
-      const uint32_t m = __shfl_xor_sync(0xffffffffu, top, o);
-      top = m > top ? m : top;
-    }
-    if (!on) continue;
-    const int code = scale_code(top);
-    const float inv = scale_inverse(code);
-    uint2 w;
-    w.x = pack_e4m3(f[0] * inv, f[1] * inv) | pack_e4m3(f[2] * inv, f[3] * inv) << 16;
-    w.y = pack_e4m3(f[4] * inv, f[5] * inv) | pack_e4m3(f[6] * inv, f[7] * inv) << 16;
-    int64_t page;
-    int row;
-    if (!locate(p, page_shift, b, start + i0 + t, &page, &row)) {
-      const int64_t pos = start + i0 + t;
-      const bool full = pos >= (static_cast<int64_t>(p.block_table_stride) << page_shift);
-      report_page(p.status, full ? B200_SDPA_ERR_CACHE_FULL : B200_SDPA_ERR_PAGE, b, static_cast<int>(pos), p.n_pages);
-      continue;
-    }
-    const int64_t* ps = is_v ? p.v_pages_stride : p.k_pages_stride;
-    const int64_t* ss = is_v ? p.v_scales_stride : p.k_scales_stride;
-    uint8_t* dst = static_cast<uint8_t*>(is_v ? p.v_pages : p.k_pages) + page * ps[0] + h * ps[1] + row * ps[2] + c0;
-    *reinterpret_cast<uint2*>(dst) = w;
-    if (lane == 0) static_cast<uint8_t*>(is_v ? p.v_scales : p.k_scales)[page * ss[0] + h * ss[1] + row * ss[2]] = static_cast<uint8_t>(code);
   }
 }
 
@@ -153,9 +164,10 @@ __global__ void __launch_bounds__(kThreads) cache_read_kernel(const B200CacheRow
   }
 }
 
-// Tokens of one CTA: enough for a few rounds of its threads, fewer where there would not be several CTAs for every SM.
-int tokens_per_cta(const B200CacheRowsParams& p, int rows_per_round) {
-  int tokens = (4 * rows_per_round + 2 * p.Hkv - 1) / (2 * p.Hkv);
+// Tokens of one CTA, `heads` rows each: enough for a few rounds of its threads, fewer where there would not be several CTAs for every SM.
+int tokens_per_cta(const B200CacheRowsParams& p, int rows_per_round, int heads) {
+  constexpr int kRounds = 4;
+  int tokens = (kRounds * rows_per_round + heads - 1) / heads;
   tokens = tokens < 1 ? 1 : tokens;
   while (tokens > 1 && static_cast<int64_t>(p.B) * ((p.L + tokens - 1) / tokens) < 4 * 148) tokens = (tokens + 1) / 2;
   return tokens;
@@ -178,8 +190,8 @@ bool rows_16b(const B200CacheRowsParams& p) {
 enum Direction { WRITE, READ, GATHER };
 
 template <Direction DIR, bool BF16, int LPR> int launch_rows(const B200CacheRowsParams& p, cudaStream_t stream) {
-  const int tokens = tokens_per_cta(p, kThreads / LPR);
-  const dim3 grid((p.L + tokens - 1) / tokens, p.B);
+  const int tokens = tokens_per_cta(p, kThreads / LPR, DIR == WRITE ? p.Hkv : 2 * p.Hkv);
+  const dim3 grid((p.L + tokens - 1) / tokens, p.B, DIR == WRITE ? 2 : 1);
   const int shift = page_shift_of(p.page_size);
   bool ok;
   if constexpr (DIR == WRITE) ok = launch_pdl(cache_write_kernel<BF16, LPR>, grid, kThreads, 0, stream, p, shift, tokens, rows_16b(p) ? 1 : 0);

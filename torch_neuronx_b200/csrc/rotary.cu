@@ -67,63 +67,68 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryArgs a) {
   __syncthreads();
 
   const int rot_items = a.pairs / V, items = rot_items + (p.D - p.rot) / (2 * V);   // of one head
-  const int heads = p.heads[0] + p.heads[1];
-  const int total = n_tok * heads * items;
-  for (int i = threadIdx.x; i < total; i += kThreads) {
-    const int row = i / items, it = i - row * items;
-    const int t = row / heads;
-    int h = row - t * heads;
-    const int which = h >= p.heads[0] ? 1 : 0;
-    h -= which ? p.heads[0] : 0;
-    const int64_t* xs = p.x_stride[which];
-    const int64_t* ys = p.y_stride[which];
-    const T* x = static_cast<const T*>(p.x[which]) + b * xs[0] + h * xs[1] + (l0 + t) * xs[2];
-    T* y = static_cast<T*>(p.y[which]) + b * ys[0] + h * ys[1] + (l0 + t) * ys[2];
-    // the two pieces of the item: the halves of V pairs, or 2 V neighbouring elements
-    int e0, e1;
-    if (it >= rot_items) {
-      e0 = p.rot + (it - rot_items) * 2 * V;
-      e1 = e0 + V;
-    } else if (p.interleaved) {
-      e0 = it * 2 * V;
-      e1 = e0 + V;
-    } else {
-      e0 = it * V;
-      e1 = e0 + a.pairs;
-    }
+  // The heads of the queries, then of the keys.  A thread's place (token, head, item) moves on by fixed steps: dividing for
+  // each item cost as much as the rotation.
+  auto walk = [&](const T* x, T* y, const int64_t(&xs)[4], const int64_t(&ys)[4], const int heads) {
+    if (heads == 0) return;
     const int64_t xi = V > 1 ? 1 : xs[3], yi = V > 1 ? 1 : ys[3];
-    __align__(16) T u[V], w[V];
-    *reinterpret_cast<W*>(u) = *reinterpret_cast<const W*>(x + e0 * xi);
-    *reinterpret_cast<W*>(w) = *reinterpret_cast<const W*>(x + e1 * xi);
-    if (it < rot_items) {
-      const float2* cs = turns + t * a.pairs + it * V;
-      if (p.interleaved && V > 1) {
-        // piece u holds pairs 0 .. V/2 - 1, piece w the others
+    x += b * xs[0] + l0 * xs[2];
+    y += b * ys[0] + l0 * ys[2];
+    int it = threadIdx.x % items, h = threadIdx.x / items % heads, t = threadIdx.x / items / heads;
+    const int d_it = kThreads % items, d_h = kThreads / items % heads, d_t = kThreads / items / heads;
+    while (t < n_tok) {
+      // the two pieces of the item: the halves of V pairs, or 2 V neighbouring elements
+      const bool tail = it >= rot_items;
+      const int e0 = tail ? p.rot + (it - rot_items) * 2 * V : (p.interleaved ? it * 2 * V : it * V);
+      const int e1 = tail || p.interleaved ? e0 + V : e0 + a.pairs;
+      const T* from = x + h * xs[1] + t * xs[2];
+      __align__(16) T u[V], w[V];
+      *reinterpret_cast<W*>(u) = *reinterpret_cast<const W*>(from + e0 * xi);
+      *reinterpret_cast<W*>(w) = *reinterpret_cast<const W*>(from + e1 * xi);
+      if (!tail) {
+        const float2* cs = turns + t * a.pairs + it * V;
+        if (p.interleaved && V > 1) {
+          // piece u holds pairs 0 .. V/2 - 1, piece w the others
 #pragma unroll
-        for (int e = 0; e + 1 < V; e += 2) {
-          const float2 c0 = cs[e / 2], c1 = cs[V / 2 + e / 2];
-          const float u0 = to_f32<T>(u[e]), u1 = to_f32<T>(u[e + 1]), w0 = to_f32<T>(w[e]), w1 = to_f32<T>(w[e + 1]);
-          u[e] = from_f32<T>(fmaf(-u1, c0.y, u0 * c0.x));
-          u[e + 1] = from_f32<T>(fmaf(u0, c0.y, u1 * c0.x));
-          w[e] = from_f32<T>(fmaf(-w1, c1.y, w0 * c1.x));
-          w[e + 1] = from_f32<T>(fmaf(w0, c1.y, w1 * c1.x));
-        }
-      } else {
+          for (int e = 0; e + 1 < V; e += 2) {
+            const float2 c0 = cs[e / 2], c1 = cs[V / 2 + e / 2];
+            const float u0 = to_f32<T>(u[e]), u1 = to_f32<T>(u[e + 1]), w0 = to_f32<T>(w[e]), w1 = to_f32<T>(w[e + 1]);
+            u[e] = from_f32<T>(fmaf(-u1, c0.y, u0 * c0.x));
+            u[e + 1] = from_f32<T>(fmaf(u0, c0.y, u1 * c0.x));
+            w[e] = from_f32<T>(fmaf(-w1, c1.y, w0 * c1.x));
+            w[e + 1] = from_f32<T>(fmaf(w0, c1.y, w1 * c1.x));
+          }
+        } else {
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const float2 c = cs[e];
-          const float x0 = to_f32<T>(u[e]), x1 = to_f32<T>(w[e]);
-          u[e] = from_f32<T>(fmaf(-x1, c.y, x0 * c.x));
-          w[e] = from_f32<T>(fmaf(x0, c.y, x1 * c.x));
+          for (int e = 0; e < V; ++e) {
+            const float2 c = cs[e];
+            const float x0 = to_f32<T>(u[e]), x1 = to_f32<T>(w[e]);
+            u[e] = from_f32<T>(fmaf(-x1, c.y, x0 * c.x));
+            w[e] = from_f32<T>(fmaf(x0, c.y, x1 * c.x));
+          }
         }
       }
+      if (dbg_bhrc(p.status, DBG_ROTARY * 100 + 1, b, p.B, h, heads, l0 + t, p.L, e0, V, p.D) &&
+          dbg_range(p.status, DBG_ROTARY * 100 + 2, e1, V, p.D)) {
+        T* to = y + h * ys[1] + t * ys[2];
+        *reinterpret_cast<W*>(to + e0 * yi) = *reinterpret_cast<const W*>(u);
+        *reinterpret_cast<W*>(to + e1 * yi) = *reinterpret_cast<const W*>(w);
+      }
+      it += d_it;
+      h += d_h;
+      t += d_t;
+      if (it >= items) {
+        it -= items;
+        ++h;
+      }
+      if (h >= heads) {
+        h -= heads;
+        ++t;
+      }
     }
-    if (!dbg_bhrc(p.status, DBG_ROTARY * 100 + 1, b, p.B, h, p.heads[which], l0 + t, p.L, e0, V, p.D) ||
-        !dbg_range(p.status, DBG_ROTARY * 100 + 2, e1, V, p.D))
-      continue;
-    *reinterpret_cast<W*>(y + e0 * yi) = *reinterpret_cast<const W*>(u);
-    *reinterpret_cast<W*>(y + e1 * yi) = *reinterpret_cast<const W*>(w);
-  }
+  };
+  walk(static_cast<const T*>(p.x[0]), static_cast<T*>(p.y[0]), p.x_stride[0], p.y_stride[0], p.heads[0]);
+  walk(static_cast<const T*>(p.x[1]), static_cast<T*>(p.y[1]), p.x_stride[1], p.y_stride[1], p.heads[1]);
 }
 
 template <typename T, int V> int launch_typed(const RotaryArgs& a, cudaStream_t stream) {
