@@ -7,8 +7,8 @@
 // exact in bf16, so reading back rounds nothing (fp16: once, below 2^-14 and beyond 65504).  A row of zeros has e = 0; a
 // row with a NaN or an infinity has the scale NaN (255) and reads as NaN; e is at least -127.
 //
-// Bound by HBM.  Writing: a row is D / 8 lanes with 8 elements each (one 16-byte load, one 8-byte store), the maximum
-// meets over those lanes.  Reading: D / 16 lanes with 16 elements each (one 16-byte load, two 16-byte stores).
+// Bound by HBM.  A row is D / 16 lanes with 16 elements each: 32 bytes on the 16-bit side, 16 on the other; writing, the maximum
+// meets over those lanes.
 // A page number outside the pool is reported through the status word and nothing is read or written there.
 #include "common.cuh"
 #include "debug.cuh"
@@ -29,10 +29,18 @@ __device__ __forceinline__ bool locate(const B200CacheRowsParams& p, int page_sh
   return *page >= 0 && *page < p.n_pages;
 }
 
-// The largest magnitude of eight 16-bit elements, as bits of their type: both types order like their bits without the sign.
-__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) { return __vmaxu2(a, b); }
+// The larger of two pairs of 16-bit numbers, a NaN where there is one.
+template <bool BF16> __device__ __forceinline__ uint32_t max_pair(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if (BF16) {
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  } else {
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  }
+  return r;
+}
 
-// LPR: lanes of a row, a power of two >= D / 8.  One CTA: `tokens` tokens of the keys or of the values of one sequence.  A thread's place
+// LPR: lanes of a row, a power of two >= D / 16.  One CTA: `tokens` tokens of the keys or of the values of one sequence.  A thread's place
 // (token, head) moves on by fixed steps and offsets are 32 x 32 bits: in the first form, which divided for each row and chose between
 // keys and values in the loop, instructions and not bytes were the bound (16 prompts of 512..4096 tokens, 8 heads of 128: 82 us).
 template <bool BF16, int LPR>
@@ -52,7 +60,7 @@ __global__ void __launch_bounds__(kThreads) cache_write_kernel(const B200CacheRo
   const uint32_t y_head = static_cast<uint32_t>(is_v ? p.v_pages_stride[1] : p.k_pages_stride[1]), y_row = static_cast<uint32_t>(is_v ? p.v_pages_stride[2] : p.k_pages_stride[2]);
   const uint32_t s_page = static_cast<uint32_t>(is_v ? p.v_scales_stride[0] : p.k_scales_stride[0]);
   const uint32_t s_head = static_cast<uint32_t>(is_v ? p.v_scales_stride[1] : p.k_scales_stride[1]), s_row = static_cast<uint32_t>(is_v ? p.v_scales_stride[2] : p.k_scales_stride[2]);
-  const int lane = threadIdx.x % LPR, c0 = lane * 8;
+  const int lane = threadIdx.x % LPR, c0 = lane * 16;
   const uint16_t* x = static_cast<const uint16_t*>(is_v ? p.v : p.k) + b * (is_v ? p.v_stride[0] : p.k_stride[0]) +
                       static_cast<int64_t>(i0) * x_row + c0;
   uint8_t* pages = static_cast<uint8_t*>(is_v ? p.v_pages : p.k_pages) + c0;
@@ -62,45 +70,61 @@ __global__ void __launch_bounds__(kThreads) cache_write_kernel(const B200CacheRo
   const int first = threadIdx.x / LPR, d_h = kRows % p.Hkv, d_t = kRows / p.Hkv;
   int h = first % p.Hkv, t = first / p.Hkv;
   const int rounds = (n_tok * p.Hkv + kRows - 1) / kRows;   // (whole warps walk on together: the maximum meets over a row's lanes)
+  __align__(16) uint32_t e[8], next[8];
+  int next_entry;
+  auto fetch = [&]() {   // the row at (t, h) and its page
+#pragma unroll
+    for (int k = 0; k < 8; ++k) next[k] = 0u;
+    next_entry = -1;
+    if (t >= n_tok || c0 >= p.D) return;
+    const uint16_t* from = x + static_cast<uint64_t>(static_cast<uint32_t>(h)) * x_head + static_cast<uint64_t>(static_cast<uint32_t>(t)) * x_row;
+    if (rows_16b) {
+      *reinterpret_cast<uint4*>(next) = ld_stream_16B(from);
+      *reinterpret_cast<uint4*>(next + 4) = ld_stream_16B(from + 8);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) next[k] = from[2 * k] | static_cast<uint32_t>(from[2 * k + 1]) << 16;
+    }
+    const int64_t pos = start + i0 + t;
+    if (pos >= 0 && (pos >> page_shift) < p.block_table_stride) next_entry = table[pos >> page_shift];
+  };
+  fetch();
   for (int i = 0; i < rounds; ++i) {
     const bool on = t < n_tok && c0 < p.D;
-    __align__(16) uint32_t e[4] = {0u, 0u, 0u, 0u};
-    int entry = -1;
     const int64_t pos = start + i0 + t;
-    if (on) {
-      const uint16_t* from = x + static_cast<uint64_t>(static_cast<uint32_t>(h)) * x_head + static_cast<uint64_t>(static_cast<uint32_t>(t)) * x_row;
-      if (rows_16b) *reinterpret_cast<uint4*>(e) = ld_stream_16B(from);
-      else {
+    const int entry = next_entry;
+    const uint64_t head = static_cast<uint32_t>(h);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) e[k] = from[2 * k] | static_cast<uint32_t>(from[2 * k + 1]) << 16;
-      }
-      if (pos >= 0 && (pos >> page_shift) < p.block_table_stride) entry = table[pos >> page_shift];
-    }
-    uint32_t top2 = max_u16x2(max_u16x2(e[0] & 0x7fff7fffu, e[1] & 0x7fff7fffu), max_u16x2(e[2] & 0x7fff7fffu, e[3] & 0x7fff7fffu));
-#pragma unroll
-    for (int o = LPR / 2; o > 0; o >>= 1) top2 = max_u16x2(top2, __shfl_xor_sync(0xffffffffu, top2, o));
-    if (on) {
-      const uint32_t top = top2 >> 16 > (top2 & 0xffffu) ? top2 >> 16 : top2 & 0xffffu;
-      const int code = scale_code(__float_as_uint(half_to_f32<BF16>(static_cast<uint16_t>(top))));
-      if (static_cast<unsigned>(entry) < static_cast<unsigned>(p.n_pages)) {
-        const float inv = scale_inverse(code);
-        uint32_t w[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          w[k] = pack_e4m3(half_to_f32<BF16>(static_cast<uint16_t>(e[k])) * inv, half_to_f32<BF16>(static_cast<uint16_t>(e[k] >> 16)) * inv);
-        const uint64_t page = static_cast<uint32_t>(entry), row = static_cast<uint32_t>(pos) & ((1u << page_shift) - 1), head = static_cast<uint32_t>(h);
-        *reinterpret_cast<uint2*>(pages + page * y_page + head * y_head + row * y_row) = make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
-        if (lane == 0) scales[page * s_page + head * s_head + row * s_row] = static_cast<uint8_t>(code);
-      } else {
-        const bool full = pos >= (static_cast<int64_t>(p.block_table_stride) << page_shift);
-        report_page(p.status, full ? B200_SDPA_ERR_CACHE_FULL : B200_SDPA_ERR_PAGE, b, static_cast<int>(pos), p.n_pages);
-      }
-    }
+    for (int k = 0; k < 8; ++k) e[k] = next[k];
     h += d_h;
     t += d_t;
     if (h >= p.Hkv) {
       h -= p.Hkv;
       ++t;
+    }
+    fetch();   // (the next row travels while this one is rounded)
+    uint32_t top2 = e[0] & 0x7fff7fffu;
+#pragma unroll
+    for (int k = 1; k < 8; ++k) top2 = max_pair<BF16>(top2, e[k] & 0x7fff7fffu);
+#pragma unroll
+    for (int o = LPR / 2; o > 0; o >>= 1) top2 = max_pair<BF16>(top2, __shfl_xor_sync(0xffffffffu, top2, o));
+    if (on) {
+      const uint32_t top = top2 >> 16 > (top2 & 0xffffu) ? top2 >> 16 : top2 & 0xffffu;   // (bits order like magnitudes)
+      const int code = scale_code(__float_as_uint(half_to_f32<BF16>(static_cast<uint16_t>(top))));
+      if (static_cast<unsigned>(entry) < static_cast<unsigned>(p.n_pages)) {
+        const float inv = scale_inverse(code);
+        uint32_t w[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          w[k] = pack_e4m3(half_to_f32<BF16>(static_cast<uint16_t>(e[k])) * inv, half_to_f32<BF16>(static_cast<uint16_t>(e[k] >> 16)) * inv);
+        const uint64_t page = static_cast<uint32_t>(entry), row = static_cast<uint32_t>(pos) & ((1u << page_shift) - 1);
+        *reinterpret_cast<uint4*>(pages + page * y_page + head * y_head + row * y_row) =
+            make_uint4(w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16);
+        if (lane == 0) scales[page * s_page + head * s_head + row * s_row] = static_cast<uint8_t>(code);
+      } else {
+        const bool full = pos >= (static_cast<int64_t>(p.block_table_stride) << page_shift);
+        report_page(p.status, full ? B200_SDPA_ERR_CACHE_FULL : B200_SDPA_ERR_PAGE, b, static_cast<int>(pos), p.n_pages);
+      }
     }
   }
 }
@@ -202,11 +226,10 @@ template <Direction DIR, bool BF16, int LPR> int launch_rows(const B200CacheRows
 }
 
 template <Direction DIR, bool BF16> int launch_lanes(const B200CacheRowsParams& p, cudaStream_t stream) {
-  const int lanes = p.D / (DIR == WRITE ? 8 : 16);
+  const int lanes = p.D / 16;
   if (lanes <= 4) return launch_rows<DIR, BF16, 4>(p, stream);
   if (lanes <= 8) return launch_rows<DIR, BF16, 8>(p, stream);
-  if (lanes <= 16) return launch_rows<DIR, BF16, 16>(p, stream);
-  return launch_rows<DIR, BF16, 32>(p, stream);
+  return launch_rows<DIR, BF16, 16>(p, stream);
 }
 
 }  // namespace

@@ -53,40 +53,50 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryArgs a) {
   const int n_tok = p.L - l0 < a.tokens ? p.L - l0 : a.tokens;
   pdl_wait();
   pdl_launch_dependents();
-  for (int i = threadIdx.x; i < n_tok * a.pairs; i += kThreads) {
-    const int t = i / a.pairs, pair = i - t * a.pairs;
-    int axis = 0, end = p.section[0];
-    while (axis + 1 < p.axes && pair >= end) end += p.section[++axis];
-    const int64_t at = axis * p.pos_stride[0] + b * p.pos_stride[1] + (l0 + t) * p.pos_stride[2];
-    const double pos = p.positions_i64 ? static_cast<double>(static_cast<const int64_t*>(p.positions)[at])
-                                       : static_cast<double>(static_cast<const int32_t*>(p.positions)[at]);
-    const double freq = p.inv_freq_f64 ? static_cast<const double*>(p.inv_freq)[pair]
-                                       : static_cast<double>(static_cast<const float*>(p.inv_freq)[pair]);
-    turns[i] = turn_of(pos, freq, p.inverse != 0);
-  }
-  __syncthreads();
-
   const int rot_items = a.pairs / V, items = rot_items + (p.D - p.rot) / (2 * V);   // of one head
   // The heads of the queries, then of the keys.  A thread's place (token, head, item) moves on by fixed steps: dividing for
   // each item cost as much as the rotation.
-  auto walk = [&](const T* x, T* y, const int64_t(&xs)[4], const int64_t(&ys)[4], const int heads) {
+  // The next item's pieces travel while one is turned, the first ones while the sines and cosines are made.
+  auto walk = [&](const T* x, T* y, const int64_t(&xs)[4], const int64_t(&ys)[4], const int heads, auto before) {
     if (heads == 0) return;
     const int64_t xi = V > 1 ? 1 : xs[3], yi = V > 1 ? 1 : ys[3];
     x += b * xs[0] + l0 * xs[2];
     y += b * ys[0] + l0 * ys[2];
     int it = threadIdx.x % items, h = threadIdx.x / items % heads, t = threadIdx.x / items / heads;
     const int d_it = kThreads % items, d_h = kThreads / items % heads, d_t = kThreads / items / heads;
+    __align__(16) T u[V], w[V], next_u[V], next_w[V];
+    // the two pieces of an item: the halves of V pairs, or 2 V neighbouring elements
+    auto piece0 = [&](int i) { return i >= rot_items ? p.rot + (i - rot_items) * 2 * V : (p.interleaved ? i * 2 * V : i * V); };
+    auto piece1 = [&](int i, int e0) { return i >= rot_items || p.interleaved ? e0 + V : e0 + a.pairs; };
+    auto fetch = [&](int i, int hd, int tk) {
+      if (tk >= n_tok) return;
+      const int e0 = piece0(i), e1 = piece1(i, e0);
+      const T* from = x + hd * xs[1] + tk * xs[2];
+      *reinterpret_cast<W*>(next_u) = *reinterpret_cast<const W*>(from + e0 * xi);
+      *reinterpret_cast<W*>(next_w) = *reinterpret_cast<const W*>(from + e1 * xi);
+    };
+    fetch(it, h, t);
+    before();
     while (t < n_tok) {
-      // the two pieces of the item: the halves of V pairs, or 2 V neighbouring elements
+      const int e0 = piece0(it), e1 = piece1(it, e0);
       const bool tail = it >= rot_items;
-      const int e0 = tail ? p.rot + (it - rot_items) * 2 * V : (p.interleaved ? it * 2 * V : it * V);
-      const int e1 = tail || p.interleaved ? e0 + V : e0 + a.pairs;
-      const T* from = x + h * xs[1] + t * xs[2];
-      __align__(16) T u[V], w[V];
-      *reinterpret_cast<W*>(u) = *reinterpret_cast<const W*>(from + e0 * xi);
-      *reinterpret_cast<W*>(w) = *reinterpret_cast<const W*>(from + e1 * xi);
+      *reinterpret_cast<W*>(u) = *reinterpret_cast<const W*>(next_u);
+      *reinterpret_cast<W*>(w) = *reinterpret_cast<const W*>(next_w);
+      const int at_it = it, at_h = h, at_t = t;
+      it += d_it;
+      h += d_h;
+      t += d_t;
+      if (it >= items) {
+        it -= items;
+        ++h;
+      }
+      if (h >= heads) {
+        h -= heads;
+        ++t;
+      }
+      fetch(it, h, t);
       if (!tail) {
-        const float2* cs = turns + t * a.pairs + it * V;
+        const float2* cs = turns + at_t * a.pairs + at_it * V;
         if (p.interleaved && V > 1) {
           // piece u holds pairs 0 .. V/2 - 1, piece w the others
 #pragma unroll
@@ -108,27 +118,30 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryArgs a) {
           }
         }
       }
-      if (dbg_bhrc(p.status, DBG_ROTARY * 100 + 1, b, p.B, h, heads, l0 + t, p.L, e0, V, p.D) &&
+      if (dbg_bhrc(p.status, DBG_ROTARY * 100 + 1, b, p.B, at_h, heads, l0 + at_t, p.L, e0, V, p.D) &&
           dbg_range(p.status, DBG_ROTARY * 100 + 2, e1, V, p.D)) {
-        T* to = y + h * ys[1] + t * ys[2];
+        T* to = y + at_h * ys[1] + at_t * ys[2];
         *reinterpret_cast<W*>(to + e0 * yi) = *reinterpret_cast<const W*>(u);
         *reinterpret_cast<W*>(to + e1 * yi) = *reinterpret_cast<const W*>(w);
       }
-      it += d_it;
-      h += d_h;
-      t += d_t;
-      if (it >= items) {
-        it -= items;
-        ++h;
-      }
-      if (h >= heads) {
-        h -= heads;
-        ++t;
-      }
     }
   };
-  walk(static_cast<const T*>(p.x[0]), static_cast<T*>(p.y[0]), p.x_stride[0], p.y_stride[0], p.heads[0]);
-  walk(static_cast<const T*>(p.x[1]), static_cast<T*>(p.y[1]), p.x_stride[1], p.y_stride[1], p.heads[1]);
+  auto make_turns = [&]() {
+    for (int i = threadIdx.x; i < n_tok * a.pairs; i += kThreads) {
+      const int t = i / a.pairs, pair = i - t * a.pairs;
+      int axis = 0, end = p.section[0];
+      while (axis + 1 < p.axes && pair >= end) end += p.section[++axis];
+      const int64_t at = axis * p.pos_stride[0] + b * p.pos_stride[1] + (l0 + t) * p.pos_stride[2];
+      const double pos = p.positions_i64 ? static_cast<double>(static_cast<const int64_t*>(p.positions)[at])
+                                         : static_cast<double>(static_cast<const int32_t*>(p.positions)[at]);
+      const double freq = p.inv_freq_f64 ? static_cast<const double*>(p.inv_freq)[pair]
+                                         : static_cast<double>(static_cast<const float*>(p.inv_freq)[pair]);
+      turns[i] = turn_of(pos, freq, p.inverse != 0);
+    }
+    __syncthreads();
+  };
+  walk(static_cast<const T*>(p.x[0]), static_cast<T*>(p.y[0]), p.x_stride[0], p.y_stride[0], p.heads[0], make_turns);
+  walk(static_cast<const T*>(p.x[1]), static_cast<T*>(p.y[1]), p.x_stride[1], p.y_stride[1], p.heads[1], [] {});
 }
 
 template <typename T, int V> int launch_typed(const RotaryArgs& a, cudaStream_t stream) {
