@@ -14,7 +14,9 @@
 namespace b200 {
 
 // cache_rows.cu: rows [0, n) of the table's pages, dense in the rows' dtype (scales null: a copy of 16-bit rows)
-int launch_cache_gather(const B200CacheRowsParams& p, cudaStream_t stream);
+// `beside`: the launch before it in the stream is none of its inputs' (it waits for it at its end, so that whoever waits for this one
+// waits for both)
+int launch_cache_gather(const B200CacheRowsParams& p, bool beside, cudaStream_t stream);
 
 namespace {
 
@@ -199,23 +201,29 @@ Problem own_problem(const B200CacheDecodeParams& a) {
   return p;
 }
 
-// The batch's rows against the prefix, dense rows at `k` and `v` ((Hkv, P, D)).
+// The batch's rows against the prefix: in the pools' pages (k null), or dense rows at `k` and `v` ((Hkv, P, D)).
 Problem prefix_problem(const B200CacheDecodeParams& a, const void* k, const void* v) {
   Problem p = own_problem(a);
-  p.k = k;
-  p.v = v;
   p.out = nullptr;
   p.lse = nullptr;
-  const int64_t kv[4] = {static_cast<int64_t>(a.Hkv) * a.prefix_len * a.D, static_cast<int64_t>(a.prefix_len) * a.D, a.D, 1};
-  for (int i = 0; i < 4; ++i) p.ks[i] = p.vs[i] = kv[i];
+  p.block_table = a.prefix_table;
+  if (k != nullptr) {
+    p.k = k;
+    p.v = v;
+    const int64_t kv[4] = {static_cast<int64_t>(a.Hkv) * a.prefix_len * a.D, static_cast<int64_t>(a.prefix_len) * a.D, a.D, 1};
+    for (int i = 0; i < 4; ++i) p.ks[i] = p.vs[i] = kv[i];
+  }
   p.qs[0] = static_cast<int64_t>(a.B) * a.q_stride[0];
   p.qs[2] = a.q_stride[0];
   p.L = a.B;
   p.B = 1;
   p.S = a.prefix_len;
   p.kv_lens = nullptr;
-  p.block_table = nullptr;
   return p;
+}
+// Tensor copies read a 16-bit prefix in its pages; an 8-bit one, or one of smaller pages, is first gathered into dense 16-bit rows.
+bool gathered(const B200CacheDecodeParams& a) {
+  return a.k_scales != nullptr || !prefix_paged(prefix_problem(a, nullptr, nullptr), a.n_pages);
 }
 
 // Keys of one CTA of the 16-bit kernel: enough CTAs for every slot of the GPU, ranges long enough to pay for a CTA's start and end.
@@ -245,7 +253,7 @@ int cache_decode_served(const B200CacheDecodeParams& a) {
       return B200_SDPA_ERR_UNSUPPORTED;
   if (static_cast<int64_t>(a.B) * a.Hq > 0x7fffffffLL) return B200_SDPA_ERR_UNSUPPORTED;
   if (a.prefix_len == 0) return a.k_scales != nullptr ? B200_SDPA_OK : B200_SDPA_ERR_UNSUPPORTED;
-  const Problem f = prefix_problem(a, reinterpret_cast<void*>(256), reinterpret_cast<void*>(256));
+  const Problem f = prefix_problem(a, nullptr, nullptr);
   if (f.group > 128) return B200_SDPA_ERR_UNSUPPORTED;
   return prefix_eligible(f, a.dtype) ? B200_SDPA_OK : B200_SDPA_ERR_ALIGNMENT;
 }
@@ -268,10 +276,10 @@ int geometry(const B200CacheDecodeParams& a, Geometry* g) {
     g->own_bytes = aligned(static_cast<uint64_t>(rows) * g->nsplit * (a.D + 2) * sizeof(float));
   }
   if (a.prefix_len > 0) {
-    const Problem f = prefix_problem(a, reinterpret_cast<void*>(256), reinterpret_cast<void*>(256));
+    const Problem f = prefix_problem(a, nullptr, nullptr);
     prefix_geometry(f, &g->pack);
     g->prefix_bytes = aligned(g->pack.ws_bytes);
-    g->dense_bytes = 2 * aligned(static_cast<uint64_t>(a.Hkv) * a.prefix_len * a.D * 2);
+    if (gathered(a)) g->dense_bytes = 2 * aligned(static_cast<uint64_t>(a.Hkv) * a.prefix_len * a.D * 2);
   }
   return B200_SDPA_OK;
 }
@@ -303,7 +311,7 @@ int plan_cache_decode(const B200CacheDecodeParams& a, B200SdpaPlan* plan) {
   plan->threads = fp8 ? 192 : 128;
   plan->smem_bytes = 0;
   plan->kv_splits = fp8 ? g.fp8.grid : g.nsplit;
-  plan->launches = 1 + (plan->kv_splits > 0 ? 1 : 0) + (a.prefix_len > 0 ? 2 : 0);
+  plan->launches = 1 + (plan->kv_splits > 0 ? 1 : 0) + (a.prefix_len > 0 ? (gathered(a) ? 2 : 1) : 0);
   plan->workspace_bytes = g.total();
   return B200_SDPA_OK;
 }
@@ -319,38 +327,7 @@ int launch_cache_decode(const B200CacheDecodeParams& a, cudaStream_t stream) {
   char* ws = static_cast<char*>(a.workspace);
   float* pre_o = reinterpret_cast<float*>(ws + g.own_bytes);
   float* pre_ml = pre_o + rows * g.pack.n_split * a.D;
-  if (a.prefix_len > 0) {
-    char* dense = ws + g.own_bytes + g.prefix_bytes;
-    B200CacheRowsParams r = {};
-    r.dtype = a.dtype;
-    r.page_size = a.page_size;
-    r.k = dense;
-    r.v = dense + g.dense_bytes / 2;
-    r.k_pages = const_cast<void*>(a.k_pages);
-    r.v_pages = const_cast<void*>(a.v_pages);
-    r.k_scales = const_cast<void*>(a.k_scales);
-    r.v_scales = const_cast<void*>(a.v_scales);
-    for (int i = 0; i < 3; ++i) {
-      r.k_pages_stride[i] = a.k_pages_stride[i];
-      r.v_pages_stride[i] = a.v_pages_stride[i];
-      r.k_scales_stride[i] = a.k_scales_stride[i];
-      r.v_scales_stride[i] = a.v_scales_stride[i];
-    }
-    r.k_stride[1] = r.v_stride[1] = static_cast<int64_t>(a.prefix_len) * a.D;
-    r.k_stride[2] = r.v_stride[2] = a.D;
-    r.B = 1;
-    r.Hkv = a.Hkv;
-    r.L = a.prefix_len;
-    r.D = a.D;
-    r.block_table = a.prefix_table;
-    r.block_table_stride = (a.prefix_len + a.page_size - 1) / a.page_size;
-    r.n_pages = a.n_pages;
-    r.status = a.status;
-    rc = launch_cache_gather(r, stream);
-    if (rc != B200_SDPA_OK) return rc;
-    rc = launch_prefix_partial(prefix_problem(a, r.k, r.v), a.dtype, g.pack, pre_o, pre_ml, stream);
-    if (rc != B200_SDPA_OK) return rc;
-  }
+  // Own keys first, then the gathering, which waits for nothing of theirs and fills the SMs beside them, then the prefix.
   Merge m = {};
   m.prefix = {pre_o, pre_ml};
   m.n_prefix = g.pack.n_split;
@@ -382,6 +359,41 @@ int launch_cache_decode(const B200CacheDecodeParams& a, cudaStream_t stream) {
     rc = launch_decode_partial_mma(p, a.dtype, g.chunk, g.nsplit, own_o, own_ml, stream);
   }
   if (rc != B200_SDPA_OK) return rc;
+  if (a.prefix_len > 0 && gathered(a)) {
+    char* dense = ws + g.own_bytes + g.prefix_bytes;
+    B200CacheRowsParams r = {};
+    r.dtype = a.dtype;
+    r.page_size = a.page_size;
+    r.k = dense;
+    r.v = dense + g.dense_bytes / 2;
+    r.k_pages = const_cast<void*>(a.k_pages);
+    r.v_pages = const_cast<void*>(a.v_pages);
+    r.k_scales = const_cast<void*>(a.k_scales);
+    r.v_scales = const_cast<void*>(a.v_scales);
+    for (int i = 0; i < 3; ++i) {
+      r.k_pages_stride[i] = a.k_pages_stride[i];
+      r.v_pages_stride[i] = a.v_pages_stride[i];
+      r.k_scales_stride[i] = a.k_scales_stride[i];
+      r.v_scales_stride[i] = a.v_scales_stride[i];
+    }
+    r.k_stride[1] = r.v_stride[1] = static_cast<int64_t>(a.prefix_len) * a.D;
+    r.k_stride[2] = r.v_stride[2] = a.D;
+    r.B = 1;
+    r.Hkv = a.Hkv;
+    r.L = a.prefix_len;
+    r.D = a.D;
+    r.block_table = a.prefix_table;
+    r.block_table_stride = (a.prefix_len + a.page_size - 1) / a.page_size;
+    r.n_pages = a.n_pages;
+    r.status = a.status;
+    rc = launch_cache_gather(r, g.own_bytes > 0, stream);
+    if (rc != B200_SDPA_OK) return rc;
+    rc = launch_prefix_partial(prefix_problem(a, r.k, r.v), a.dtype, g.pack, pre_o, pre_ml, stream, 0);
+    if (rc != B200_SDPA_OK) return rc;
+  } else if (a.prefix_len > 0) {
+    rc = launch_prefix_partial(prefix_problem(a, nullptr, nullptr), a.dtype, g.pack, pre_o, pre_ml, stream, a.n_pages);
+    if (rc != B200_SDPA_OK) return rc;
+  }
   return a.dtype == B200_SDPA_BF16 ? launch_combine<__nv_bfloat16>(p, m, stream) : launch_combine<__half>(p, m, stream);
 }
 

@@ -133,17 +133,16 @@ __global__ void __launch_bounds__(kThreads) cache_write_kernel(const B200CacheRo
 // elements).  Without lens every row is there.
 template <bool BF16, int LPR, bool QUANT>
 __global__ void __launch_bounds__(kThreads) cache_read_kernel(const B200CacheRowsParams p, const int page_shift, const int tokens,
-                                                               const int rows_16b) {
+                                                               const int rows_16b, const int beside) {
   constexpr int kRows = kThreads / LPR;
   const int b = blockIdx.y, i0 = blockIdx.x * tokens;
-  pdl_wait();
+  if (!beside) pdl_wait();
   pdl_launch_dependents();
   int n = p.lens != nullptr ? p.lens[b] : p.L;
   n = n < p.L ? n : p.L;
   const int n_tok = p.L - i0 < tokens ? p.L - i0 : tokens;
   const int lane = threadIdx.x % LPR, c0 = lane * 16;
-  if (c0 >= p.D) return;
-  const int total = n_tok * 2 * p.Hkv;
+  const int total = c0 < p.D ? n_tok * 2 * p.Hkv : 0;
   for (int r = threadIdx.x / LPR; r < total; r += kRows) {
     const int hk = r / n_tok, t = r - hk * n_tok;   // neighbouring tokens of a head: neighbouring rows of the result
     const bool is_v = hk >= p.Hkv;
@@ -186,6 +185,7 @@ __global__ void __launch_bounds__(kThreads) cache_read_kernel(const B200CacheRow
       for (int i = 0; i < 16; ++i) x[i] = static_cast<uint16_t>(out[i / 2] >> (16 * (i & 1)));
     }
   }
+  if (beside) pdl_wait();   // (complete no sooner than the launch before)
 }
 
 // Tokens of one CTA, `heads` rows each: enough for a few rounds of its threads, fewer where there would not be several CTAs for every SM.
@@ -213,23 +213,23 @@ bool rows_16b(const B200CacheRowsParams& p) {
 
 enum Direction { WRITE, READ, GATHER };
 
-template <Direction DIR, bool BF16, int LPR> int launch_rows(const B200CacheRowsParams& p, cudaStream_t stream) {
+template <Direction DIR, bool BF16, int LPR> int launch_rows(const B200CacheRowsParams& p, int beside, cudaStream_t stream) {
   const int tokens = tokens_per_cta(p, kThreads / LPR, DIR == WRITE ? p.Hkv : 2 * p.Hkv);
   const dim3 grid((p.L + tokens - 1) / tokens, p.B, DIR == WRITE ? 2 : 1);
   const int shift = page_shift_of(p.page_size);
   bool ok;
   if constexpr (DIR == WRITE) ok = launch_pdl(cache_write_kernel<BF16, LPR>, grid, kThreads, 0, stream, p, shift, tokens, rows_16b(p) ? 1 : 0);
-  else ok = launch_pdl(cache_read_kernel<BF16, LPR, DIR == READ>, grid, kThreads, 0, stream, p, shift, tokens, rows_16b(p) ? 1 : 0);
+  else ok = launch_pdl(cache_read_kernel<BF16, LPR, DIR == READ>, grid, kThreads, 0, stream, p, shift, tokens, rows_16b(p) ? 1 : 0, beside);
   if (!ok) return B200_SDPA_ERR_CUDA;
   count_launch(DIR == WRITE ? KID_CACHE_WRITE : KID_CACHE_READ);
   return B200_SDPA_OK;
 }
 
-template <Direction DIR, bool BF16> int launch_lanes(const B200CacheRowsParams& p, cudaStream_t stream) {
+template <Direction DIR, bool BF16> int launch_lanes(const B200CacheRowsParams& p, cudaStream_t stream, int beside = 0) {
   const int lanes = p.D / 16;
-  if (lanes <= 4) return launch_rows<DIR, BF16, 4>(p, stream);
-  if (lanes <= 8) return launch_rows<DIR, BF16, 8>(p, stream);
-  return launch_rows<DIR, BF16, 16>(p, stream);
+  if (lanes <= 4) return launch_rows<DIR, BF16, 4>(p, beside, stream);
+  if (lanes <= 8) return launch_rows<DIR, BF16, 8>(p, beside, stream);
+  return launch_rows<DIR, BF16, 16>(p, beside, stream);
 }
 
 }  // namespace
@@ -240,9 +240,9 @@ int launch_cache_write(const B200CacheRowsParams& p, cudaStream_t stream) {
 int launch_cache_read(const B200CacheRowsParams& p, cudaStream_t stream) {
   return p.dtype == B200_SDPA_BF16 ? launch_lanes<READ, true>(p, stream) : launch_lanes<READ, false>(p, stream);
 }
-int launch_cache_gather(const B200CacheRowsParams& p, cudaStream_t stream) {
-  if (p.k_scales != nullptr) return launch_cache_read(p, stream);
-  return launch_lanes<GATHER, true>(p, stream);   // (a copy: either 16-bit type)
+int launch_cache_gather(const B200CacheRowsParams& p, bool beside, cudaStream_t stream) {
+  if (p.k_scales == nullptr) return launch_lanes<GATHER, true>(p, stream, beside);   // (a copy: either 16-bit type)
+  return p.dtype == B200_SDPA_BF16 ? launch_lanes<READ, true>(p, stream, beside) : launch_lanes<READ, false>(p, stream, beside);
 }
 
 }  // namespace b200

@@ -174,7 +174,9 @@ struct PackGeom {
 };
 bool prefix_eligible(const Problem& p, int dtype);
 void prefix_geometry(const Problem& p, PackGeom* g);
-int launch_prefix_partial(const Problem& p, int dtype, const PackGeom& g, float* part_o, float* part_ml, cudaStream_t stream);
+bool prefix_paged(const Problem& p, int n_pages);
+// n_pages: k and v are pools of that many pages and block_table is the prefix's (prefix_paged() has agreed); 0: dense
+int launch_prefix_partial(const Problem& p, int dtype, const PackGeom& g, float* part_o, float* part_ml, cudaStream_t stream, int n_pages);
 
 int launch_bwd_generic(const BwdProblem& bp, int dtype, cudaStream_t stream);
 int plan_bwd_generic(const BwdProblem& bp, int dtype, B200SdpaPlan* plan);

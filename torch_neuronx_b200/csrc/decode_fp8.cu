@@ -399,6 +399,7 @@ __global__ void __launch_bounds__(kThreads, Geo<D, HEADS>::kCtas)
   }
   __syncthreads();
   pdl_wait();
+  pdl_launch_dependents();   // (a gathering of the shared prefix may run beside this)
   const List list = {p, p.Hkv * ((p.group + HEADS - 1) / HEADS)};
   Cursor c = first_place(list, fixed_blocks, lane);
 
@@ -649,7 +650,6 @@ __global__ void __launch_bounds__(kThreads, Geo<D, HEADS>::kCtas)
       }
     }
   }
-  pdl_launch_dependents();
   __syncthreads();   // (the warp that brings rows leaves last when the CTA gave up: the ring is its copies' until they have landed)
 }
 

@@ -118,14 +118,21 @@ struct PackArgs {
   int split_tiles;      // key tiles of one split
   float* part_o;        // [B][Hq][L][n_split][Dv]
   float* part_ml;       // [B][Hq][L][n_split][2]: maximum in log2 units, sum
+  // (PAGED) the keys' pages: key j is row j & (page - 1) of page table[j >> page_shift]
+  const int* table;
+  int page_shift, n_pages;
 };
 
+// PAGED (of the split form): the keys and values are rows of a paged cache, pages of 8 rows or more; a tile's rows come by one
+// tensor copy for each page and 64 columns, started by the lanes of the producer warp, which look a tile's pages up one item ahead.
+// Pages behind the last key are not read, and what lies behind it in its page is anything: those value rows become zeros.
+//
 // PAD: head dimensions E, Dv (multiples of 8) that do not fill the D = 128 tile.  The tensor maps carry the
 // real extents, so the copies fill the tile's remaining columns with zeros and the output store clips them;
 // the products run over ceil(E / 16) k-steps and ceil(Dv / 16) * 16 output columns only.  These shapes had fp32
 // probabilities on the CUDA-core kernel, so P goes into the second product as hi + lo (remainder2), lo in the second
 // half of the columns of S.
-template <int D, bool BF16, bool BIAS, bool ACC, bool PAD, bool PACK>
+template <int D, bool BF16, bool BIAS, bool ACC, bool PAD, bool PACK, bool PAGED = false>
 __global__ void __launch_bounds__(kThreads, 1)
 prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_o, const Problem p,
@@ -250,7 +257,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
       for (int bx = 0; bx < C::kBoxes; ++bx)
         tma_load_4d(q_smem[t] + bx * kBoxBytes, &tm_q, qbar, bx * 64, tg.row0, head_of_tile[t], b);
     }
-    for (; items_issued < n_ring && items_issued < C::kStages; ++items_issued) {
+    for (; !PAGED && items_issued < n_ring && items_issued < C::kStages; ++items_issued) {
       if (!item_exists(items_issued)) continue;
       const uint32_t bar = smem_u32(&sync->kv_full[items_issued]);
       mbar_arrive_expect_tx(bar, C::kTileBytes);
@@ -288,7 +295,52 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
 
   if (warp == kProducerWarp) {
     // ------------------------------------------------------------ TMA producer
-    if (lane == 0) {
+    if constexpr (PAGED) {
+      const int page = 1 << pack.page_shift, rows = page < kBlockN ? page : kBlockN;   // of one copy
+      auto entry_of = [&](int item) {   // lane i: the page of copy i of an item's tile, -1 behind the last key
+        const int key = (key_tile0 + item_tile(item)) * kBlockN + lane * rows;
+        return item < n_ring && lane * rows < kBlockN && key < kv_limit ? pack.table[key >> pack.page_shift] : -1;
+      };
+      bool alive = true;
+      int entry = entry_of(0);
+      for (int item = 0; item < n_ring && alive; ++item) {
+        const int next = entry_of(item + 1);
+        if (item_exists(item)) {
+          const int stage = item % C::kStages;
+          const uint32_t round = static_cast<uint32_t>(item / C::kStages);
+          if (round > 0) {
+            alive = wait_clocked(smem_u32(&sync->kv_empty[stage]), (round - 1) & 1u, abort_flag, wait_limit);
+            alive = __all_sync(0xffffffffu, alive);
+            if (!alive) {
+              if (lane == 0) report(p.status, 1, item, stage);
+              break;
+            }
+          }
+          const uint32_t bar = smem_u32(&sync->kv_full[stage]);
+          const int key = (key_tile0 + item_tile(item)) * kBlockN + lane * rows;
+          const bool mine = lane * rows < kBlockN && key < kv_limit;
+          if (mine && static_cast<unsigned>(entry) >= static_cast<unsigned>(pack.n_pages)) {   // reported, and page 0 read in its place
+            if (p.status != nullptr && atomicCAS(p.status, 0, B200_SDPA_ERR_PAGE) == 0) {
+              p.status[1] = -1;
+              p.status[2] = key;
+              p.status[3] = pack.n_pages;
+            }
+            entry = 0;
+          }
+          const unsigned copies = __popc(__ballot_sync(0xffffffffu, mine));
+          if (lane == 0) mbar_arrive_expect_tx(bar, copies * rows * 128 * C::kBoxes);
+          __syncwarp();
+          if (mine) {
+            const CUtensorMap* map = item_is_v(item) ? &tm_v : &tm_k;
+            for (int bx = 0; bx < C::kBoxes; ++bx)
+              tma_load_4d(kv_smem + stage * C::kTileBytes + bx * kBoxBytes + lane * rows * 128, map, bar, bx * 64, key & (page - 1), hk, entry);
+          }
+          __syncwarp();
+        }
+        items_issued = item + 1;
+        entry = next;
+      }
+    } else if (lane == 0) {
       bool alive = true;
       for (int item = items_issued; item < n_ring && alive; ++item) {
         if (!item_exists(item)) continue;
@@ -405,6 +457,9 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
           }
           alive = wait_full(4 * j + 2 + t);
           if (!alive) return;
+          if (PAGED && (key_tile0 + 2 * j + t + 1) * kBlockN > kv_limit)
+            zero_tile_rows<C::kBoxes, kBlockN>(kv_smem + stage_addr(4 * j + 2 + t) * C::kTileBytes,
+                                               kv_limit - (key_tile0 + 2 * j + t) * kBlockN, lane);
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             alive = wait_clocked(smem_u32(&sync->p_ready[t][half]), j & 1, abort_flag, wait_limit);
@@ -448,6 +503,8 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         // (these shapes came from a kernel that never reads a key beyond kv_lens)
         if (PAD && !has_next && kv_limit < p.S && (j + 1) * kBlockN > kv_limit)
           zero_tile_rows<C::kBoxes, kBlockN>(kv_smem + stage_addr(item_v) * C::kTileBytes, kv_limit - j * kBlockN, lane);
+        if (PAGED && (key_tile0 + j + 1) * kBlockN > kv_limit)
+          zero_tile_rows<C::kBoxes, kBlockN>(kv_smem + stage_addr(item_v) * C::kTileBytes, kv_limit - (key_tile0 + j) * kBlockN, lane);
         // one tile: P_t(j) V(j) in two halves as the halves of P arrive, then Q_t K(j+1)^T
         auto serve = [&](auto tile_const) {
           constexpr int t = decltype(tile_const)::value;
@@ -1057,19 +1114,24 @@ bool pack_geometry(const Problem& p, PackGeom* best) {
   return found;
 }
 
-template <int D, bool BF16>
-int launch_pack_partial(const Problem& p, const PackGeom& g, float* part_o, float* part_ml, cudaStream_t stream) {
+// pages: PAGED, the problem's k and v are pools of `n_pages` pages; 0: dense.
+template <int D, bool BF16, bool PAGED = false>
+int launch_pack_partial(const Problem& p, const PackGeom& g, float* part_o, float* part_ml, cudaStream_t stream, int n_pages = 0) {
   using C = Cfg<D>;
   CUtensorMap tq, tk, tv;
-  if (!make_map(&tq, p.q, BF16, D, p.L, p.Hq, p.B, p.qs, g.lb, p.group) || !make_map(&tk, p.k, BF16, D, p.S, p.Hkv, p.B, p.ks) ||
-      !make_map(&tv, p.v, BF16, D, p.S, p.Hkv, p.B, p.vs))
+  const int page = 1 << p.page_shift, rows = PAGED ? page : p.S, outer = PAGED ? n_pages : p.B, box = PAGED && page < kTileRows ? page : kTileRows;
+  if (!make_map(&tq, p.q, BF16, D, p.L, p.Hq, p.B, p.qs, g.lb, p.group) || !make_map(&tk, p.k, BF16, D, rows, p.Hkv, outer, p.ks, box) ||
+      !make_map(&tv, p.v, BF16, D, rows, p.Hkv, outer, p.vs, box))
     return B200_SDPA_ERR_CUDA;
-  auto kern = prefill_kernel<D, BF16, false, false, false, true>;
+  auto kern = prefill_kernel<D, BF16, false, false, false, true, PAGED>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes) != cudaSuccess) {
     cudaGetLastError();
     return B200_SDPA_ERR_CUDA;
   }
-  PackArgs a;
+  PackArgs a = {};
+  a.table = p.block_table;
+  a.page_shift = p.page_shift;
+  a.n_pages = n_pages;
   a.lb = g.lb;
   a.dual = g.dual;
   a.n_pairs = g.n_pairs;
@@ -1105,7 +1167,13 @@ bool prefix_eligible(const Problem& p, int dtype) {
   if (dtype != B200_SDPA_F16 && dtype != B200_SDPA_BF16) return false;
   if (!(p.scale > 0.f) || !(p.scale < 1e30f) || p.L < 1 || p.S < 1 || p.E != p.Dv || (p.E != 64 && p.E != 128) || p.group > kBlockM)
     return false;
-  return strides_ok(p.q, p.qs, p.L, p.Hq, p.B) && strides_ok(p.k, p.ks, p.S, p.Hkv, p.B) && strides_ok(p.v, p.vs, p.S, p.Hkv, p.B);
+  return strides_ok(p.q, p.qs, p.L, p.Hq, p.B);
+}
+
+// Whether tensor copies can read the prefix where it is, from the pages of 16-bit pools.
+bool prefix_paged(const Problem& p, int n_pages) {
+  const int page = 1 << p.page_shift;
+  return page >= 8 && strides_ok(p.k, p.ks, page, p.Hkv, n_pages) && strides_ok(p.v, p.vs, page, p.Hkv, n_pages);
 }
 
 void prefix_geometry(const Problem& p, PackGeom* best) {
@@ -1134,9 +1202,16 @@ void prefix_geometry(const Problem& p, PackGeom* best) {
   }
 }
 
-int launch_prefix_partial(const Problem& p, int dtype, const PackGeom& g, float* part_o, float* part_ml, cudaStream_t stream) {
+int launch_prefix_partial(const Problem& p, int dtype, const PackGeom& g, float* part_o, float* part_ml, cudaStream_t stream, int n_pages) {
   if (g.grid <= 0 || g.grid > 0x7fffffffLL) return B200_SDPA_ERR_UNSUPPORTED;
   const bool bf16 = dtype == B200_SDPA_BF16;
+  if (n_pages > 0) {
+    if (p.E == 128)
+      return bf16 ? launch_pack_partial<128, true, true>(p, g, part_o, part_ml, stream, n_pages)
+                  : launch_pack_partial<128, false, true>(p, g, part_o, part_ml, stream, n_pages);
+    return bf16 ? launch_pack_partial<64, true, true>(p, g, part_o, part_ml, stream, n_pages)
+                : launch_pack_partial<64, false, true>(p, g, part_o, part_ml, stream, n_pages);
+  }
   if (p.E == 128)
     return bf16 ? launch_pack_partial<128, true>(p, g, part_o, part_ml, stream) : launch_pack_partial<128, false>(p, g, part_o, part_ml, stream);
   return bf16 ? launch_pack_partial<64, true>(p, g, part_o, part_ml, stream) : launch_pack_partial<64, false>(p, g, part_o, part_ml, stream);
