@@ -208,7 +208,7 @@ __device__ __forceinline__ bool wait_read(const Problem& p, S* sync, int n, int 
   return ok;
 }
 
-// The warp that brings the rows.  Lane l looks up the pages of keys l, l + 32, ... of a block, kStages blocks ahead.  TMA: pages of 8
+// The warp that brings the rows.  Lane l looks up the pages of keys l, l + 32, ... of a block, a block ahead.  TMA: pages of 8
 // rows or more, one tensor copy for each page and operand.  Smaller pages: 16-byte copies of single rows.
 template <int D, int HEADS, bool TMA>
 __device__ __forceinline__ void bring_rows(const List& l, const CacheScales& sc, const CUtensorMap* tm_k, const CUtensorMap* tm_v,
@@ -217,28 +217,26 @@ __device__ __forceinline__ void bring_rows(const List& l, const CacheScales& sc,
   constexpr int kStages = G::kStages, kLook = kBlockKeys / 32;
   const Problem& p = l.p;
   const int page_mask = (1 << p.page_shift) - 1;
-  int entries[kStages][kLook];
-  Cursor ahead = c;
+  int entries[kLook], next[kLook];   // of this block and the next (a loop of one block: unrolled over the stages, the code came slower
+                                     // from behind the instruction caches than the table's latency is)
+  Cursor after = c;
   auto look_up = [&](int (&e)[kLook]) {
 #pragma unroll
-    for (int i = 0; i < kLook; ++i) e[i] = entry_of(p, ahead, ahead.blk * kBlockKeys + lane + 32 * i);
-    ahead.step(l);
+    for (int i = 0; i < kLook; ++i) e[i] = entry_of(p, after, after.blk * kBlockKeys + lane + 32 * i);
   };
-#pragma unroll
-  for (int s = 0; s < kStages; ++s) look_up(entries[s]);
+  look_up(entries);
   bool alive = true;
   int n = 0;
-  while (c.left > 0 && alive) {
-#pragma unroll
-    for (int s = 0; s < kStages; ++s) {
-      if (c.left <= 0 || !alive) break;
+#pragma unroll 1
+  while (c.left > 0) {
+      const int s = n % kStages;
+      after.step(l);
+      look_up(next);
       alive = wait_read(p, sync, n, 1, lane, wait_limit);
       if (!alive) break;
       const int hk = c.unit % p.Hkv;
       const uint32_t stage = ring + s * G::kStageBytes, bar = smem_u32(&sync->full[s]);
       const int key0 = c.blk * kBlockKeys;
-      Cursor after = c;
-      after.step(l);
       if (lane == 0) {
         const bool more = after.left > 0;
         Block& k = sync->block[s];
@@ -254,7 +252,7 @@ __device__ __forceinline__ void bring_rows(const List& l, const CacheScales& sc,
         int entry = 0;
 #pragma unroll
         for (int i = 0; i < kLook; ++i) {
-          const int e = __shfl_sync(0xffffffffu, entries[s][i], first & 31);
+          const int e = __shfl_sync(0xffffffffu, entries[i], first & 31);
           entry = (first >> 5) == i ? e : entry;
         }
         const int page = first < kBlockKeys ? page_of(p, sc, c, entry, key0 + first) : -1;
@@ -270,7 +268,7 @@ __device__ __forceinline__ void bring_rows(const List& l, const CacheScales& sc,
 #pragma unroll 4
           for (int x = lane; x < 32 * G::kChunksPerRow; x += 32) {
             const int row = 32 * i + x / G::kChunksPerRow, ch = x % G::kChunksPerRow;
-            const int64_t page = page_of(p, sc, c, __shfl_sync(0xffffffffu, entries[s][i], row & 31), key0 + row);
+            const int64_t page = page_of(p, sc, c, __shfl_sync(0xffffffffu, entries[i], row & 31), key0 + row);
             if (page < 0) continue;
             const int in_page = (key0 + row) & page_mask;
             const uint32_t dst = stage + row * D + ((ch ^ G::swizzle(row)) << 4);
@@ -283,8 +281,8 @@ __device__ __forceinline__ void bring_rows(const List& l, const CacheScales& sc,
       }
       ++n;
       c = after;
-      look_up(entries[s]);
-    }
+#pragma unroll
+      for (int i = 0; i < kLook; ++i) entries[i] = next[i];
   }
   if constexpr (!TMA) cp_async_wait_all();
   if (*static_cast<volatile int*>(&sync->abort_flag) != 0 && lane == 0) {
@@ -295,21 +293,21 @@ __device__ __forceinline__ void bring_rows(const List& l, const CacheScales& sc,
 
 // The warp that brings the scales of a block's keys l, l + 32, ... and of their values, and with the first block of a pair its query
 // rows.  All by asynchronous copies: a value that passes through a register would be waited for, and under load each takes as
-// long as a block.  (Scales are single bytes at any stride, so the four bytes around one are copied.)  Pages are looked up two blocks ahead.
+// long as a block.  (Scales are single bytes at any stride, so the four bytes around one are copied.)  Pages are looked up a block ahead.
 template <int D, int HEADS>
 __device__ __forceinline__ void bring_scales(const List& l, const CacheScales& sc, Sync<D, HEADS>* sync, Cursor c, int lane,
                                              long long wait_limit) {
-  constexpr int kStages = Geo<D, HEADS>::kStages, kLook = kBlockKeys / 32, kAhead = 2;
+  constexpr int kStages = Geo<D, HEADS>::kStages, kLook = kBlockKeys / 32;
   const Problem& p = l.p;
   const int page_mask = (1 << p.page_shift) - 1;
   const uint32_t k_page = static_cast<uint32_t>(sc.ks[0]), v_page = static_cast<uint32_t>(sc.vs[0]);
   const uint32_t k_row = static_cast<uint32_t>(sc.ks[2]), v_row = static_cast<uint32_t>(sc.vs[2]);
-  int entries[kAhead][kLook];
+  int e[kLook];
   Cursor ahead = c;
   const int blocks = c.left;
   int b = -1, unit = -1;   // whose queries were brought last
   const uint8_t *k_base = nullptr, *v_base = nullptr;
-  auto look_up = [&](int (&e)[kLook]) {
+  auto look_up = [&]() {
     const int* table = p.block_table + static_cast<int64_t>(ahead.b) * p.table_stride;
     const int key0 = ahead.blk * kBlockKeys + lane;
 #pragma unroll
@@ -319,16 +317,10 @@ __device__ __forceinline__ void bring_scales(const List& l, const CacheScales& s
     }
     ahead.step(l);
   };
-#pragma unroll
-  for (int d = 0; d < kAhead; ++d) look_up(entries[d]);
-  bool alive = true;
-  for (int n0 = 0; n0 < blocks && alive; n0 += kAhead) {
-#pragma unroll
-    for (int d = 0; d < kAhead; ++d) {
-      const int n = n0 + d;
-      if (n >= blocks || !alive) break;
-      alive = wait_read(p, sync, n, 3, lane, wait_limit);
-      if (!alive) break;
+  look_up();
+#pragma unroll 1
+  for (int n = 0; n < blocks; ++n) {
+      if (!wait_read(p, sync, n, 3, lane, wait_limit)) break;
       const int s = n % kStages;
       if (c.unit != unit || c.b != b) {
         b = c.b;
@@ -344,7 +336,6 @@ __device__ __forceinline__ void bring_scales(const List& l, const CacheScales& s
           for (int i = lane; i < heads * D; i += 32) sync->query[s][i / D][i % D] = q[i / D * p.qs[1] + i % D * p.qs[3]];
         }
       }
-      int(&e)[kLook] = entries[d];
       unsigned worst = 0;
 #pragma unroll
       for (int i = 0; i < kLook; ++i) worst = max(worst, static_cast<unsigned>(e[i]));
@@ -371,8 +362,7 @@ __device__ __forceinline__ void bring_scales(const List& l, const CacheScales& s
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&sync->full[s]));
       c.step(l);
-      look_up(e);
-    }
+      look_up();
   }
   cp_async_wait_all();   // (before the CTA lets go of its memory, should it give up)
 }
