@@ -107,8 +107,9 @@ int launch_decode(const Problem& p, int dtype, int kv_chunk, void* workspace, ui
 int plan_decode(const Problem& p, int dtype, int kv_chunk, B200SdpaPlan* plan);
 bool decode_eligible(const Problem& p, int dtype);
 bool decode_mma_eligible(const Problem& p, int dtype);
+// beside: (paged, no append) the launch before it in the stream is none of its inputs'
 int launch_decode_partial_mma(const Problem& p, int dtype, int chunk, int nsplit, float* part_o, float* part_ml,
-                              cudaStream_t stream);
+                              cudaStream_t stream, bool beside = false);
 int launch_decode_static(const Problem& p, int dtype, int kv_chunk, cudaStream_t stream);
 
 // `workspace` (optional, >= 4 bytes): the counter from which the persistent CTAs draw their work items

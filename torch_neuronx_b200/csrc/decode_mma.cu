@@ -147,7 +147,9 @@ __device__ __forceinline__ void rotate8(const Problem& p, int b, int ch, uint16_
   for (int e = 0; e < 8; ++e) x[e] = rot[e];
 }
 
-template <int D, bool BF16, bool PAGED, bool APPEND, bool ROPE>
+// BESIDE: none of the inputs come from the launch before it in the stream, which lets this one in early: it runs beside that one
+// and waits for it at its end, so that whoever waits for this grid waits for both.
+template <int D, bool BF16, bool PAGED, bool APPEND, bool ROPE, bool BESIDE = false>
 __global__ void __launch_bounds__(kThreads, 3) decode_mma_kernel(const Problem p, const int chunk, const int nsplit,
                                                                  float* __restrict__ part_o,
                                                                  float* __restrict__ part_ml) {
@@ -162,7 +164,7 @@ __global__ void __launch_bounds__(kThreads, 3) decode_mma_kernel(const Problem p
   const int hk = blockIdx.x % p.Hkv;
   const int gsub = blockIdx.x / p.Hkv;
   const int b = blockIdx.y;
-  pdl_wait();
+  if (!BESIDE) pdl_wait();
   const int n_keys = valid_keys(p, b);
   const int s0 = split * chunk;
   if (s0 >= n_keys && split != 0) return;  // split 0 still writes an (empty) partial
@@ -461,13 +463,14 @@ __global__ void __launch_bounds__(kThreads, 3) decode_mma_kernel(const Problem p
       part_ml[slot * 2 + 1] = lsum;
     }
   }
+  if (BESIDE) pdl_wait();
 }
 
-template <int D, bool BF16, bool PAGED, bool APPEND, bool ROPE>
+template <int D, bool BF16, bool PAGED, bool APPEND, bool ROPE, bool BESIDE = false>
 int launch_one(const Problem& p, int chunk, int nsplit, float* po, float* pml, cudaStream_t stream) {
   using G = Geo<D>;
   static_assert(kWarps * 16 * D * 4 + kWarps * 16 * 2 * 4 <= G::kSmemBytes, "merge buffer must fit in the ring");
-  auto kern = decode_mma_kernel<D, BF16, PAGED, APPEND, ROPE>;
+  auto kern = decode_mma_kernel<D, BF16, PAGED, APPEND, ROPE, BESIDE>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, G::kSmemBytes) != cudaSuccess) {
     cudaGetLastError();
     return B200_SDPA_ERR_CUDA;
@@ -489,10 +492,17 @@ bool decode_mma_eligible(const Problem& p, int dtype) {
 }
 
 int launch_decode_partial_mma(const Problem& p, int dtype, int chunk, int nsplit, float* po, float* pml,
-                              cudaStream_t stream) {
+                              cudaStream_t stream, bool beside) {
   const bool bf16 = dtype == B200_SDPA_BF16;
   const bool d128 = p.E == 128, paged = p.block_table != nullptr, append = p.k_new != nullptr;
   const bool rope = p.rope_cos != nullptr;
+  if (beside) {
+    if (!paged || append || rope) return B200_SDPA_ERR_UNSUPPORTED;
+    if (d128) return bf16 ? launch_one<128, true, true, false, false, true>(p, chunk, nsplit, po, pml, stream)
+                          : launch_one<128, false, true, false, false, true>(p, chunk, nsplit, po, pml, stream);
+    return bf16 ? launch_one<64, true, true, false, false, true>(p, chunk, nsplit, po, pml, stream)
+                : launch_one<64, false, true, false, false, true>(p, chunk, nsplit, po, pml, stream);
+  }
   if (rope) {
 #define B200_DECODE_ROPE_CASE(DD, BB, PP)                                                              \
   if (d128 == (DD == 128) && bf16 == BB && paged == PP) return launch_one<DD, BB, PP, true, true>(p, chunk, nsplit, po, pml, stream);
