@@ -156,6 +156,31 @@ def test_a_serving_step(dtype):
         U.check(got[:, :, i:i + 1].cpu(), want[1].float(), want, p_bits=dtype)
 
 
+@pytest.mark.parametrize("quantised,page", [(False, 16), (False, 4), (True, 16)])
+def test_a_bad_page_is_reported(quantised, page):
+    """A number outside the pool, in the prefix or a sequence's own table, is looked over before it is used: page 0 stands in."""
+    import torch_neuronx_b200 as T
+
+    q, k, v, ks, vs, prefix, table, lens = _setup(5, torch.bfloat16, quantised, 3, 4, 2, 64, page, 5 * page, 3, "NHD")
+    lens[0] = 3 * page
+    want = U.attend(q, k, v, ks, vs, table, lens, "NHD", prefix=prefix, P=5 * page)
+    dev = _cuda(q, k, v, ks, vs)
+    n = k.shape[0]
+    for which, number in (("prefix", n), ("prefix", -1), ("own", n + 7), ("own", -2147483648)):
+        p2, t2 = prefix.clone(), table.clone()
+        if which == "prefix":
+            p2[2] = number
+        else:
+            t2[0, 1] = number
+        out, _ = T.shared_prefix_decode(*dev[:3], p2.cuda(), 5 * page, t2.cuda(), lens.cuda(), k_scales=dev[3], v_scales=dev[4])
+        with pytest.raises(RuntimeError, match="page"):
+            T.check_device_status()
+        assert torch.isfinite(out).all()
+    out, lse = T.shared_prefix_decode(*dev[:3], prefix.cuda(), 5 * page, table.cuda(), lens.cuda(), need_lse=True, k_scales=dev[3], v_scales=dev[4])
+    T.check_device_status()
+    U.check(out.cpu(), lse.cpu(), want, p_bits=torch.bfloat16)
+
+
 def test_refusals():
     import torch_neuronx_b200 as T
 

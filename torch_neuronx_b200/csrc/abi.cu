@@ -57,6 +57,7 @@ int validate(const B200SdpaParams* a, Problem* p) {
   p->block_table = a->block_table;
   p->table_stride = a->block_table_stride;
   p->page_shift = 0;
+  p->n_pages = 0;
   p->k_new = a->k_new;
   p->v_new = a->v_new;
   p->lens_out = a->kv_lens_out;
@@ -274,6 +275,7 @@ int validate_bwd(const B200SdpaBwdParams* a, BwdProblem& bp) {
   p.block_table = nullptr;
   p.table_stride = 0;
   p.page_shift = 0;
+  p.n_pages = 0;
   p.k_new = nullptr;
   p.v_new = nullptr;
   p.lens_out = nullptr;

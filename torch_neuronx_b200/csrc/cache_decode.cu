@@ -197,6 +197,7 @@ Problem own_problem(const B200CacheDecodeParams& a) {
   p.status = a.status;
   p.block_table = a.block_table;
   p.table_stride = a.block_table_stride;
+  p.n_pages = a.n_pages;
   while ((1 << p.page_shift) < a.page_size) ++p.page_shift;
   return p;
 }

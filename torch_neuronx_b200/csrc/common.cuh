@@ -38,6 +38,7 @@ struct Problem {
   const int* block_table;
   int table_stride;
   int page_shift;
+  int n_pages;           // of the pools, where a kernel looks page numbers over (decode beside a shared prefix)
   // Decode with append: the key/value row of the token being decoded arrives separately
   // ((B, Hkv, D), unit inner stride); it is attended to as key kv_lens[b] and written into the
   // cache at that position by the CTA that reads it.  lens_out (if set, not aliasing kv_lens)

@@ -26,6 +26,7 @@
 // rescaled; P rounded to the cache dtype once (torch_neuronx/_sdpa_math.py:94).
 #include "common.cuh"
 #include "debug.cuh"
+#include "report.cuh"
 
 namespace b200 {
 
@@ -233,7 +234,11 @@ __global__ void __launch_bounds__(kThreads, 3) decode_mma_kernel(const Problem p
       const int srow = ok ? key0 + row : s0;
       int64_t k_off, v_off;
       if (PAGED) {
-        const int64_t page = pages[i];
+        int64_t page = pages[i];
+        if (BESIDE && static_cast<unsigned>(pages[i]) >= static_cast<unsigned>(p.n_pages)) {   // reported, and page 0 read in its place
+          report_page(p.status, B200_SDPA_ERR_PAGE, b, srow, p.n_pages);
+          page = 0;
+        }
         const int in_page = srow & page_mask;
         k_off = (page * p.ks[0]) * 2 + in_page * k_row;
         v_off = (page * p.vs[0]) * 2 + in_page * v_row;

@@ -2,6 +2,7 @@
 #pragma once
 
 #include "common.cuh"
+#include "report.cuh"
 
 namespace b200 {
 
@@ -68,15 +69,6 @@ __device__ __forceinline__ uint4 ld_stream_16B(const void* ptr) {
                : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
                : "l"(ptr));
   return r;
-}
-
-// A position whose page is not there: said once, nothing is accessed.
-__device__ __forceinline__ void report_page(int* status, int error, int b, int pos, int n_pages) {
-  if (status != nullptr && atomicCAS(status, 0, error) == 0) {
-    status[1] = b;
-    status[2] = pos;
-    status[3] = n_pages;
-  }
 }
 
 }  // namespace b200

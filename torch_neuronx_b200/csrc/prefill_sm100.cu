@@ -31,6 +31,7 @@
 // B200_SDPA_ERR_TIMEOUT.
 #include "tc_common.cuh"
 #include "debug.cuh"
+#include "report.cuh"
 
 #include <type_traits>
 
@@ -320,11 +321,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
           const int key = (key_tile0 + item_tile(item)) * kBlockN + lane * rows;
           const bool mine = lane * rows < kBlockN && key < kv_limit;
           if (mine && static_cast<unsigned>(entry) >= static_cast<unsigned>(pack.n_pages)) {   // reported, and page 0 read in its place
-            if (p.status != nullptr && atomicCAS(p.status, 0, B200_SDPA_ERR_PAGE) == 0) {
-              p.status[1] = -1;
-              p.status[2] = key;
-              p.status[3] = pack.n_pages;
-            }
+            report_page(p.status, B200_SDPA_ERR_PAGE, -1, key, pack.n_pages);
             entry = 0;
           }
           const unsigned copies = __popc(__ballot_sync(0xffffffffu, mine));
