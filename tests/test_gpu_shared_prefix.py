@@ -22,6 +22,9 @@ CASES = [
     (torch.bfloat16, True, 7, 5, 1, 128, 16, 0, 3, "NHD"),
     (torch.float16, False, 4, 8, 2, 128, 16, 77, 0, "NHD"),         # nothing but the prefix
     (torch.float16, True, 300, 3, 3, 64, 4, 50, 2, "HND"),
+    (torch.bfloat16, True, 64, 16, 8, 64, 4, 900, 2, "NHD"),        # small pages, gathered
+    (torch.float16, True, 1, 40, 2, 128, 16, 3000, 0, "HND"),       # one sequence with nothing of its own, twenty query heads
+    (torch.bfloat16, True, 6, 8, 2, 128, 2, 333, 40, "NHD"),        # small pages, the prefix before each sequence's keys
 ]
 
 

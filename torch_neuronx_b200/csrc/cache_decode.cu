@@ -35,6 +35,7 @@ struct Merge {
   int n_own, chunk;    // 16-bit cache: ranges of `chunk` keys, rows (sequence * Hq + head) * n_own + range
   const int2* range;   // 8-bit cache (decode_fp8.cu)
   int heads, units;
+  int front;           // the prefix's partials are among these too, each sequence's before its own
 };
 
 // WARPS warps for each (sequence, query head), 4 / WARPS rows in a CTA: the prefix's partials (rows (h * B + b) * n ..) and the own
@@ -51,28 +52,32 @@ __global__ void __launch_bounds__(kCombineWarps * 32) cache_combine_kernel(const
   pdl_launch_dependents();
   if (id >= static_cast<int64_t>(p.B) * p.Hq) return;   // (whole warps; with four to a row the grid is exact)
   const int h = static_cast<int>(id % p.Hq), b = static_cast<int>(id / p.Hq);
-  // own partials: row own0 + s * step
-  int used = 0, step = 1;
-  int64_t own0 = 0;
+  // own partials: rows own0 + s * step; the prefix's: rows pre0 + s * pre_step
+  int used = 0, step = 1, n_prefix = a.n_prefix, pre_step = 1;
+  int64_t own0 = 0, pre0 = (static_cast<int64_t>(h) * p.B + b) * a.n_prefix;
   if (a.range != nullptr) {
-    const int in_group = h % p.group;
-    const int64_t pair = static_cast<int64_t>(b) * a.units + in_group / a.heads * p.Hkv + h / p.group;
+    const int in_group = h % p.group, unit = in_group / a.heads * p.Hkv + h / p.group, twice = a.front != 0 ? 1 : 0;
+    step = a.heads;
     if (valid_keys(p, b) > 0) {
-      const int2 r = a.range[pair];
+      const int2 r = a.range[((static_cast<int64_t>(b) << twice) + twice) * a.units + unit];
       used = (r.y - r.x + 1) * kFp8Parts;
-      step = a.heads;
       own0 = static_cast<int64_t>(r.x) * kFp8Parts * a.heads + in_group % a.heads;
+    }
+    if (twice) {
+      const int2 r = a.range[(static_cast<int64_t>(b) << 1) * a.units + unit];
+      n_prefix = (r.y - r.x + 1) * kFp8Parts;
+      pre_step = a.heads;
+      pre0 = static_cast<int64_t>(r.x) * kFp8Parts * a.heads + in_group % a.heads;
     }
   } else if (a.n_own > 0) {
     used = (valid_keys(p, b) + a.chunk - 1) / a.chunk;
     used = used < 1 ? 1 : (used > a.n_own ? a.n_own : used);
     own0 = (static_cast<int64_t>(b) * p.Hq + h) * a.n_own;
   }
-  const int64_t pre0 = (static_cast<int64_t>(h) * p.B + b) * a.n_prefix;
   if (!dbg_bhrc(p.status, DBG_CACHE_DECODE * 100 + 1, b, p.B, h, p.Hq, 0, 1, lane * C, C, p.Dv)) return;
-  auto row_of = [&](int s) { return s < a.n_prefix ? pre0 + s : own0 + static_cast<int64_t>(s - a.n_prefix) * step; };
-  const int total = a.n_prefix + used;
-  auto pair_of = [&](int s) { return *reinterpret_cast<const float2*>((s < a.n_prefix ? a.prefix.ml : a.own.ml) + row_of(s) * 2); };
+  auto row_of = [&](int s) { return s < n_prefix ? pre0 + static_cast<int64_t>(s) * pre_step : own0 + static_cast<int64_t>(s - n_prefix) * step; };
+  const int total = n_prefix + used;
+  auto pair_of = [&](int s) { return *reinterpret_cast<const float2*>((s < n_prefix ? a.prefix.ml : a.own.ml) + row_of(s) * 2); };
   auto together = [&]() {
     if constexpr (WARPS > 1) __syncthreads();
     else __syncwarp();
@@ -116,7 +121,7 @@ __global__ void __launch_bounds__(kCombineWarps * 32) cache_combine_kernel(const
 #pragma unroll
         for (int c = 0; c < C; ++c) v[i][c] = 0.f;
         if (w[i] != 0.f) {
-          const float* src = (s0 + s < a.n_prefix ? a.prefix.o : a.own.o) + row_of(s0 + s) * D + lane * C;
+          const float* src = (s0 + s < n_prefix ? a.prefix.o : a.own.o) + row_of(s0 + s) * D + lane * C;
           if constexpr (C == 4) *reinterpret_cast<float4*>(v[i]) = *reinterpret_cast<const float4*>(src);
           else *reinterpret_cast<float2*>(v[i]) = *reinterpret_cast<const float2*>(src);
         }
@@ -163,6 +168,7 @@ __global__ void __launch_bounds__(kCombineWarps * 32) cache_combine_kernel(const
 struct Geometry {
   int chunk, nsplit;          // own keys of a 16-bit cache; nsplit = 0: no table, or an 8-bit cache
   Fp8Geometry fp8;            // own keys of an 8-bit cache
+  bool front;                 // ... and the prefix's with them, once for each sequence
   PackGeom pack;              // prefix
   uint64_t own_bytes, prefix_bytes, dense_bytes;
   uint64_t total() const { return own_bytes + prefix_bytes + dense_bytes; }
@@ -249,6 +255,28 @@ int default_chunk(const Problem& p) {
 
 }  // namespace
 
+namespace {
+
+// Whether an 8-bit prefix is read for each sequence, before its own keys, instead of once for all.  Once for all costs two more launches
+// (gathered rows, then tiles of 128 query rows whether there are as many or not); for each costs B times the keys, from L2 all but
+// once.  Both in us, fitted to 1 to 128 sequences under 300 to 11008 keys (each against once, with up to 100 own keys): 1 sequence,
+// 8192 keys, 8 kv heads of 128: 16.4 against 27.7; 5, 3708, 4: 15.8 against 20.5; 8, 4096, 8: 26.7 against 25.9; 16, 2048, 8: 26.9
+// against 23.0; 128, 2048, 8: 105 against 38; 64, 4096, 2 heads of 64: 28.1 against 20.6.
+bool in_front(const B200CacheDecodeParams& a) {
+  const Problem f = prefix_problem(a, nullptr, nullptr);
+  const int heads = f.group <= 8 ? 8 : 16;
+  const double blocks = static_cast<double>(a.B) * a.Hkv * ((f.group + heads - 1) / heads) * ((a.prefix_len + 127) / 128);
+  const double each = blocks / 148 * (a.D == 128 ? 1.0 : 0.6);
+  PackGeom g;
+  prefix_geometry(f, &g);
+  const double steps = g.dual ? (g.split_tiles + 1) / 2 : g.split_tiles;
+  const double rounds = static_cast<double>((g.grid + 147) / 148);
+  const double once = 6.5 + 6.0 * a.prefix_len * a.Hkv * a.D / 8.0e6 + rounds * steps * 1.9;
+  return each < once;
+}
+
+}  // namespace
+
 int cache_decode_served(const B200CacheDecodeParams& a) {
   for (int i = 0; i < 3 && a.k_scales != nullptr; ++i)   // (the kernels multiply page and row by 32 bits)
     if (a.k_scales_stride[i] < 0 || a.k_scales_stride[i] > 0x7fffffffLL || a.v_scales_stride[i] < 0 || a.v_scales_stride[i] > 0x7fffffffLL)
@@ -268,8 +296,9 @@ int geometry(const B200CacheDecodeParams& a, Geometry* g) {
   const Problem p = own_problem(a);
   *g = {};
   const int64_t rows = static_cast<int64_t>(a.B) * a.Hq;
-  if (p.S > 0 && a.k_scales != nullptr) {
-    if (!decode_fp8_geometry(p, a.kv_chunk, &g->fp8)) return B200_SDPA_ERR_UNSUPPORTED;
+  g->front = a.k_scales != nullptr && a.prefix_len > 0 && in_front(a);
+  if (a.k_scales != nullptr && (p.S > 0 || g->front)) {
+    if (!decode_fp8_served(p, a.n_pages) || !decode_fp8_geometry(p, g->front ? a.prefix_len : 0, a.kv_chunk, &g->fp8)) return B200_SDPA_ERR_UNSUPPORTED;
     g->own_bytes = aligned(g->fp8.bytes);
   } else if (p.S > 0) {
     g->chunk = a.kv_chunk > 0 ? (a.kv_chunk + 31) / 32 * 32 : default_chunk(p);
@@ -277,7 +306,7 @@ int geometry(const B200CacheDecodeParams& a, Geometry* g) {
     if (g->nsplit > 65535 || static_cast<int64_t>(p.Hkv) * ((p.group + 15) / 16) > 65535) return B200_SDPA_ERR_UNSUPPORTED;
     g->own_bytes = aligned(static_cast<uint64_t>(rows) * g->nsplit * (a.D + 2) * sizeof(float));
   }
-  if (a.prefix_len > 0) {
+  if (a.prefix_len > 0 && !g->front) {
     const Problem f = prefix_problem(a, nullptr, nullptr);
     prefix_geometry(f, &g->pack);
     g->prefix_bytes = aligned(g->pack.ws_bytes);
@@ -313,7 +342,7 @@ int plan_cache_decode(const B200CacheDecodeParams& a, B200SdpaPlan* plan) {
   plan->threads = fp8 ? 192 : 128;
   plan->smem_bytes = 0;
   plan->kv_splits = fp8 ? g.fp8.grid : g.nsplit;
-  plan->launches = 1 + (plan->kv_splits > 0 ? 1 : 0) + (a.prefix_len > 0 ? (gathered(a) ? 2 : 1) : 0);
+  plan->launches = 1 + (plan->kv_splits > 0 ? 1 : 0) + (a.prefix_len > 0 && !g.front ? (gathered(a) ? 2 : 1) : 0);
   plan->workspace_bytes = g.total();
   return B200_SDPA_OK;
 }
@@ -331,7 +360,7 @@ int launch_cache_decode(const B200CacheDecodeParams& a, cudaStream_t stream) {
   float* pre_ml = pre_o + rows * g.pack.n_split * a.D;
   Merge m = {};
   m.prefix = {pre_o, pre_ml};
-  m.n_prefix = g.pack.n_split;
+  m.n_prefix = g.front ? 0 : g.pack.n_split;
   // 8-bit: the own keys first; the gathering, which needs nothing of theirs, runs beside them.  16-bit: the prefix first; the
   // own keys run beside it, on the SMs that it leaves or has done with.  (64 sequences under 16384 keys: 70 us one behind the other.)
   if (g.fp8.grid > 0) {
@@ -352,10 +381,17 @@ int launch_cache_decode(const B200CacheDecodeParams& a, cudaStream_t stream) {
     m.range = part.range;
     m.heads = g.fp8.heads;
     m.units = g.fp8.units;
-    rc = launch_decode_partial_fp8(p, sc, a.dtype, g.fp8, part, stream);
+    if (g.front) {
+      m.front = 1;
+      m.prefix = m.own;
+    }
+    const FrontKeys front = {a.prefix_table, g.front ? a.prefix_len : 0};
+    rc = launch_decode_partial_fp8(p, sc, a.dtype, g.fp8, front, part, stream);
     if (rc != B200_SDPA_OK) return rc;
   }
-  if (a.prefix_len > 0 && gathered(a)) {
+  if (g.front) {
+    // nothing more: the prefix is among the own keys' partials
+  } else if (a.prefix_len > 0 && gathered(a)) {
     char* dense = ws + g.own_bytes + g.prefix_bytes;
     B200CacheRowsParams r = {};
     r.dtype = a.dtype;

@@ -146,8 +146,8 @@ struct CacheScales {
   int64_t ks[3], vs[3];   // page, head, row in page
   int n_pages;
 };
-// Partials of the own keys of an 8-bit cache (decode_fp8.cu): slots of kFp8Parts x `heads` rows; a pair (sequence, unit) has the slots
-// range[pair].x to range[pair].y, all written, unless its sequence is empty.
+// Partials of the own keys of an 8-bit cache (decode_fp8.cu): slots of kFp8Parts x `heads` rows; a pair (sequence -- or with a front
+// its two parts, one after the other --, unit) has the slots range[pair].x to range[pair].y, all written, unless its sequence is empty.
 constexpr int kFp8Parts = 4;
 struct OwnPartials {
   float* o;      // [slot][part][heads][D]
@@ -160,9 +160,15 @@ struct Fp8Geometry {
   int64_t slots;
   uint64_t bytes;
 };
-bool decode_fp8_geometry(const Problem& p, int kv_chunk, Fp8Geometry* g);
-int launch_decode_partial_fp8(const Problem& p, const CacheScales& sc, int dtype, const Fp8Geometry& g, const OwnPartials& part,
-                              cudaStream_t stream);
+// Keys of a prefix that every sequence shares, read for each of them before its own; len 0: none.
+struct FrontKeys {
+  const int* table;
+  int len;
+};
+bool decode_fp8_served(const Problem& p, int n_pages);
+bool decode_fp8_geometry(const Problem& p, int front_keys, int kv_chunk, Fp8Geometry* g);
+int launch_decode_partial_fp8(const Problem& p, const CacheScales& sc, int dtype, const Fp8Geometry& g, const FrontKeys& front,
+                              const OwnPartials& part, cudaStream_t stream);
 int cache_decode_served(const B200CacheDecodeParams& a);   // a status
 int plan_cache_decode(const B200CacheDecodeParams& a, B200SdpaPlan* plan);
 int launch_cache_decode(const B200CacheDecodeParams& a, cudaStream_t stream);

@@ -5,6 +5,8 @@
 // batches leave no SM without work and no CTA starts twice.  A CTA leaves fp32 partials (o, m, l), one of each computing warp, for
 // each (sequence, kv head) that its range touches, in slot `CTA + number of the pair` (both only ever grow along the list, so no slot is used twice),
 // and whoever has a pair's first or last block notes the slot; a second launch merges (cache_decode.cu).
+// With a prefix that all sequences share (FrontKeys) and that is not worth launches of its own, every sequence is two in the list:
+// the prefix's keys, then its own.
 // What the format changes:
 //   * e4m3 is exact in fp16, so both products are fp16 m16n8k16 MMAs with the bytes expanded in registers (8-bit MMAs would
 //     need P and Q in 8 bits).  Both are taken transposed, S^T = K Q^T and O^T = V^T P^T: the keys, then the columns of V,
@@ -119,18 +121,24 @@ __device__ __forceinline__ uint32_t turn8x8(uint32_t x) {
 // The list of blocks: for each sequence and unit (a kv head and a block of its query heads) the blocks of its keys.
 struct List {
   const Problem& p;
-  const int units;
-  __device__ __forceinline__ int blocks(int b) const { return (valid_keys(p, b) + kBlockKeys - 1) / kBlockKeys; }
+  const FrontKeys& front;
+  const int units, twice;   // twice: 1 with a front, sequence b is entries 2 b (the front) and 2 b + 1
+  __device__ __forceinline__ int count() const { return p.B << twice; }
+  __device__ __forceinline__ int keys(int e) const { return twice && (e & 1) == 0 ? front.len : valid_keys(p, e >> twice); }
+  __device__ __forceinline__ int blocks(int e) const { return (keys(e) + kBlockKeys - 1) / kBlockKeys; }
+  __device__ __forceinline__ const int* table(int e) const {
+    return twice && (e & 1) == 0 ? front.table : p.block_table + static_cast<int64_t>(e >> twice) * p.table_stride;
+  }
 };
 
 // A place in the list and the number of blocks behind it that the CTA still has to do; every role walks on its own.
 struct Cursor {
-  int b, unit, blk;     // sequence, unit, block of the sequence
-  int n_keys, n_blk;    // of the sequence
+  int b, unit, blk;     // entry (a sequence, or one of its two parts), unit, block of the entry
+  int n_keys, n_blk;    // of the entry
   int left;
 
   __device__ __forceinline__ void enter(const List& l) {
-    n_keys = valid_keys(l.p, b);
+    n_keys = l.keys(b);
     n_blk = (n_keys + kBlockKeys - 1) / kBlockKeys;
   }
   // The next block; `left` reaches 0 at the end of the range.
@@ -147,14 +155,14 @@ struct Cursor {
     do {
       ++b;
       enter(l);
-    } while (n_blk == 0 && b + 1 < l.p.B);
+    } while (n_blk == 0 && b + 1 < l.count());
   }
 };
 
 // The first place of this CTA's range.  Whole warp; lens are read 32 at a time, twice.
 __device__ __forceinline__ Cursor first_place(const List& l, int fixed_blocks, int lane) {
   int64_t sum = 0;
-  for (int b0 = 0; b0 < l.p.B; b0 += 32) sum += __reduce_add_sync(0xffffffffu, b0 + lane < l.p.B ? l.blocks(b0 + lane) : 0);
+  for (int b0 = 0; b0 < l.count(); b0 += 32) sum += __reduce_add_sync(0xffffffffu, b0 + lane < l.count() ? l.blocks(b0 + lane) : 0);
   const int64_t total = sum * l.units;
   int64_t per = fixed_blocks;
   if (per == 0) per = (total + gridDim.x - 1) / gridDim.x;
@@ -163,8 +171,8 @@ __device__ __forceinline__ Cursor first_place(const List& l, int fixed_blocks, i
   if (start >= total) return c;
   c.left = static_cast<int>(total - start < per ? total - start : per);
   int64_t before = 0;
-  for (int b0 = 0; b0 < l.p.B; b0 += 32) {
-    const int mine = b0 + lane < l.p.B ? l.blocks(b0 + lane) : 0;
+  for (int b0 = 0; b0 < l.count(); b0 += 32) {
+    const int mine = b0 + lane < l.count() ? l.blocks(b0 + lane) : 0;
     int upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o *= 2) {
@@ -187,9 +195,9 @@ __device__ __forceinline__ Cursor first_place(const List& l, int fixed_blocks, i
 }
 
 // Table entry of a key position; -1 behind the end.  Looked at where it is used: a look here would wait for the load.
-__device__ __forceinline__ int entry_of(const Problem& p, const Cursor& c, int row) {
+__device__ __forceinline__ int entry_of(const List& l, const Cursor& c, int row) {
   int page = -1;
-  if (c.left > 0 && row < c.n_keys) page = p.block_table[static_cast<int64_t>(c.b) * p.table_stride + (row >> p.page_shift)];
+  if (c.left > 0 && row < c.n_keys) page = l.table(c.b)[row >> l.p.page_shift];
   return page;
 }
 // A number outside the pool is reported, and page 0 read in its place.
@@ -224,7 +232,7 @@ __device__ __forceinline__ void bring_rows(const List& l, const CacheScales& sc,
   Cursor after = c;
   auto look_up = [&](int (&e)[kLook]) {
 #pragma unroll
-    for (int i = 0; i < kLook; ++i) e[i] = entry_of(p, after, after.blk * kBlockKeys + lane + 32 * i);
+    for (int i = 0; i < kLook; ++i) e[i] = entry_of(l, after, after.blk * kBlockKeys + lane + 32 * i);
   };
   look_up(entries);
   bool alive = true;
@@ -265,18 +273,28 @@ __device__ __forceinline__ void bring_rows(const List& l, const CacheScales& sc,
         if (mine)
           tma_load_4d(stage + (lane & 1) * G::kTileBytes + first * D, (lane & 1) ? tm_v : tm_k, bar, 0, (key0 + first) & page_mask, hk, page);
       } else {
+// where this lane's rows start, in pieces of 16 bytes; then lanes of a row share out its pieces
+        const uint8_t* k_head = static_cast<const uint8_t*>(p.k) + hk * p.ks[1];
+        const uint8_t* v_head = static_cast<const uint8_t*>(p.v) + hk * p.vs[1];
+        constexpr int kRowsAtOnce = 32 / G::kChunksPerRow;
+        const int ch = lane % G::kChunksPerRow;
 #pragma unroll
-        for (int i = 0; i < kLook; ++i)
+        for (int i = 0; i < kLook; ++i) {
+          const int row = 32 * i + lane;
+          const int page = page_of(p, sc, c, entries[i], key0 + row);
+          const uint32_t in_page = static_cast<uint32_t>((key0 + row) & page_mask), at = static_cast<uint32_t>(page);
+          const uint32_t k_at = at * static_cast<uint32_t>(p.ks[0] >> 4) + in_page * static_cast<uint32_t>(p.ks[2] >> 4);
+          const uint32_t v_at = at * static_cast<uint32_t>(p.vs[0] >> 4) + in_page * static_cast<uint32_t>(p.vs[2] >> 4);
 #pragma unroll 4
-          for (int x = lane; x < 32 * G::kChunksPerRow; x += 32) {
-            const int row = 32 * i + x / G::kChunksPerRow, ch = x % G::kChunksPerRow;
-            const int64_t page = page_of(p, sc, c, __shfl_sync(0xffffffffu, entries[i], row & 31), key0 + row);
-            if (page < 0) continue;
-            const int in_page = (key0 + row) & page_mask;
-            const uint32_t dst = stage + row * D + ((ch ^ G::swizzle(row)) << 4);
-            cp_async_16(dst, static_cast<const uint8_t*>(p.k) + hk * p.ks[1] + page * p.ks[0] + in_page * p.ks[2] + ch * 16);
-            cp_async_16(dst + G::kTileBytes, static_cast<const uint8_t*>(p.v) + hk * p.vs[1] + page * p.vs[0] + in_page * p.vs[2] + ch * 16);
+          for (int r = lane / G::kChunksPerRow; r < 32; r += kRowsAtOnce) {
+            const int there = __shfl_sync(0xffffffffu, page, r);
+            const uint32_t k_from = __shfl_sync(0xffffffffu, k_at, r), v_from = __shfl_sync(0xffffffffu, v_at, r);
+            if (there < 0) continue;
+            const uint32_t dst = stage + (32 * i + r) * D + ((ch ^ G::swizzle(32 * i + r)) << 4);
+            cp_async_16(dst, k_head + (static_cast<uint64_t>(k_from) << 4) + ch * 16);
+            cp_async_16(dst + G::kTileBytes, v_head + (static_cast<uint64_t>(v_from) << 4) + ch * 16);
           }
+        }
         cp_async_arrive(bar);   // (every lane's copies; the barrier counts the 32 lanes)
         __syncwarp();
         if (lane == 0) mbar_arrive(bar);   // (the block's record)
@@ -310,7 +328,7 @@ __device__ __forceinline__ void bring_scales(const List& l, const CacheScales& s
   int b = -1, unit = -1;   // whose queries were brought last
   const uint8_t *k_base = nullptr, *v_base = nullptr;
   auto look_up = [&]() {
-    const int* table = p.block_table + static_cast<int64_t>(ahead.b) * p.table_stride;
+    const int* table = l.table(ahead.b);
     const int key0 = ahead.blk * kBlockKeys + lane;
 #pragma unroll
     for (int i = 0; i < kLook; ++i) {
@@ -330,7 +348,7 @@ __device__ __forceinline__ void bring_scales(const List& l, const CacheScales& s
         const int hk = unit % p.Hkv, h0 = unit / p.Hkv * HEADS, heads = p.group - h0 < HEADS ? p.group - h0 : HEADS;
         k_base = sc.k + hk * sc.ks[1];
         v_base = sc.v + hk * sc.vs[1];
-        const uint16_t* q = reinterpret_cast<const uint16_t*>(p.q) + b * p.qs[0] + static_cast<int64_t>(hk * p.group + h0) * p.qs[1];
+        const uint16_t* q = reinterpret_cast<const uint16_t*>(p.q) + (b >> l.twice) * p.qs[0] + static_cast<int64_t>(hk * p.group + h0) * p.qs[1];
         if (p.qs[3] == 1 && ((reinterpret_cast<uintptr_t>(q) | static_cast<uint64_t>(p.qs[1] * 2)) & 15) == 0) {
           for (int i = lane; i < heads * (D / 8); i += 32)
             cp_async_16(smem_u32(&sync->query[s][i / (D / 8)][i % (D / 8) * 8]), q + i / (D / 8) * p.qs[1] + i % (D / 8) * 8);
@@ -373,7 +391,7 @@ __device__ __forceinline__ void bring_scales(const List& l, const CacheScales& s
 template <int D, bool BF16, int HEADS, bool TMA>
 __global__ void __launch_bounds__(kThreads, Geo<D, HEADS>::kCtas)
     decode_fp8_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const Problem p, const CacheScales sc,
-                      const OwnPartials part, const int fixed_blocks, const long long wait_limit) {
+                      const FrontKeys front, const OwnPartials part, const int fixed_blocks, const long long wait_limit) {
   using G = Geo<D, HEADS>;
   constexpr int KS = D / 16, NB = HEADS / 8;
   extern __shared__ __align__(16) uint8_t smem_raw[];
@@ -392,7 +410,7 @@ __global__ void __launch_bounds__(kThreads, Geo<D, HEADS>::kCtas)
   __syncthreads();
   pdl_wait();
   pdl_launch_dependents();   // (a gathering of the shared prefix may run beside this)
-  const List list = {p, p.Hkv * ((p.group + HEADS - 1) / HEADS)};
+  const List list = {p, front, p.Hkv * ((p.group + HEADS - 1) / HEADS), front.len > 0 ? 1 : 0};
   Cursor c = first_place(list, fixed_blocks, lane);
 
   if (warp == kWarps) {
@@ -668,7 +686,7 @@ bool tma_pages(const Problem& p, int pages) {
 }
 
 template <int D, bool BF16, int HEADS, bool TMA>
-int launch_one(const Problem& p, const CacheScales& sc, const Fp8Geometry& g, const OwnPartials& part, cudaStream_t stream) {
+int launch_one(const Problem& p, const CacheScales& sc, const Fp8Geometry& g, const FrontKeys& front, const OwnPartials& part, cudaStream_t stream) {
   CUtensorMap tk = {}, tv = {};
   if (TMA && (!make_page_map(&tk, p.k, D, 1 << p.page_shift, p.Hkv, sc.n_pages, p.ks) ||
               !make_page_map(&tv, p.v, D, 1 << p.page_shift, p.Hkv, sc.n_pages, p.vs)))
@@ -680,25 +698,33 @@ int launch_one(const Problem& p, const CacheScales& sc, const Fp8Geometry& g, co
     cudaGetLastError();
     return B200_SDPA_ERR_CUDA;
   }
-  if (!launch_pdl(kern, dim3(g.grid), kThreads, smem, stream, tk, tv, p, sc, part, g.fixed_blocks, wait_limit_cycles())) return B200_SDPA_ERR_CUDA;
+  if (!launch_pdl(kern, dim3(g.grid), kThreads, smem, stream, tk, tv, p, sc, front, part, g.fixed_blocks, wait_limit_cycles())) return B200_SDPA_ERR_CUDA;
   count_launch(KID_DECODE);
   return B200_SDPA_OK;
 }
 
 template <int D, bool BF16>
-int launch_heads(const Problem& p, const CacheScales& sc, const Fp8Geometry& g, const OwnPartials& part, cudaStream_t stream) {
+int launch_heads(const Problem& p, const CacheScales& sc, const Fp8Geometry& g, const FrontKeys& front, const OwnPartials& part, cudaStream_t stream) {
   const bool tma = tma_pages(p, sc.n_pages);
-  if (g.heads == 8) return tma ? launch_one<D, BF16, 8, true>(p, sc, g, part, stream) : launch_one<D, BF16, 8, false>(p, sc, g, part, stream);
-  return tma ? launch_one<D, BF16, 16, true>(p, sc, g, part, stream) : launch_one<D, BF16, 16, false>(p, sc, g, part, stream);
+  if (g.heads == 8) return tma ? launch_one<D, BF16, 8, true>(p, sc, g, front, part, stream) : launch_one<D, BF16, 8, false>(p, sc, g, front, part, stream);
+  return tma ? launch_one<D, BF16, 16, true>(p, sc, g, front, part, stream) : launch_one<D, BF16, 16, false>(p, sc, g, front, part, stream);
 }
 
 }  // namespace
 
-bool decode_fp8_geometry(const Problem& p, int kv_chunk, Fp8Geometry* g) {
+// Pools whose offsets the copies of small pages can count: rows in 32 bits of 16 bytes.
+bool decode_fp8_served(const Problem& p, int n_pages) {
+  if (tma_pages(p, n_pages)) return true;
+  const int64_t page = 1LL << p.page_shift, limit = 1LL << 36;
+  return p.ks[0] * n_pages + p.ks[2] * page < limit && p.vs[0] * n_pages + p.vs[2] * page < limit;
+}
+
+bool decode_fp8_geometry(const Problem& p, int front_keys, int kv_chunk, Fp8Geometry* g) {
   constexpr int64_t kSms = 148;
   g->heads = p.group <= 8 ? 8 : 16;
   g->units = p.Hkv * ((p.group + g->heads - 1) / g->heads);
-  const int64_t pairs = static_cast<int64_t>(p.B) * g->units, most = pairs * ((p.S + kBlockKeys - 1) / kBlockKeys);
+  const int64_t one = static_cast<int64_t>(p.B) * g->units, pairs = front_keys > 0 ? 2 * one : one;
+  const int64_t most = one * ((static_cast<int64_t>(p.S) + kBlockKeys - 1) / kBlockKeys + (static_cast<int64_t>(front_keys) + kBlockKeys - 1) / kBlockKeys);
   int64_t grid = kSms * (p.E == 128 || g->heads == 16 ? 2 : 3);
   static_assert(Geo<128, 8>::kCtas == 2 && Geo<128, 16>::kCtas == 2 && Geo<64, 16>::kCtas == 2 && Geo<64, 8>::kCtas == 3, "as above");
   g->fixed_blocks = 0;
@@ -707,17 +733,17 @@ bool decode_fp8_geometry(const Problem& p, int kv_chunk, Fp8Geometry* g) {
     grid = (most + g->fixed_blocks - 1) / g->fixed_blocks;
   }
   if (grid > most) grid = most;
-  if (grid + pairs > 0x7fffffffLL) return false;
+  if (grid < 1 || grid + pairs > 0x7fffffffLL) return false;
   g->grid = static_cast<int>(grid);
   g->slots = grid + pairs;
   g->bytes = static_cast<uint64_t>(g->slots) * kWarps * g->heads * (p.E + 2) * sizeof(float) + static_cast<uint64_t>(pairs) * sizeof(int2);
   return true;
 }
 
-int launch_decode_partial_fp8(const Problem& p, const CacheScales& sc, int dtype, const Fp8Geometry& g, const OwnPartials& part, cudaStream_t stream) {
+int launch_decode_partial_fp8(const Problem& p, const CacheScales& sc, int dtype, const Fp8Geometry& g, const FrontKeys& front, const OwnPartials& part, cudaStream_t stream) {
   const bool bf16 = dtype == B200_SDPA_BF16;
-  if (p.E == 128) return bf16 ? launch_heads<128, true>(p, sc, g, part, stream) : launch_heads<128, false>(p, sc, g, part, stream);
-  return bf16 ? launch_heads<64, true>(p, sc, g, part, stream) : launch_heads<64, false>(p, sc, g, part, stream);
+  if (p.E == 128) return bf16 ? launch_heads<128, true>(p, sc, g, front, part, stream) : launch_heads<128, false>(p, sc, g, front, part, stream);
+  return bf16 ? launch_heads<64, true>(p, sc, g, front, part, stream) : launch_heads<64, false>(p, sc, g, front, part, stream);
 }
 
 }  // namespace b200
