@@ -367,7 +367,7 @@ PyObject* py_decode(PyObject*, PyObject* const* args, Py_ssize_t n) {
 // ---------------------------------------------------------------------------------------------------------------------
 
 struct RotaryRest {
-  at::Tensor positions, inv_freq;   // (axes, B, L) with broadcast strides
+  at::Tensor positions, inv_freq;   // (axes, B, L), (B, L) or (L,), extents of 1 broadcast
   std::vector<int64_t> sections;
   bool interleaved = false, inverse = false;
 };
@@ -401,7 +401,8 @@ std::array<at::Tensor, 2> rotate(const at::Tensor& query, const at::Tensor& key,
   p.interleaved = r.interleaved ? 1 : 0;
   for (size_t i = 0; i < r.sections.size(); ++i) p.section[i] = static_cast<int32_t>(r.sections[i]);
   p.positions = r.positions.data_ptr();
-  copy_strides(r.positions, p.pos_stride);
+  for (int64_t i = 0, pd = r.positions.dim(); i < pd; ++i)
+    p.pos_stride[3 - pd + i] = r.positions.size(i) == 1 ? 0 : r.positions.stride(i);   // (dimensions in front: 0)
   p.inv_freq = r.inv_freq.data_ptr();
   p.positions_i64 = r.positions.scalar_type() == at::kLong;
   p.inv_freq_f64 = r.inv_freq.scalar_type() == at::kDouble;
@@ -487,8 +488,7 @@ PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
   std::array<at::Tensor, 2> out;
   {
     NoGil nogil;
-    const int64_t shape[3] = {axes, B, L};
-    r.positions = positions.expand(at::IntArrayRef(shape, 3));
+    r.positions = positions;
     if (grad) {
       auto got = Rotary::apply(q, key.defined() ? std::optional<at::Tensor>(key) : std::nullopt, r.positions, r.inv_freq, r.sections, r.interleaved, false);
       out[0] = got[0];
