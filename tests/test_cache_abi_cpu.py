@@ -98,7 +98,8 @@ def _plan(p):
     ({"scale": -1.0}, _lib.ERR_UNSUPPORTED), ({"scale": float("nan")}, _lib.ERR_UNSUPPORTED), ({"page_size": 0}, _lib.ERR_SHAPE),
     ({"prefix_len": -1}, _lib.ERR_SHAPE), ({"prefix_len": 5, "prefix_table": None}, _lib.ERR_NULL), ({"v_scales": None}, _lib.ERR_NULL),
     ({"k_scales": None, "v_scales": None}, _lib.ERR_UNSUPPORTED), ({"kv_lens": None}, _lib.ERR_NULL), ({"k_pages": 4097}, _lib.ERR_ALIGNMENT),
-    ({"prefix_len": 5, "q": 4098}, _lib.ERR_ALIGNMENT), ({"prefix_len": 5, "Hq": 258}, _lib.ERR_UNSUPPORTED), ({"B": 70000}, _lib.ERR_UNSUPPORTED),
+    ({"block_table_stride": 1 << 27}, _lib.ERR_UNSUPPORTED), ({"prefix_len": 0x7FFFFFFF}, _lib.ERR_UNSUPPORTED),
+    ({"k_scales_stride": _triple(1 << 32, 1, 1)}, _lib.ERR_UNSUPPORTED), ({"prefix_len": 5, "q": 4098}, _lib.ERR_ALIGNMENT), ({"prefix_len": 5, "Hq": 258}, _lib.ERR_UNSUPPORTED), ({"B": 70000}, _lib.ERR_UNSUPPORTED),
 ])
 def test_decode_refusals(change, code):
     assert _plan(_decode(**change))[0] == code
@@ -109,12 +110,18 @@ def test_decode_plans():
     rc, plan = _plan(_decode())
     assert rc == _lib.OK and plan.launches == 2 and plan.kv_splits >= 1
     assert plan.workspace_bytes >= 8 * plan.kv_splits * 130 * 4
+    # few sequences: the prefix is an entry before each one's own keys, in the same two launches; many: gathered, multiplied once
     rc, shared = _plan(_decode(prefix_len=1000))
-    assert rc == _lib.OK and shared.workspace_bytes > plan.workspace_bytes
-    rc, only = _plan(_decode(prefix_len=1000, block_table_stride=0, block_table=None))
-    assert rc == _lib.OK and only.kv_splits == 0
+    assert rc == _lib.OK and shared.launches == 2 and shared.workspace_bytes > plan.workspace_bytes
+    rc, shared = _plan(_decode(prefix_len=4000, B=128))
+    assert rc == _lib.OK and shared.launches == 4 and shared.workspace_bytes > 2 * 4000 * 2 * 128 * 2
+    rc, only = _plan(_decode(prefix_len=4000, B=128, block_table_stride=0, block_table=None))
+    assert rc == _lib.OK and only.kv_splits == 0 and only.launches == 3
+    # a 16-bit prefix is read in its pages, or gathered from pages of fewer than 8 rows
     rc, sixteen = _plan(_decode(prefix_len=1000, k_scales=None, v_scales=None))
-    assert rc == _lib.OK
+    assert rc == _lib.OK and sixteen.launches == 3
+    rc, sixteen = _plan(_decode(prefix_len=1000, k_scales=None, v_scales=None, page_size=4))
+    assert rc == _lib.OK and sixteen.launches == 4
 
 
 def test_struct_layout_matches_the_header():

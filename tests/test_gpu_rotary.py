@@ -1,5 +1,6 @@
 """Rotary embedding with several axes: against 64 bits, its gradient against the formula and against differences."""
 
+import gc
 import math
 
 import pytest
@@ -161,6 +162,75 @@ def test_other_stream_and_captured_graph():
     graph.replay()
     torch.cuda.synchronize()
     _check(z.cpu(), _want(q, pos + 7, freq, (16, 24, 24), False))
+
+
+def _capture_parts():
+    import torch_neuronx_b200 as T
+
+    g = torch.Generator().manual_seed(8)
+    q, k = (torch.randn(2, 5, h, 64, generator=g).transpose(1, 2) for h in (4, 2))
+    gq, gk = (torch.randn(2, h, 5, 64, generator=g) for h in (4, 2))
+    pos = torch.randint(0, 300, (2, 5), generator=g)
+    freq = _freqs(64)
+    dev = [t.cuda() for t in (q, k, gq, gk, pos, freq)]
+    lq, lk = dev[0].requires_grad_(), dev[1].requires_grad_()
+
+    def forward():
+        return T.rotary_embedding(lq, lk, dev[4], dev[5])
+
+    def step():
+        out = forward()
+        return out + torch.autograd.grad(out, (lq, lk), (dev[2], dev[3]))
+
+    def replayed(graph, got):
+        with torch.no_grad():
+            lq.mul_(-2)
+            dev[3].add_(1)
+        graph.replay()
+        torch.cuda.synchronize()
+        full = pos.expand(1, 2, 5)
+        for y, x, sign in zip(got, (q * -2, k, gq, gk + 1), (1, 1, -1, -1)):
+            _check(y.detach().cpu(), _want(x, full, freq, (32,), False, sign))
+
+    return forward, step, replayed
+
+
+def test_gradient_captured_while_an_eager_graph_lives():
+    """A training step's rotation and its gradient are captured and replayed with new inputs; an eager graph of the same
+    leaves, built on the stream that is captured, is alive all the while."""
+    forward, step, replayed = _capture_parts()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        alive = forward()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            got = step()
+    side.synchronize()
+    replayed(graph, got)
+    assert alive[0].grad_fn is not None
+
+
+def test_gradient_captured_while_a_default_stream_graph_lives_is_refused():
+    """The engine would make the default stream wait for the capture.  The call is refused while the capture is whole: it
+    ends without an error of its own, and once the eager graph is gone the same leaves are captured and replayed."""
+    forward, step, replayed = _capture_parts()
+    alive = forward()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        with pytest.raises(RuntimeError, match="eager graph from the default stream"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
+                step()
+        step()   # eager, the older graph still alive
+        side.synchronize()
+        del alive
+        gc.collect()   # (the refused step's frames, which the exception holds)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            got = step()
+    side.synchronize()
+    replayed(graph, got)
 
 
 def test_refusals():

@@ -5,7 +5,7 @@
 
 namespace b200 {
 
-// A position whose page is not there: said once, nothing is accessed.
+// A position whose page is not there is reported once.  Its write is left out, its read takes page 0 instead.
 __device__ __forceinline__ void report_page(int* status, int error, int b, int pos, int n_pages) {
   if (status != nullptr && atomicCAS(status, 0, error) == 0) {
     status[1] = b;

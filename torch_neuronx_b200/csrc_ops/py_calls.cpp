@@ -20,6 +20,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
@@ -412,6 +413,26 @@ std::array<at::Tensor, 2> rotate(const at::Tensor& query, const at::Tensor& key,
   return out;
 }
 
+// Inside a stream capture a gradient cannot flow to a leaf whose accumulation node was made on the default stream, by an
+// eager graph that is still alive: the engine would have the default stream wait for the capture, which ends the capture.
+// This runs before that wait, so that the capture itself is still whole when the error reaches its caller.
+void check_leaf_streams() {
+  const auto node = torch::autograd::get_current_node();
+  if (node == nullptr) return;
+  for (const auto& edge : node->next_edges()) {
+    if (dynamic_cast<torch::autograd::AccumulateGrad*>(edge.function.get()) == nullptr) continue;
+    const auto made_on = edge.function->stream();
+    if (!made_on.has_value() || made_on->device_type() != c10::kCUDA) continue;
+    const auto now = c10::cuda::getCurrentCUDAStream(made_on->device_index());
+    if (*made_on == now.unwrap() || *made_on != c10::cuda::getDefaultCUDAStream(made_on->device_index()).unwrap()) continue;
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    TORCH_CHECK(cudaStreamIsCapturing(now.stream(), &status) == cudaSuccess, "rotary_embedding: the stream's capture could not be queried");
+    TORCH_CHECK(status == cudaStreamCaptureStatusNone,
+                "rotary_embedding: a captured backward pass reaches a leaf that an eager graph from the default stream still holds; "
+                "drop that graph, or build it on the stream that is captured");
+  }
+}
+
 // A rotation's gradient is the rotation by the opposite angle, itself differentiable.
 struct Rotary : torch::autograd::Function<Rotary> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& query, const std::optional<at::Tensor>& key,
@@ -427,6 +448,7 @@ struct Rotary : torch::autograd::Function<Rotary> {
     return {out[0], out[1]};
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    check_leaf_streams();
     const auto saved = ctx->get_saved_variables();
     const auto sections = ctx->saved_data["sections"].toIntVector();
     const bool interleaved = ctx->saved_data["interleaved"].toBool(), inverse = !ctx->saved_data["inverse"].toBool();

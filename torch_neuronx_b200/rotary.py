@@ -28,12 +28,13 @@ def rotary_embedding(
 ):
     """``(query, key)`` rotated by their positions, in new tensors of the same layout; ``key`` may be ``None``.
 
-    ``query`` is ``(B, Hq, L, D)`` and ``key`` ``(B, Hkv, L, D)``, any strides, fp32, fp16 or bf16.  ``inv_freq`` is a
+    ``query`` is ``(B, Hq, L, D)`` and ``key`` ``(B, Hkv, L, D)``, any strides, fp32, fp16 or bf16, ``B`` at most 65535.  ``inv_freq`` is a
     contiguous fp32 or fp64 vector of ``R / 2`` frequencies (``R <= D``, even; elements behind ``R`` are copied).  ``positions`` is
     int32 or int64, ``(axes, B, L)``, or ``(B, L)`` or ``(L,)`` for one axis; extents of 1 are broadcast.  ``sections``
     says how many consecutive pairs belong to each axis (their sum is ``R / 2``).  Pair ``i`` is elements ``(i, i + R / 2)``, or
     ``(2 i, 2 i + 1)`` when ``interleaved``, and is turned by ``positions[axis of i] * inv_freq[i]``, an angle that is formed in
-    64 bits; the rest is computed in 32 and rounded once.  Gradients flow to ``query`` and ``key``."""
+    64 bits; the rest is computed in 32 and rounded once.  Gradients flow to ``query`` and ``key``; a backward pass
+    captured into a CUDA graph is refused while an eager graph that was built on the default stream still holds one of its leaves."""
     if _lib.native is not None and not torch.compiler.is_compiling():
         got = _lib.native.rotary(query, key, positions, inv_freq, sections, interleaved)
         if got is not None:
