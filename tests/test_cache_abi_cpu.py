@@ -110,6 +110,10 @@ def test_decode_plans():
     rc, plan = _plan(_decode())
     assert rc == _lib.OK and plan.launches == 2 and plan.kv_splits >= 1
     assert plan.workspace_bytes >= 8 * plan.kv_splits * 130 * 4
+    # a range longer than any table is the whole table
+    for scales in ({}, {"k_scales": None, "v_scales": None, "prefix_len": 100}):
+        rc, whole = _plan(_decode(kv_chunk=0x7FFFFFFF, **scales))
+        assert rc == _lib.OK and whole.kv_splits >= 1 and whole.workspace_bytes < 1 << 32
     # few sequences: the prefix is an entry before each one's own keys, in the same two launches; many: gathered, multiplied once
     rc, shared = _plan(_decode(prefix_len=1000))
     assert rc == _lib.OK and shared.launches == 2 and shared.workspace_bytes > plan.workspace_bytes

@@ -75,6 +75,46 @@ def test_against_64_bits(dtype, quantised, B, Hq, Hkv, D, page, P, pages, layout
     assert none is None and got is mine and torch.equal(mine, out)
 
 
+def test_largest_fp16_rows_of_an_8_bit_prefix():
+    """e4m3 makes 65536 of fp16's largest numbers.  Such keys and values, in a prefix that is gathered as fp16, count as 65504, 2^-11
+    less: scores q k / 8 of at most 2^-14 * 65536 / 8 = 1/2 are off by at most 2^-12 each, probabilities by a factor within e^(2^-11), so
+    the result by 2^-11 of the largest value, and another 2^-11 for the values' own rounding (on top of the usual)."""
+    import torch_neuronx_b200 as T
+
+    B, Hkv, D, page, P = 128, 2, 64, 16, 4000
+    q, k, v, ks, vs, prefix, table, lens = _setup(5, torch.float16, True, B, 4, Hkv, D, page, P, 1, "NHD")
+    for pool, scales in ((k, ks), (v, vs)):
+        pool.zero_()
+        scales.view(torch.uint8).fill_(127 + 8)
+    g = torch.Generator().manual_seed(6)
+    k[..., 0] = torch.randint(-1, 2, k.shape[:3], generator=g).float().mul(256).to(U.F8)      # -65536, 0, 65536
+    v[..., ::3] = torch.randint(-1, 2, v[..., ::3].shape, generator=g).float().mul(256).to(U.F8)
+    q = torch.zeros_like(q)
+    q[..., 0] = 2.0**-14 * torch.randint(-1, 2, q.shape[:3], generator=g)
+    ref, ref_l, big = U.attend(q, k, v, ks, vs, table, lens, "NHD", prefix=prefix, P=P)
+    assert ref.abs().max() < 60000
+    dev = _cuda(q, k, v, prefix)
+    T.reset_launch_counts()
+    out, lse = T.shared_prefix_decode(*dev, P, *_cuda(table, lens), need_lse=True, k_scales=_cuda(ks)[0], v_scales=_cuda(vs)[0])
+    assert T.launch_counts()["cache_read"] == 1
+    room = 2.0**-11 * ref.abs() + (2.0**-10 + 2.0**-11 + 2.0**-16) * big   # (probabilities in fp16: 2^-11)
+    assert torch.all((out.cpu().double() - ref).abs() <= room)
+    assert torch.all((lse.cpu().double() - ref_l).abs() <= 2.0**-12 + 2.0**-16 * (1 + ref_l.abs()))
+
+
+def test_subnormal_key_scales():
+    """Keys at 2^-127 under queries of 2^115: their products are ordinary numbers."""
+    import torch_neuronx_b200 as T
+
+    q, k, v, ks, vs, prefix, table, lens = _setup(9, torch.bfloat16, True, 3, 4, 2, 128, 16, 0, 9, "NHD")
+    ks.view(torch.uint8)[..., 0] = 0
+    q *= 2.0**115
+    k.view(torch.uint8)[..., 1, :] = 0   # (the other head's keys are zeros: their scale is not so small)
+    want = U.attend(q, k, v, ks, vs, table, lens, "NHD")
+    out, lse = T.paged_decode(*_cuda(q, k, v, table, lens), need_lse=True, k_scales=_cuda(ks)[0], v_scales=_cuda(vs)[0])
+    U.check(out.cpu(), lse.cpu(), want)
+
+
 def test_other_streams_and_captured_graphs():
     """Two graphs that were captured one after the other do not share their scratch; replayed with new inputs."""
     import torch_neuronx_b200 as T

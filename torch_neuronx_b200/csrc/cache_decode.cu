@@ -296,13 +296,14 @@ int geometry(const B200CacheDecodeParams& a, Geometry* g) {
   const Problem p = own_problem(a);
   *g = {};
   const int64_t rows = static_cast<int64_t>(a.B) * a.Hq;
+  const int kv_chunk = a.kv_chunk < (1 << 30) ? a.kv_chunk : 1 << 30;   // (no table has more)
   g->front = a.k_scales != nullptr && a.prefix_len > 0 && in_front(a);
   if (a.k_scales != nullptr && (p.S > 0 || g->front)) {
-    if (!decode_fp8_served(p, a.n_pages) || !decode_fp8_geometry(p, g->front ? a.prefix_len : 0, a.kv_chunk, &g->fp8)) return B200_SDPA_ERR_UNSUPPORTED;
+    if (!decode_fp8_served(p, a.n_pages) || !decode_fp8_geometry(p, g->front ? a.prefix_len : 0, kv_chunk, &g->fp8)) return B200_SDPA_ERR_UNSUPPORTED;
     g->own_bytes = aligned(g->fp8.bytes);
   } else if (p.S > 0) {
-    g->chunk = a.kv_chunk > 0 ? (a.kv_chunk + 31) / 32 * 32 : default_chunk(p);
-    g->nsplit = (p.S + g->chunk - 1) / g->chunk;
+    g->chunk = kv_chunk > 0 ? (kv_chunk + 31) / 32 * 32 : default_chunk(p);
+    g->nsplit = (p.S - 1) / g->chunk + 1;
     if (g->nsplit > 65535 || static_cast<int64_t>(p.Hkv) * ((p.group + 15) / 16) > 65535) return B200_SDPA_ERR_UNSUPPORTED;
     g->own_bytes = aligned(static_cast<uint64_t>(rows) * g->nsplit * (a.D + 2) * sizeof(float));
   }

@@ -130,9 +130,13 @@ __global__ void __launch_bounds__(kThreads) cache_write_kernel(const B200CacheRo
   }
 }
 
+// A gathered fp16 row holds nothing beyond 65504: e4m3 makes 65536 of what was at most 65504, half an fp16 step more, and an infinite
+// key or value would stand for a finite one.  NaN stays.
+__device__ __forceinline__ float within_f16(float x) { return fabsf(x) > 65504.f ? copysignf(65504.f, x) : x; }
+
 // LPR: lanes of a row, a power of two >= D / 16.  QUANT false: the pools hold the rows' own 16-bit type (strides in
-// elements).  Without lens every row is there.
-template <bool BF16, int LPR, bool QUANT>
+// elements).  Without lens every row is there.  GATHERED: rows for this library's own products.
+template <bool BF16, int LPR, bool QUANT, bool GATHERED>
 __global__ void __launch_bounds__(kThreads) cache_read_kernel(const B200CacheRowsParams p, const int page_shift, const int tokens,
                                                                const int rows_16b, const int beside) {
   constexpr int kRows = kThreads / LPR;
@@ -167,8 +171,10 @@ __global__ void __launch_bounds__(kThreads) cache_read_kernel(const B200CacheRow
           for (int i = 0; i < 4; ++i) {
             float f[4];
             unpack_e4m3x4(in[i], f);
-            out[2 * i] = pack16<BF16>(f[0] * scale, f[1] * scale);
-            out[2 * i + 1] = pack16<BF16>(f[2] * scale, f[3] * scale);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) f[j] = GATHERED && !BF16 ? within_f16(f[j] * scale) : f[j] * scale;
+            out[2 * i] = pack16<BF16>(f[0], f[1]);
+            out[2 * i + 1] = pack16<BF16>(f[2], f[3]);
           }
         } else {
           *reinterpret_cast<uint4*>(out) = ld_stream_16B(static_cast<const uint16_t*>(pool) + at);
@@ -212,7 +218,7 @@ bool rows_16b(const B200CacheRowsParams& p) {
   return true;
 }
 
-enum Direction { WRITE, READ, GATHER };
+enum Direction { WRITE, READ, GATHER, COPY };   // COPY: gathered rows of a 16-bit cache
 
 template <Direction DIR, bool BF16, int LPR> int launch_rows(const B200CacheRowsParams& p, int beside, cudaStream_t stream) {
   const int tokens = tokens_per_cta(p, kThreads / LPR, DIR == WRITE ? p.Hkv : 2 * p.Hkv);
@@ -220,7 +226,7 @@ template <Direction DIR, bool BF16, int LPR> int launch_rows(const B200CacheRows
   const int shift = page_shift_of(p.page_size);
   bool ok;
   if constexpr (DIR == WRITE) ok = launch_pdl(cache_write_kernel<BF16, LPR>, grid, kThreads, 0, stream, p, shift, tokens, rows_16b(p) ? 1 : 0);
-  else ok = launch_pdl(cache_read_kernel<BF16, LPR, DIR == READ>, grid, kThreads, 0, stream, p, shift, tokens, rows_16b(p) ? 1 : 0, beside);
+  else ok = launch_pdl(cache_read_kernel<BF16, LPR, DIR != COPY, DIR != READ>, grid, kThreads, 0, stream, p, shift, tokens, rows_16b(p) ? 1 : 0, beside);
   if (!ok) return B200_SDPA_ERR_CUDA;
   count_launch(DIR == WRITE ? KID_CACHE_WRITE : KID_CACHE_READ);
   return B200_SDPA_OK;
@@ -242,8 +248,8 @@ int launch_cache_read(const B200CacheRowsParams& p, cudaStream_t stream) {
   return p.dtype == B200_SDPA_BF16 ? launch_lanes<READ, true>(p, stream) : launch_lanes<READ, false>(p, stream);
 }
 int launch_cache_gather(const B200CacheRowsParams& p, bool beside, cudaStream_t stream) {
-  if (p.k_scales == nullptr) return launch_lanes<GATHER, true>(p, stream, beside);   // (a copy: either 16-bit type)
-  return p.dtype == B200_SDPA_BF16 ? launch_lanes<READ, true>(p, stream, beside) : launch_lanes<READ, false>(p, stream, beside);
+  if (p.k_scales == nullptr) return launch_lanes<COPY, true>(p, stream, beside);   // (a copy: either 16-bit type)
+  return p.dtype == B200_SDPA_BF16 ? launch_lanes<GATHER, true>(p, stream, beside) : launch_lanes<GATHER, false>(p, stream, beside);
 }
 
 }  // namespace b200

@@ -201,10 +201,10 @@ __device__ __forceinline__ int entry_of(const List& l, const Cursor& c, int row)
   return page;
 }
 // A number outside the pool is reported, and page 0 read in its place.
-__device__ __forceinline__ int page_of(const Problem& p, const CacheScales& sc, const Cursor& c, int entry, int row) {
+__device__ __forceinline__ int page_of(const List& l, const CacheScales& sc, const Cursor& c, int entry, int row) {
   if (row >= c.n_keys) return -1;
   if (static_cast<unsigned>(entry) < static_cast<unsigned>(sc.n_pages)) return entry;
-  report_page(p.status, B200_SDPA_ERR_PAGE, c.b, row, sc.n_pages);
+  report_page(l.p.status, B200_SDPA_ERR_PAGE, c.b >> l.twice, row, sc.n_pages);
   return 0;
 }
 
@@ -239,70 +239,70 @@ __device__ __forceinline__ void bring_rows(const List& l, const CacheScales& sc,
   int n = 0;
 #pragma unroll 1
   while (c.left > 0) {
-      const int s = n % kStages;
-      after.step(l);
-      look_up(next);
-      alive = wait_read(p, sync, n, 1, lane, wait_limit);
-      if (!alive) break;
-      const int hk = c.unit % p.Hkv;
-      const uint32_t stage = ring + s * G::kStageBytes, bar = smem_u32(&sync->full[s]);
-      const int key0 = c.blk * kBlockKeys;
-      if (lane == 0) {
-        const bool more = after.left > 0;
-        Block& k = sync->block[s];
-        k.blk = c.blk;
-        k.n_keys = c.n_keys;
-        k.last = !more || after.b != c.b || after.unit != c.unit;
-        k.next_unit = more ? after.unit : -1;
-        k.next_b = after.b;
+    const int s = n % kStages;
+    after.step(l);
+    look_up(next);
+    alive = wait_read(p, sync, n, 1, lane, wait_limit);
+    if (!alive) break;
+    const int hk = c.unit % p.Hkv;
+    const uint32_t stage = ring + s * G::kStageBytes, bar = smem_u32(&sync->full[s]);
+    const int key0 = c.blk * kBlockKeys;
+    if (lane == 0) {
+      const bool more = after.left > 0;
+      Block& k = sync->block[s];
+      k.blk = c.blk;
+      k.n_keys = c.n_keys;
+      k.last = !more || after.b != c.b || after.unit != c.unit;
+      k.next_unit = more ? after.unit : -1;
+      k.next_b = after.b;
+    }
+    if constexpr (TMA) {
+      const int rows = page_mask + 1 < kBlockKeys ? page_mask + 1 : kBlockKeys;   // of one copy
+      const int first = (lane >> 1) * rows;                  // lanes 2 i and 2 i + 1: keys and values of copy i
+      int entry = 0;
+#pragma unroll
+      for (int i = 0; i < kLook; ++i) {
+        const int e = __shfl_sync(0xffffffffu, entries[i], first & 31);
+        entry = (first >> 5) == i ? e : entry;
       }
-      if constexpr (TMA) {
-        const int rows = page_mask + 1 < kBlockKeys ? page_mask + 1 : kBlockKeys;   // of one copy
-        const int first = (lane >> 1) * rows;                  // lanes 2 i and 2 i + 1: keys and values of copy i
-        int entry = 0;
+      const int page = first < kBlockKeys ? page_of(l, sc, c, entry, key0 + first) : -1;
+      const bool mine = page >= 0;
+      const unsigned copies = __popc(__ballot_sync(0xffffffffu, mine));
+      if (lane == 0) mbar_arrive_expect_tx(bar, copies * rows * D);
+      __syncwarp();
+      if (mine)
+        tma_load_4d(stage + (lane & 1) * G::kTileBytes + first * D, (lane & 1) ? tm_v : tm_k, bar, 0, (key0 + first) & page_mask, hk, page);
+    } else {
+      // where this lane's rows start, in pieces of 16 bytes; then lanes of a row share out its pieces
+      const uint8_t* k_head = static_cast<const uint8_t*>(p.k) + hk * p.ks[1];
+      const uint8_t* v_head = static_cast<const uint8_t*>(p.v) + hk * p.vs[1];
+      constexpr int kRowsAtOnce = 32 / G::kChunksPerRow;
+      const int ch = lane % G::kChunksPerRow;
 #pragma unroll
-        for (int i = 0; i < kLook; ++i) {
-          const int e = __shfl_sync(0xffffffffu, entries[i], first & 31);
-          entry = (first >> 5) == i ? e : entry;
-        }
-        const int page = first < kBlockKeys ? page_of(p, sc, c, entry, key0 + first) : -1;
-        const bool mine = page >= 0;
-        const unsigned copies = __popc(__ballot_sync(0xffffffffu, mine));
-        if (lane == 0) mbar_arrive_expect_tx(bar, copies * rows * D);
-        __syncwarp();
-        if (mine)
-          tma_load_4d(stage + (lane & 1) * G::kTileBytes + first * D, (lane & 1) ? tm_v : tm_k, bar, 0, (key0 + first) & page_mask, hk, page);
-      } else {
-// where this lane's rows start, in pieces of 16 bytes; then lanes of a row share out its pieces
-        const uint8_t* k_head = static_cast<const uint8_t*>(p.k) + hk * p.ks[1];
-        const uint8_t* v_head = static_cast<const uint8_t*>(p.v) + hk * p.vs[1];
-        constexpr int kRowsAtOnce = 32 / G::kChunksPerRow;
-        const int ch = lane % G::kChunksPerRow;
-#pragma unroll
-        for (int i = 0; i < kLook; ++i) {
-          const int row = 32 * i + lane;
-          const int page = page_of(p, sc, c, entries[i], key0 + row);
-          const uint32_t in_page = static_cast<uint32_t>((key0 + row) & page_mask), at = static_cast<uint32_t>(page);
-          const uint32_t k_at = at * static_cast<uint32_t>(p.ks[0] >> 4) + in_page * static_cast<uint32_t>(p.ks[2] >> 4);
-          const uint32_t v_at = at * static_cast<uint32_t>(p.vs[0] >> 4) + in_page * static_cast<uint32_t>(p.vs[2] >> 4);
+      for (int i = 0; i < kLook; ++i) {
+        const int row = 32 * i + lane;
+        const int page = page_of(l, sc, c, entries[i], key0 + row);
+        const uint32_t in_page = static_cast<uint32_t>((key0 + row) & page_mask), at = static_cast<uint32_t>(page);
+        const uint32_t k_at = at * static_cast<uint32_t>(p.ks[0] >> 4) + in_page * static_cast<uint32_t>(p.ks[2] >> 4);
+        const uint32_t v_at = at * static_cast<uint32_t>(p.vs[0] >> 4) + in_page * static_cast<uint32_t>(p.vs[2] >> 4);
 #pragma unroll 4
-          for (int r = lane / G::kChunksPerRow; r < 32; r += kRowsAtOnce) {
-            const int there = __shfl_sync(0xffffffffu, page, r);
-            const uint32_t k_from = __shfl_sync(0xffffffffu, k_at, r), v_from = __shfl_sync(0xffffffffu, v_at, r);
-            if (there < 0) continue;
-            const uint32_t dst = stage + (32 * i + r) * D + ((ch ^ G::swizzle(32 * i + r)) << 4);
-            cp_async_16(dst, k_head + (static_cast<uint64_t>(k_from) << 4) + ch * 16);
-            cp_async_16(dst + G::kTileBytes, v_head + (static_cast<uint64_t>(v_from) << 4) + ch * 16);
-          }
+        for (int r = lane / G::kChunksPerRow; r < 32; r += kRowsAtOnce) {
+          const int there = __shfl_sync(0xffffffffu, page, r);
+          const uint32_t k_from = __shfl_sync(0xffffffffu, k_at, r), v_from = __shfl_sync(0xffffffffu, v_at, r);
+          if (there < 0) continue;
+          const uint32_t dst = stage + (32 * i + r) * D + ((ch ^ G::swizzle(32 * i + r)) << 4);
+          cp_async_16(dst, k_head + (static_cast<uint64_t>(k_from) << 4) + ch * 16);
+          cp_async_16(dst + G::kTileBytes, v_head + (static_cast<uint64_t>(v_from) << 4) + ch * 16);
         }
-        cp_async_arrive(bar);   // (every lane's copies; the barrier counts the 32 lanes)
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar);   // (the block's record)
       }
-      ++n;
-      c = after;
+      cp_async_arrive(bar);   // (every lane's copies; the barrier counts the 32 lanes)
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);   // (the block's record)
+    }
+    ++n;
+    c = after;
 #pragma unroll
-      for (int i = 0; i < kLook; ++i) entries[i] = next[i];
+    for (int i = 0; i < kLook; ++i) entries[i] = next[i];
   }
   if constexpr (!TMA) cp_async_wait_all();
   if (*static_cast<volatile int*>(&sync->abort_flag) != 0 && lane == 0) {
@@ -340,49 +340,49 @@ __device__ __forceinline__ void bring_scales(const List& l, const CacheScales& s
   look_up();
 #pragma unroll 1
   for (int n = 0; n < blocks; ++n) {
-      if (!wait_read(p, sync, n, 3, lane, wait_limit)) break;
-      const int s = n % kStages;
-      if (c.unit != unit || c.b != b) {
-        b = c.b;
-        unit = c.unit;
-        const int hk = unit % p.Hkv, h0 = unit / p.Hkv * HEADS, heads = p.group - h0 < HEADS ? p.group - h0 : HEADS;
-        k_base = sc.k + hk * sc.ks[1];
-        v_base = sc.v + hk * sc.vs[1];
-        const uint16_t* q = reinterpret_cast<const uint16_t*>(p.q) + (b >> l.twice) * p.qs[0] + static_cast<int64_t>(hk * p.group + h0) * p.qs[1];
-        if (p.qs[3] == 1 && ((reinterpret_cast<uintptr_t>(q) | static_cast<uint64_t>(p.qs[1] * 2)) & 15) == 0) {
-          for (int i = lane; i < heads * (D / 8); i += 32)
-            cp_async_16(smem_u32(&sync->query[s][i / (D / 8)][i % (D / 8) * 8]), q + i / (D / 8) * p.qs[1] + i % (D / 8) * 8);
-        } else {
-          for (int i = lane; i < heads * D; i += 32) sync->query[s][i / D][i % D] = q[i / D * p.qs[1] + i % D * p.qs[3]];
+    if (!wait_read(p, sync, n, 3, lane, wait_limit)) break;
+    const int s = n % kStages;
+    if (c.unit != unit || c.b != b) {
+      b = c.b;
+      unit = c.unit;
+      const int hk = unit % p.Hkv, h0 = unit / p.Hkv * HEADS, heads = p.group - h0 < HEADS ? p.group - h0 : HEADS;
+      k_base = sc.k + hk * sc.ks[1];
+      v_base = sc.v + hk * sc.vs[1];
+      const uint16_t* q = reinterpret_cast<const uint16_t*>(p.q) + (b >> l.twice) * p.qs[0] + static_cast<int64_t>(hk * p.group + h0) * p.qs[1];
+      if (p.qs[3] == 1 && ((reinterpret_cast<uintptr_t>(q) | static_cast<uint64_t>(p.qs[1] * 2)) & 15) == 0) {
+        for (int i = lane; i < heads * (D / 8); i += 32)
+          cp_async_16(smem_u32(&sync->query[s][i / (D / 8)][i % (D / 8) * 8]), q + i / (D / 8) * p.qs[1] + i % (D / 8) * 8);
+      } else {
+        for (int i = lane; i < heads * D; i += 32) sync->query[s][i / D][i % D] = q[i / D * p.qs[1] + i % D * p.qs[3]];
+      }
+    }
+    unsigned worst = 0;
+#pragma unroll
+    for (int i = 0; i < kLook; ++i) worst = max(worst, static_cast<unsigned>(e[i]));
+    if (__any_sync(0xffffffffu, worst >= static_cast<unsigned>(sc.n_pages))) {
+#pragma unroll
+      for (int i = 0; i < kLook; ++i)
+        if (static_cast<unsigned>(e[i]) >= static_cast<unsigned>(sc.n_pages)) {
+          report_page(p.status, B200_SDPA_ERR_PAGE, b >> l.twice, c.blk * kBlockKeys + lane + 32 * i, sc.n_pages);
+          e[i] = 0;
         }
-      }
-      unsigned worst = 0;
+    }
 #pragma unroll
-      for (int i = 0; i < kLook; ++i) worst = max(worst, static_cast<unsigned>(e[i]));
-      if (__any_sync(0xffffffffu, worst >= static_cast<unsigned>(sc.n_pages))) {
-#pragma unroll
-        for (int i = 0; i < kLook; ++i)
-          if (static_cast<unsigned>(e[i]) >= static_cast<unsigned>(sc.n_pages)) {
-            report_page(p.status, B200_SDPA_ERR_PAGE, b, c.blk * kBlockKeys + lane + 32 * i, sc.n_pages);
-            e[i] = 0;
-          }
-      }
-#pragma unroll
-      for (int i = 0; i < kLook; ++i) {
-        const uint32_t row = static_cast<uint32_t>((c.blk * kBlockKeys + lane + 32 * i) & page_mask);
-        const uint64_t page = static_cast<uint32_t>(e[i]);
-        const uintptr_t k = reinterpret_cast<uintptr_t>(k_base) + page * k_page + static_cast<uint64_t>(row) * k_row;
-        const uintptr_t v = reinterpret_cast<uintptr_t>(v_base) + page * v_page + static_cast<uint64_t>(row) * v_row;
-        cp_async_4(smem_u32(&sync->scale[s][0][lane + 32 * i]), reinterpret_cast<const void*>(k & ~static_cast<uintptr_t>(3)));
-        cp_async_4(smem_u32(&sync->scale[s][1][lane + 32 * i]), reinterpret_cast<const void*>(v & ~static_cast<uintptr_t>(3)));
-        sync->shift[s][0][lane + 32 * i] = static_cast<uint8_t>((k & 3) * 8);
-        sync->shift[s][1][lane + 32 * i] = static_cast<uint8_t>((v & 3) * 8);
-      }
-      cp_async_arrive(smem_u32(&sync->full[s]));
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&sync->full[s]));
-      c.step(l);
-      look_up();
+    for (int i = 0; i < kLook; ++i) {
+      const uint32_t row = static_cast<uint32_t>((c.blk * kBlockKeys + lane + 32 * i) & page_mask);
+      const uint64_t page = static_cast<uint32_t>(e[i]);
+      const uintptr_t k = reinterpret_cast<uintptr_t>(k_base) + page * k_page + static_cast<uint64_t>(row) * k_row;
+      const uintptr_t v = reinterpret_cast<uintptr_t>(v_base) + page * v_page + static_cast<uint64_t>(row) * v_row;
+      cp_async_4(smem_u32(&sync->scale[s][0][lane + 32 * i]), reinterpret_cast<const void*>(k & ~static_cast<uintptr_t>(3)));
+      cp_async_4(smem_u32(&sync->scale[s][1][lane + 32 * i]), reinterpret_cast<const void*>(v & ~static_cast<uintptr_t>(3)));
+      sync->shift[s][0][lane + 32 * i] = static_cast<uint8_t>((k & 3) * 8);
+      sync->shift[s][1][lane + 32 * i] = static_cast<uint8_t>((v & 3) * 8);
+    }
+    cp_async_arrive(smem_u32(&sync->full[s]));
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&sync->full[s]));
+    c.step(l);
+    look_up();
   }
   cp_async_wait_all();   // (before the CTA lets go of its memory, should it give up)
 }
@@ -427,237 +427,235 @@ __global__ void __launch_bounds__(kThreads, Geo<D, HEADS>::kCtas)
     const int blocks = c.left;
     bool fresh = true, ok = true;
     for (int n = 0; n < blocks; ++n) {
-      {
-        const int st = n % G::kStages;
-        ok = __all_sync(0xffffffffu, wait_clocked(smem_u32(&sync->full[st]), (n / G::kStages) & 1, &sync->abort_flag, wait_limit));
-        if (!ok) {   // the CTA gives up
-          if (lane == 0) report(p.status, 2, n, warp);
-          break;
-        }
-        const int blk = sync->block[st].blk, n_keys = sync->block[st].n_keys;
-        if (fresh) {
-          fresh = false;
-          first = blk;
-          r_exp = -CUDART_INF_F;
+      const int st = n % G::kStages;
+      ok = __all_sync(0xffffffffu, wait_clocked(smem_u32(&sync->full[st]), (n / G::kStages) & 1, &sync->abort_flag, wait_limit));
+      if (!ok) {   // the CTA gives up
+        if (lane == 0) report(p.status, 2, n, warp);
+        break;
+      }
+      const int blk = sync->block[st].blk, n_keys = sync->block[st].n_keys;
+      if (fresh) {
+        fresh = false;
+        first = blk;
+        r_exp = -CUDART_INF_F;
 #pragma unroll
-          for (int i = 0; i < NB; ++i) {
-            // fragments: k-step s holds elements 16 s + 4 tq .. + 3 of head g, as the bytes of a key's fragment word; a head's
-            // quad has all of it
-            uint32_t top = 0;   // (magnitudes of either type order like their bits)
+        for (int i = 0; i < NB; ++i) {
+          // fragments: k-step s holds elements 16 s + 4 tq .. + 3 of head g, as the bytes of a key's fragment word; a head's
+          // quad has all of it
+          uint32_t top = 0;   // (magnitudes of either type order like their bits)
 #pragma unroll
-            for (int s = 0; s < KS; ++s) {
-              q[i][s] = *reinterpret_cast<const uint2*>(&sync->query[st][8 * i + g][16 * s + 4 * tq]);
-              top = max(max(top, max(q[i][s].x & 0x7fffu, (q[i][s].x >> 16) & 0x7fffu)), max(q[i][s].y & 0x7fffu, (q[i][s].y >> 16) & 0x7fffu));
-            }
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            top = __float_as_uint(half_to_f32<BF16>(static_cast<uint16_t>(top)));
-            // largest element into [2^14, 2^15); zeros, infinities and NaN stay as they are
-            int up = top == 0u || top >= 0x7f800000u ? 0 : 127 + 14 - static_cast<int>(top >> 23);
-            if (!BF16 && up < 0) up = 0;
-            if (up > 126) up = 126;
-            const bool here = unit / p.Hkv * HEADS + 8 * i + g < p.group;   // (else the row is whatever was there)
-            const float f = __int_as_float((127 + up) << 23);               // up >= -113
-            const float factor = p.scale * kLog2e * __int_as_float((127 - up) << 23);
+          for (int s = 0; s < KS; ++s) {
+            q[i][s] = *reinterpret_cast<const uint2*>(&sync->query[st][8 * i + g][16 * s + 4 * tq]);
+            top = max(max(top, max(q[i][s].x & 0x7fffu, (q[i][s].x >> 16) & 0x7fffu)), max(q[i][s].y & 0x7fffu, (q[i][s].y >> 16) & 0x7fffu));
+          }
+          top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          top = __float_as_uint(half_to_f32<BF16>(static_cast<uint16_t>(top)));
+          // largest element into [2^14, 2^15); zeros, infinities and NaN stay as they are
+          int up = top == 0u || top >= 0x7f800000u ? 0 : 127 + 14 - static_cast<int>(top >> 23);
+          if (!BF16 && up < 0) up = 0;
+          if (up > 126) up = 126;
+          const bool here = unit / p.Hkv * HEADS + 8 * i + g < p.group;   // (else the row is whatever was there)
+          const float f = __int_as_float((127 + up) << 23);               // up >= -113
+          const float factor = p.scale * kLog2e * __int_as_float((127 - up) << 23);
 #pragma unroll
-            for (int s = 0; s < KS; ++s) {
-              const uint2 v = q[i][s];
-              q[i][s].x = here ? pack16<false>(half_to_f32<BF16>(static_cast<uint16_t>(v.x)) * f, half_to_f32<BF16>(static_cast<uint16_t>(v.x >> 16)) * f) : 0u;
-              q[i][s].y = here ? pack16<false>(half_to_f32<BF16>(static_cast<uint16_t>(v.y)) * f, half_to_f32<BF16>(static_cast<uint16_t>(v.y >> 16)) * f) : 0u;
-            }
+          for (int s = 0; s < KS; ++s) {
+            const uint2 v = q[i][s];
+            q[i][s].x = here ? pack16<false>(half_to_f32<BF16>(static_cast<uint16_t>(v.x)) * f, half_to_f32<BF16>(static_cast<uint16_t>(v.x >> 16)) * f) : 0u;
+            q[i][s].y = here ? pack16<false>(half_to_f32<BF16>(static_cast<uint16_t>(v.y)) * f, half_to_f32<BF16>(static_cast<uint16_t>(v.y >> 16)) * f) : 0u;
+          }
 #pragma unroll
-            for (int j = 0; j < D / 16; ++j)
+          for (int j = 0; j < D / 16; ++j)
 #pragma unroll
-              for (int r = 0; r < 4; ++r) o[j][i][r] = 0.f;
+            for (int r = 0; r < 4; ++r) o[j][i][r] = 0.f;
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              sl2[i][e] = __shfl_sync(0xffffffffu, here ? factor : 0.f, (2 * tq + e) * 4);
-              m[i][e] = -CUDART_INF_F;
-              lsum[i][e] = 0.f;
-            }
+          for (int e = 0; e < 2; ++e) {
+            sl2[i][e] = __shfl_sync(0xffffffffu, here ? factor : 0.f, (2 * tq + e) * 4);
+            m[i][e] = -CUDART_INF_F;
+            lsum[i][e] = 0.f;
           }
         }
-        const int key_w = blk * kBlockKeys + warp * kWarpKeys;   // first key of this warp's 32
-        if (key_w < n_keys) {
-          // the rows in matrices of 8 rows x 16 bytes: rows 0-7 and 8-15 of one piece, then of the next
-          const int row = warp * kWarpKeys + ((lane >> 3) & 1) * 8 + (lane & 7);
-          const uint32_t k_row = ring + st * G::kStageBytes + row * D, v_row = k_row + G::kTileBytes;
-          auto piece = [&](int x) { return static_cast<uint32_t>(((x + (lane >> 4)) ^ G::swizzle(lane & 7)) << 4); };
-          float kx[2][2], ev[2][2];
-          int e_max = -1;
-          uint32_t kf[2][KS / 2][4];
+      }
+      const int key_w = blk * kBlockKeys + warp * kWarpKeys;   // first key of this warp's 32
+      if (key_w < n_keys) {
+        // the rows in matrices of 8 rows x 16 bytes: rows 0-7 and 8-15 of one piece, then of the next
+        const int row = warp * kWarpKeys + ((lane >> 3) & 1) * 8 + (lane & 7);
+        const uint32_t k_row = ring + st * G::kStageBytes + row * D, v_row = k_row + G::kTileBytes;
+        auto piece = [&](int x) { return static_cast<uint32_t>(((x + (lane >> 4)) ^ G::swizzle(lane & 7)) << 4); };
+        float kx[2][2], ev[2][2];
+        int e_max = -1;
+        uint32_t kf[2][KS / 2][4];
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
+        for (int t = 0; t < 2; ++t) {
 #pragma unroll
-            for (int s = 0; s < KS; s += 2) ldsm_x4(k_row + t * 16 * D + piece(s), kf[t][s / 2]);
+          for (int s = 0; s < KS; s += 2) ldsm_x4(k_row + t * 16 * D + piece(s), kf[t][s / 2]);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const int at = warp * kWarpKeys + 16 * t + g + 8 * i;
-              const uint32_t k = (sync->scale[st][0][at] >> sync->shift[st][0][at]) & 255u, v = (sync->scale[st][1][at] >> sync->shift[st][1][at]) & 255u;
-              // 2^e as bits (2^-127 as 0: beside such a key every score is 0 in fp32), and e as a number, by way of 2^23 + code
-              kx[t][i] = __uint_as_float(k == 255u ? 0x7fffffffu : k << 23);
-              ev[t][i] = v == 255u ? CUDART_NAN_F : __uint_as_float(0x4b000000u | v) - (8388608.f + 127.f);
-              if (v < 255u && key_w + 16 * t + g + 8 * i < n_keys) e_max = max(e_max, static_cast<int>(v));
-            }
+          for (int i = 0; i < 2; ++i) {
+            const int at = warp * kWarpKeys + 16 * t + g + 8 * i;
+            const uint32_t k = (sync->scale[st][0][at] >> sync->shift[st][0][at]) & 255u, v = (sync->scale[st][1][at] >> sync->shift[st][1][at]) & 255u;
+            // 2^e as bits (2^-127 is subnormal), and e as a number, by way of 2^23 + code
+            kx[t][i] = __uint_as_float(k == 255u ? 0x7fffffffu : max(k << 23, 0x00400000u));
+            ev[t][i] = v == 255u ? CUDART_NAN_F : __uint_as_float(0x4b000000u | v) - (8388608.f + 127.f);
+            if (v < 255u && key_w + 16 * t + g + 8 * i < n_keys) e_max = max(e_max, static_cast<int>(v));
           }
-          e_max = __reduce_max_sync(0xffffffffu, e_max);
-          const float e_top = e_max < 0 ? -CUDART_INF_F : static_cast<float>(e_max - 127);   // the largest e of a value here
-          const bool tail = key_w + kWarpKeys > n_keys;
-          if (tail) {
-            // what lies behind the end is anything: its weight is 0, and 0 times a NaN is not
-            for (int i = lane; i < kWarpKeys * G::kChunksPerRow; i += 32)
-              if (key_w + i / G::kChunksPerRow >= n_keys)
-                *reinterpret_cast<uint4*>(smem + st * G::kStageBytes + G::kTileBytes + warp * kWarpKeys * D + i * 16) = make_uint4(0, 0, 0, 0);
-            fence_proxy_async_smem();   // (the stage's next block comes by tensor copies)
-            __syncwarp();
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-              for (int i = 0; i < 2; ++i)
-                if (key_w + 16 * t + g + 8 * i >= n_keys) ev[t][i] = -CUDART_INF_F;
-          }
-          // ---- S^T = K Q^T: keys 16 t + g, + 8 x heads 2 tq, 2 tq + 1
-          constexpr int kChains = NB == 1 ? 2 : 1;   // even and odd k-steps apart
-          float sv[2][NB][4], part_s[2][NB][kChains][4];
+        }
+        e_max = __reduce_max_sync(0xffffffffu, e_max);
+        const float e_top = e_max < 0 ? -CUDART_INF_F : static_cast<float>(e_max - 127);   // the largest e of a value here
+        const bool tail = key_w + kWarpKeys > n_keys;
+        if (tail) {
+          // what lies behind the end is anything: its weight is 0, and 0 times a NaN is not
+          for (int i = lane; i < kWarpKeys * G::kChunksPerRow; i += 32)
+            if (key_w + i / G::kChunksPerRow >= n_keys)
+              *reinterpret_cast<uint4*>(smem + st * G::kStageBytes + G::kTileBytes + warp * kWarpKeys * D + i * 16) = make_uint4(0, 0, 0, 0);
+          fence_proxy_async_smem();   // (the stage's next block comes by tensor copies)
+          __syncwarp();
 #pragma unroll
           for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int i = 0; i < NB; ++i)
+            for (int i = 0; i < 2; ++i)
+              if (key_w + 16 * t + g + 8 * i >= n_keys) ev[t][i] = -CUDART_INF_F;
+        }
+        // ---- S^T = K Q^T: keys 16 t + g, + 8 x heads 2 tq, 2 tq + 1
+        constexpr int kChains = NB == 1 ? 2 : 1;   // even and odd k-steps apart
+        float sv[2][NB][4], part_s[2][NB][kChains][4];
 #pragma unroll
-              for (int x = 0; x < kChains; ++x)
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) part_s[t][i][x][r] = 0.f;
+          for (int i = 0; i < NB; ++i)
 #pragma unroll
-          for (int s = 0; s < KS; ++s)
+            for (int x = 0; x < kChains; ++x)
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-              uint32_t a0, a1, a2, a3;
-              unpack_e4m3_f16(kf[t][s / 2][2 * (s & 1)], a0, a2);
-              unpack_e4m3_f16(kf[t][s / 2][2 * (s & 1) + 1], a1, a3);
+              for (int r = 0; r < 4; ++r) part_s[t][i][x][r] = 0.f;
 #pragma unroll
-              for (int i = 0; i < NB; ++i) mma_f16(part_s[t][i][s % kChains], a0, a1, a2, a3, q[i][s].x, q[i][s].y);
-            }
-          float mn[NB][2];
-          bool grow = e_top > r_exp;
-#pragma unroll
-          for (int i = 0; i < NB; ++i) {
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                sv[t][i][r] = (kChains == 2 ? part_s[t][i][0][r] + part_s[t][i][kChains - 1][r] : part_s[t][i][0][r]) * kx[t][r >> 1];
-                if (tail && key_w + 16 * t + g + 8 * (r >> 1) >= n_keys) sv[t][i][r] = -CUDART_INF_F;
-              }
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              float x = fmaxf(fmaxf(sv[0][i][e], sv[0][i][2 + e]), fmaxf(sv[1][i][e], sv[1][i][2 + e]));
-#pragma unroll
-              for (int d = 4; d < 32; d *= 2) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-              mn[i][e] = fmaxf(m[i][e], x);
-              grow |= (mn[i][e] - m[i][e]) * sl2[i][e] > kRescaleThreshold;
-            }
-          }
-          // ---- o is rescaled when the largest value exponent or a row maximum grows
-          if (__any_sync(0xffffffffu, grow)) {
-            const float re = fmaxf(r_exp, e_top);
-            const float down = re == r_exp ? 1.f : ex2(r_exp - re);   // -inf -> 0
-            r_exp = re;
-#pragma unroll
-            for (int i = 0; i < NB; ++i) {
-              float f[2];
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                f[e] = mn[i][e] == m[i][e] ? 1.f : ex2((m[i][e] - mn[i][e]) * sl2[i][e]);
-                m[i][e] = mn[i][e];
-                lsum[i][e] *= f[e];
-                f[e] *= down;
-              }
-#pragma unroll
-              for (int j = 0; j < D / 16; ++j)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) o[j][i][r] *= f[r & 1];
-            }
-          }
-          // ---- probabilities; times the value scale relative to r, hi and lo, turned round: heads g x keys 2 tq, 2 tq + 1
-          uint32_t ph[2][NB][2], pl[2][NB][2];
+        for (int s = 0; s < KS; ++s)
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
-            float w[2];
+            uint32_t a0, a1, a2, a3;
+            unpack_e4m3_f16(kf[t][s / 2][2 * (s & 1)], a0, a2);
+            unpack_e4m3_f16(kf[t][s / 2][2 * (s & 1) + 1], a1, a3);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) w[i] = ev[t][i] == -CUDART_INF_F ? 0.f : ex2(ev[t][i] - r_exp + kProbShift);
-#pragma unroll
-            for (int i = 0; i < NB; ++i) {
-              float x[4];
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const float nm = (m[i][e] == -CUDART_INF_F) ? 0.f : -m[i][e] * sl2[i][e];
-                x[e] = ex2(fmaf(sv[t][i][e], sl2[i][e], nm));
-                x[2 + e] = ex2(fmaf(sv[t][i][2 + e], sl2[i][e], nm));
-                lsum[i][e] += x[e] + x[2 + e];
-              }
-#pragma unroll
-              for (int y = 0; y < 2; ++y) {
-                split_f16(x[2 * y] * w[y], x[2 * y + 1] * w[y], ph[t][i][y], pl[t][i][y]);
-                ph[t][i][y] = turn8x8(ph[t][i][y]);
-                pl[t][i][y] = turn8x8(pl[t][i][y]);
-              }
-            }
+            for (int i = 0; i < NB; ++i) mma_f16(part_s[t][i][s % kChains], a0, a1, a2, a3, q[i][s].x, q[i][s].y);
           }
-          // ---- O^T += V^T P^T, sixteen columns of V at a time
+        float mn[NB][2];
+        bool grow = e_top > r_exp;
 #pragma unroll
-          for (int j = 0; j < D / 16; j += 2)
+        for (int i = 0; i < NB; ++i) {
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-              uint32_t vf[4];
-              ldsm_x4_trans(v_row + t * 16 * D + piece(j), vf);
+          for (int t = 0; t < 2; ++t)
 #pragma unroll
-              for (int u = 0; u < 2; ++u) {
-                uint32_t a0, a1, a2, a3;   // even and odd columns of keys 0-7, then of keys 8-15
-                unpack_e4m3_f16(__byte_perm(vf[2 * u], 0, 0x3120), a0, a1);
-                unpack_e4m3_f16(__byte_perm(vf[2 * u + 1], 0, 0x3120), a2, a3);
-#pragma unroll
-                for (int i = 0; i < NB; ++i) {
-                  mma_f16(o[j + u][i], a0, a1, a2, a3, ph[t][i][0], ph[t][i][1]);
-                  mma_f16(o[j + u][i], a0, a1, a2, a3, pl[t][i][0], pl[t][i][1]);
-                }
-              }
+            for (int r = 0; r < 4; ++r) {
+              sv[t][i][r] = (kChains == 2 ? part_s[t][i][0][r] + part_s[t][i][kChains - 1][r] : part_s[t][i][0][r]) * kx[t][r >> 1];
+              if (tail && key_w + 16 * t + g + 8 * (r >> 1) >= n_keys) sv[t][i][r] = -CUDART_INF_F;
             }
-        }
-        const int last = sync->block[st].last, next_unit = sync->block[st].next_unit, next_b = sync->block[st].next_b;
-        const bool ends = blk + 1 == (n_keys + kBlockKeys - 1) / kBlockKeys;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sync->empty[st]));
-        if (last == 0) continue;
-
-        // ---- the pair's last block here: every warp leaves its partial, the merge is the second launch's.  (A merge of the
-        // four in shared memory took longer than the few bytes more.)
-        const int64_t pair = static_cast<int64_t>(b) * list.units + unit;
-        const int64_t slot = pair + blockIdx.x;
-        if (tid == 0) {
-          if (first == 0) part.range[pair].x = static_cast<int>(slot);
-          if (ends) part.range[pair].y = static_cast<int>(slot);
-        }
-        const float back = r_exp == -CUDART_INF_F ? 0.f : ex2(0.5f * (r_exp - kProbShift));   // 2^(r - 9), in two factors
-#pragma unroll
-        for (int i = 0; i < NB; ++i)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float sum = lsum[i][e];
+            float x = fmaxf(fmaxf(sv[0][i][e], sv[0][i][2 + e]), fmaxf(sv[1][i][e], sv[1][i][2 + e]));
 #pragma unroll
-            for (int d = 4; d < 32; d *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-            const int head = 8 * i + 2 * tq + e;
-            if (unit / p.Hkv * HEADS + head >= p.group || !dbg_range(p.status, DBG_DECODE_FP8 * 100 + 1, slot, 1, part.slots)) continue;
-            const int64_t row = (slot * kWarps + warp) * HEADS + head;
+            for (int d = 4; d < 32; d *= 2) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+            mn[i][e] = fmaxf(m[i][e], x);
+            grow |= (mn[i][e] - m[i][e]) * sl2[i][e] > kRescaleThreshold;
+          }
+        }
+        // ---- o is rescaled when the largest value exponent or a row maximum grows
+        if (__any_sync(0xffffffffu, grow)) {
+          const float re = fmaxf(r_exp, e_top);
+          const float down = re == r_exp ? 1.f : ex2(r_exp - re);   // -inf -> 0
+          r_exp = re;
+#pragma unroll
+          for (int i = 0; i < NB; ++i) {
+            float f[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              f[e] = mn[i][e] == m[i][e] ? 1.f : ex2((m[i][e] - mn[i][e]) * sl2[i][e]);
+              m[i][e] = mn[i][e];
+              lsum[i][e] *= f[e];
+              f[e] *= down;
+            }
 #pragma unroll
             for (int j = 0; j < D / 16; ++j)
-              *reinterpret_cast<float2*>(part.o + row * D + 16 * j + 2 * g) = make_float2(o[j][i][e] * back * back, o[j][i][2 + e] * back * back);
-            if (g == 0)
-              *reinterpret_cast<float2*>(part.ml + row * 2) = make_float2(m[i][e] == -CUDART_INF_F ? -CUDART_INF_F : m[i][e] * sl2[i][e], sum);
+#pragma unroll
+              for (int r = 0; r < 4; ++r) o[j][i][r] *= f[r & 1];
           }
-        b = next_b;
-        unit = next_unit;
-        fresh = true;
+        }
+        // ---- probabilities; times the value scale relative to r, hi and lo, turned round: heads g x keys 2 tq, 2 tq + 1
+        uint32_t ph[2][NB][2], pl[2][NB][2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          float w[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) w[i] = ev[t][i] == -CUDART_INF_F ? 0.f : ex2(ev[t][i] - r_exp + kProbShift);
+#pragma unroll
+          for (int i = 0; i < NB; ++i) {
+            float x[4];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float nm = (m[i][e] == -CUDART_INF_F) ? 0.f : -m[i][e] * sl2[i][e];
+              x[e] = ex2(fmaf(sv[t][i][e], sl2[i][e], nm));
+              x[2 + e] = ex2(fmaf(sv[t][i][2 + e], sl2[i][e], nm));
+              lsum[i][e] += x[e] + x[2 + e];
+            }
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              split_f16(x[2 * y] * w[y], x[2 * y + 1] * w[y], ph[t][i][y], pl[t][i][y]);
+              ph[t][i][y] = turn8x8(ph[t][i][y]);
+              pl[t][i][y] = turn8x8(pl[t][i][y]);
+            }
+          }
+        }
+        // ---- O^T += V^T P^T, sixteen columns of V at a time
+#pragma unroll
+        for (int j = 0; j < D / 16; j += 2)
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            uint32_t vf[4];
+            ldsm_x4_trans(v_row + t * 16 * D + piece(j), vf);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              uint32_t a0, a1, a2, a3;   // even and odd columns of keys 0-7, then of keys 8-15
+              unpack_e4m3_f16(__byte_perm(vf[2 * u], 0, 0x3120), a0, a1);
+              unpack_e4m3_f16(__byte_perm(vf[2 * u + 1], 0, 0x3120), a2, a3);
+#pragma unroll
+              for (int i = 0; i < NB; ++i) {
+                mma_f16(o[j + u][i], a0, a1, a2, a3, ph[t][i][0], ph[t][i][1]);
+                mma_f16(o[j + u][i], a0, a1, a2, a3, pl[t][i][0], pl[t][i][1]);
+              }
+            }
+          }
       }
+      const int last = sync->block[st].last, next_unit = sync->block[st].next_unit, next_b = sync->block[st].next_b;
+      const bool ends = blk + 1 == (n_keys + kBlockKeys - 1) / kBlockKeys;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&sync->empty[st]));
+      if (last == 0) continue;
+
+      // ---- the pair's last block here: every warp leaves its partial, the merge is the second launch's.  (A merge of the
+      // four in shared memory took longer than the few bytes more.)
+      const int64_t pair = static_cast<int64_t>(b) * list.units + unit;
+      const int64_t slot = pair + blockIdx.x;
+      if (tid == 0) {
+        if (first == 0) part.range[pair].x = static_cast<int>(slot);
+        if (ends) part.range[pair].y = static_cast<int>(slot);
+      }
+      const float back = r_exp == -CUDART_INF_F ? 0.f : ex2(0.5f * (r_exp - kProbShift));   // 2^(r - 9), in two factors
+#pragma unroll
+      for (int i = 0; i < NB; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float sum = lsum[i][e];
+#pragma unroll
+          for (int d = 4; d < 32; d *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+          const int head = 8 * i + 2 * tq + e;
+          if (unit / p.Hkv * HEADS + head >= p.group || !dbg_range(p.status, DBG_DECODE_FP8 * 100 + 1, slot, 1, part.slots)) continue;
+          const int64_t row = (slot * kWarps + warp) * HEADS + head;
+#pragma unroll
+          for (int j = 0; j < D / 16; ++j)
+            *reinterpret_cast<float2*>(part.o + row * D + 16 * j + 2 * g) = make_float2(o[j][i][e] * back * back, o[j][i][2 + e] * back * back);
+          if (g == 0)
+            *reinterpret_cast<float2*>(part.ml + row * 2) = make_float2(m[i][e] == -CUDART_INF_F ? -CUDART_INF_F : m[i][e] * sl2[i][e], sum);
+        }
+      b = next_b;
+      unit = next_unit;
+      fresh = true;
     }
   }
   __syncthreads();   // (the warp that brings rows leaves last when the CTA gave up: the ring is its copies' until they have landed)
