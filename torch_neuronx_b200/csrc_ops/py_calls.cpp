@@ -466,6 +466,14 @@ struct Rotary : torch::autograd::Function<Rotary> {
   }
 };
 
+// check_leaf_streams(): the same for a backward pass in Python
+PyObject* py_check_leaf_streams(PyObject*, PyObject*) {
+  HANDLE_TH_ERRORS
+  check_leaf_streams();
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
 // rotary(query, key, positions, inv_freq, sections, interleaved) -> (query', key' or None), or None
 PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -784,6 +792,7 @@ PyMethodDef kMethods[] = {
     {"forward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_forward)), METH_FASTCALL, nullptr},
     {"decode", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_decode)), METH_FASTCALL, nullptr},
     {"rotary", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_rotary)), METH_FASTCALL, nullptr},
+    {"check_leaf_streams", reinterpret_cast<PyCFunction>(py_check_leaf_streams), METH_NOARGS, nullptr},
     {"paged_write", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_paged_write)), METH_FASTCALL, nullptr},
     {"paged_read", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_paged_read)), METH_FASTCALL, nullptr},
     {"cache_decode", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(py_cache_decode)), METH_FASTCALL, nullptr},

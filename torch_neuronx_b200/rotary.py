@@ -128,6 +128,8 @@ class _Rotary(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad_query, grad_key):
+        if _lib.native is not None:
+            _lib.native.check_leaf_streams()
         positions, inv_freq = ctx.saved_tensors
         sections, interleaved, inverse = ctx.rest
         want_q = grad_query is not None and ctx.needs_input_grad[0]
