@@ -121,11 +121,10 @@ def test_decode_plans():
     assert rc == _lib.OK and shared.launches == 4 and shared.workspace_bytes > 2 * 4000 * 2 * 128 * 2
     rc, only = _plan(_decode(prefix_len=4000, B=128, block_table_stride=0, block_table=None))
     assert rc == _lib.OK and only.kv_splits == 0 and only.launches == 3
-    # a 16-bit prefix is read in its pages, or gathered from pages of fewer than 8 rows
-    rc, sixteen = _plan(_decode(prefix_len=1000, k_scales=None, v_scales=None))
-    assert rc == _lib.OK and sixteen.launches == 3
-    rc, sixteen = _plan(_decode(prefix_len=1000, k_scales=None, v_scales=None, page_size=4))
-    assert rc == _lib.OK and sixteen.launches == 4
+    # a 16-bit prefix likewise, or it is read in its pages, or gathered from pages of fewer than 8 rows
+    for more, launches in (({}, 2), ({"B": 500}, 3), ({"B": 500, "page_size": 4}, 4)):
+        rc, sixteen = _plan(_decode(prefix_len=1000, k_scales=None, v_scales=None, **more))
+        assert rc == _lib.OK and sixteen.launches == launches
 
 
 def test_struct_layout_matches_the_header():

@@ -24,6 +24,11 @@ CASES = [
     (torch.float16, True, 300, 3, 3, 64, 4, 50, 2, "HND"),
     (torch.bfloat16, True, 64, 16, 8, 64, 4, 900, 2, "NHD"),        # small pages, gathered
     (torch.float16, True, 1, 40, 2, 128, 16, 3000, 0, "HND"),       # one sequence with nothing of its own, twenty query heads
+    (torch.bfloat16, False, 64, 16, 2, 128, 16, 1000, 3, "NHD"),    # 16-bit, the prefix once for all: in its pages ...
+    (torch.float16, False, 70, 8, 4, 64, 8, 643, 4, "HND"),
+    (torch.bfloat16, False, 40, 6, 2, 64, 1, 1501, 5, "NHD"),       # ... and gathered
+    (torch.float16, False, 3, 40, 2, 64, 2, 333, 40, "HND"),        # 16-bit likewise, twenty query heads
+    (torch.bfloat16, False, 1, 8, 1, 128, 16, 5001, 7, "NHD"),      # many ranges, most of the prefix
     (torch.bfloat16, True, 6, 8, 2, 128, 2, 333, 40, "NHD"),        # small pages, the prefix before each sequence's keys
 ]
 
@@ -115,11 +120,12 @@ def test_subnormal_key_scales():
     U.check(out.cpu(), lse.cpu(), want)
 
 
-def test_other_streams_and_captured_graphs():
+@pytest.mark.parametrize("B", [6, 400])   # the prefix for each sequence, and once for all
+def test_other_streams_and_captured_graphs(B):
     """Two graphs that were captured one after the other do not share their scratch; replayed with new inputs."""
     import torch_neuronx_b200 as T
 
-    sets = [_setup(s, torch.bfloat16, s == 2, 6, 8, 2, 128, 16, 200 * s, 3, "NHD") for s in (1, 2)]
+    sets = [_setup(s, torch.bfloat16, s == 2, B, 8, 2, 128, 16, 200 * s, 3, "NHD") for s in (1, 2)]
     graphs, outs, devs = [], [], []
     side = torch.cuda.Stream()
     for i, (q, k, v, ks, vs, prefix, table, lens) in enumerate(sets):
@@ -199,12 +205,12 @@ def test_a_serving_step(dtype):
         U.check(got[:, :, i:i + 1].cpu(), want[1].float(), want, p_bits=dtype)
 
 
-@pytest.mark.parametrize("quantised,page", [(False, 16), (False, 4), (True, 16)])
-def test_a_bad_page_is_reported(quantised, page):
+@pytest.mark.parametrize("quantised,page,B", [(False, 16, 3), (False, 4, 3), (True, 16, 3), (False, 16, 500), (False, 4, 2000), (True, 16, 1500)])
+def test_a_bad_page_is_reported(quantised, page, B):
     """A number outside the pool, in the prefix or a sequence's own table, is looked over before it is used: page 0 stands in."""
     import torch_neuronx_b200 as T
 
-    q, k, v, ks, vs, prefix, table, lens = _setup(5, torch.bfloat16, quantised, 3, 4, 2, 64, page, 5 * page, 3, "NHD")
+    q, k, v, ks, vs, prefix, table, lens = _setup(5, torch.bfloat16, quantised, B, 4, 2, 64, page, 5 * page, 3, "NHD")
     lens[0] = 3 * page
     want = U.attend(q, k, v, ks, vs, table, lens, "NHD", prefix=prefix, P=5 * page)
     dev = _cuda(q, k, v, ks, vs)

@@ -341,7 +341,7 @@ int validate_rows(const B200CacheRowsParams* a) {
   if (a->B <= 0 || a->Hkv <= 0 || a->L <= 0 || a->D <= 0 || a->n_pages <= 0) return B200_SDPA_ERR_SHAPE;
   if (!page_size_ok(a->page_size) || a->block_table_stride < 1) return B200_SDPA_ERR_SHAPE;
   if (a->D % 16 != 0 || a->D > 256 || a->B > 65535 || a->Hkv > (1 << 16)) return B200_SDPA_ERR_UNSUPPORTED;
-  if (static_cast<int64_t>(a->block_table_stride) * a->page_size > (1 << 30)) return B200_SDPA_ERR_UNSUPPORTED;
+  if (static_cast<int64_t>(a->block_table_stride) * a->page_size >= (1 << 30)) return B200_SDPA_ERR_UNSUPPORTED;
   if (a->k == nullptr || a->v == nullptr || a->k_pages == nullptr || a->v_pages == nullptr || a->k_scales == nullptr ||
       a->v_scales == nullptr || a->block_table == nullptr)
     return B200_SDPA_ERR_NULL;
@@ -362,7 +362,7 @@ int validate_cache_decode(const B200CacheDecodeParams* a) {
   if ((a->D != 64 && a->D != 128) || a->B > 65535) return B200_SDPA_ERR_UNSUPPORTED;
   if (!(a->scale > 0.f) || !(a->scale < 1e30f)) return B200_SDPA_ERR_UNSUPPORTED;
   // (positions are counted in 32 bits, up to a range of keys beyond the last)
-  if (static_cast<int64_t>(a->block_table_stride) * a->page_size > (1 << 30) || a->prefix_len > (1 << 30)) return B200_SDPA_ERR_UNSUPPORTED;
+  if (static_cast<int64_t>(a->block_table_stride) * a->page_size >= (1 << 30) || a->prefix_len >= (1 << 30)) return B200_SDPA_ERR_UNSUPPORTED;
   if (a->q == nullptr || a->out == nullptr || a->k_pages == nullptr || a->v_pages == nullptr || a->kv_lens == nullptr) return B200_SDPA_ERR_NULL;
   if ((a->k_scales == nullptr) != (a->v_scales == nullptr)) return B200_SDPA_ERR_NULL;
   if (a->block_table == nullptr && a->block_table_stride > 0) return B200_SDPA_ERR_NULL;

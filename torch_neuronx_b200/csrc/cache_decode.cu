@@ -35,7 +35,7 @@ struct Merge {
   int n_own, chunk;    // 16-bit cache: ranges of `chunk` keys, rows (sequence * Hq + head) * n_own + range
   const int2* range;   // 8-bit cache (decode_fp8.cu)
   int heads, units;
-  int front;           // the prefix's partials are among these too, each sequence's before its own
+  int front;           // the prefix's partials are among these too, each sequence's before its own (16-bit: so many of them)
 };
 
 // WARPS warps for each (sequence, query head), 4 / WARPS rows in a CTA: the prefix's partials (rows (h * B + b) * n ..) and the own
@@ -72,7 +72,12 @@ __global__ void __launch_bounds__(kCombineWarps * 32) cache_combine_kernel(const
   } else if (a.n_own > 0) {
     used = (valid_keys(p, b) + a.chunk - 1) / a.chunk;
     used = used < 1 ? 1 : (used > a.n_own ? a.n_own : used);
-    own0 = (static_cast<int64_t>(b) * p.Hq + h) * a.n_own;
+    own0 = (static_cast<int64_t>(b) * p.Hq + h) * (a.front + a.n_own);
+    if (a.front > 0) {
+      pre0 = own0;
+      n_prefix = a.front;
+      own0 += a.front;
+    }
   }
   if (!dbg_bhrc(p.status, DBG_CACHE_DECODE * 100 + 1, b, p.B, h, p.Hq, 0, 1, lane * C, C, p.Dv)) return;
   auto row_of = [&](int s) { return s < n_prefix ? pre0 + static_cast<int64_t>(s) * pre_step : own0 + static_cast<int64_t>(s - n_prefix) * step; };
@@ -166,9 +171,9 @@ __global__ void __launch_bounds__(kCombineWarps * 32) cache_combine_kernel(const
 }
 
 struct Geometry {
-  int chunk, nsplit;          // own keys of a 16-bit cache; nsplit = 0: no table, or an 8-bit cache
+  int chunk, nsplit, n_front; // own keys of a 16-bit cache; nsplit = 0: no table, or an 8-bit cache; n_front: ranges of the prefix before them
   Fp8Geometry fp8;            // own keys of an 8-bit cache
-  bool front;                 // ... and the prefix's with them, once for each sequence
+  bool front;                 // the prefix's keys with them, once for each sequence
   PackGeom pack;              // prefix
   uint64_t own_bytes, prefix_bytes, dense_bytes;
   uint64_t total() const { return own_bytes + prefix_bytes + dense_bytes; }
@@ -235,12 +240,12 @@ bool gathered(const B200CacheDecodeParams& a) {
 }
 
 // Keys of one CTA of the 16-bit kernel: enough CTAs for every slot of the GPU, ranges long enough to pay for a CTA's start and end.
-int default_chunk(const Problem& p) {
+int default_chunk(const Problem& p, int keys) {
   const int64_t units = static_cast<int64_t>(p.B) * p.Hkv * ((p.group + 15) / 16);
   int best = 256;
   double best_us = 1e30;
   for (int chunk = 64; chunk <= 2048; chunk += chunk < 512 ? 64 : 256) {
-    const int n = (p.S + chunk - 1) / chunk;
+    const int n = (keys - 1) / chunk + 1;
     const double fill = static_cast<double>(units) * n / 444;
     const double rounds = fill < 1.0 ? 1.0 : fill + 0.35;
     const double us = rounds * (3.5 + chunk / 64.0 * (1.1 + 1.6 * (fill < 1.0 ? fill : 1.0))) * (1.0 + 0.002 * n);
@@ -248,7 +253,7 @@ int default_chunk(const Problem& p) {
       best_us = us;
       best = chunk;
     }
-    if (chunk >= p.S) break;
+    if (chunk >= keys) break;
   }
   return best;
 }
@@ -257,13 +262,22 @@ int default_chunk(const Problem& p) {
 
 namespace {
 
-// Whether an 8-bit prefix is read for each sequence, before its own keys, instead of once for all.  Once for all costs two more launches
-// (gathered rows, then tiles of 128 query rows whether there are as many or not); for each costs B times the keys, from L2 all but
-// once.  Both in us, fitted to 1 to 128 sequences under 300 to 11008 keys (each against once, with up to 100 own keys): 1 sequence,
-// 8192 keys, 8 kv heads of 128: 16.4 against 27.7; 5, 3708, 4: 15.8 against 20.5; 8, 4096, 8: 26.7 against 25.9; 16, 2048, 8: 26.9
-// against 23.0; 128, 2048, 8: 105 against 38; 64, 4096, 2 heads of 64: 28.1 against 20.6.
+// Whether the prefix is read for each sequence, before its own keys, instead of once for all.  For each costs B times its keys, from
+// L2 all but once.
+// 8-bit: once for all costs two more launches (gathered rows, then tiles of 128 query rows whether there are as many or not).  Both in
+// us, fitted to 1 to 128 sequences under 300 to 11008 keys (each against once, with up to 100 own keys): 1 sequence, 8192 keys, 8 kv
+// heads of 128: 16.4 against 27.7; 5, 3708, 4: 15.8 against 20.5; 8, 4096, 8: 26.7 against 25.9; 16, 2048, 8: 26.9 against 23.0;
+// 128, 2048, 8: 105 against 38; 64, 4096, 2 heads of 64: 28.1 against 20.6.
+// 16-bit: one more launch, and the own keys run beside it; so for each only while its elements, for all sequences, are few.  With up to
+// 100 own keys: 1, 300, 2: 6.9 against 11.0; 5, 1000, 4 heads of 64: 8.2 against 10.3; 2, 2048, 8: 11.0 against 12.3; 4, 2048, 8: 13.7
+// against 12.6; 8, 1024, 8: 13.7 against 13.0; 16, 2048, 8: 27.7 against 14.6.
 bool in_front(const B200CacheDecodeParams& a) {
   const Problem f = prefix_problem(a, nullptr, nullptr);
+  if (a.k_scales == nullptr) {
+    const Problem p = own_problem(a);
+    const double keys = static_cast<double>(a.B) * a.Hkv * ((p.group + 15) / 16) * (static_cast<double>(a.prefix_len) + p.S);
+    return p.S > 0 && keys * a.D < 7.0e6;
+  }
   const int heads = f.group <= 8 ? 8 : 16;
   const double blocks = static_cast<double>(a.B) * a.Hkv * ((f.group + heads - 1) / heads) * ((a.prefix_len + 127) / 128);
   const double each = blocks / 148 * (a.D == 128 ? 1.0 : 0.6);
@@ -297,15 +311,16 @@ int geometry(const B200CacheDecodeParams& a, Geometry* g) {
   *g = {};
   const int64_t rows = static_cast<int64_t>(a.B) * a.Hq;
   const int kv_chunk = a.kv_chunk < (1 << 30) ? a.kv_chunk : 1 << 30;   // (no table has more)
-  g->front = a.k_scales != nullptr && a.prefix_len > 0 && in_front(a);
+  g->front = a.prefix_len > 0 && in_front(a);
   if (a.k_scales != nullptr && (p.S > 0 || g->front)) {
     if (!decode_fp8_served(p, a.n_pages) || !decode_fp8_geometry(p, g->front ? a.prefix_len : 0, kv_chunk, &g->fp8)) return B200_SDPA_ERR_UNSUPPORTED;
     g->own_bytes = aligned(g->fp8.bytes);
   } else if (p.S > 0) {
-    g->chunk = kv_chunk > 0 ? (kv_chunk + 31) / 32 * 32 : default_chunk(p);
+    g->chunk = kv_chunk > 0 ? (kv_chunk + 31) / 32 * 32 : default_chunk(p, p.S + (g->front ? a.prefix_len : 0));
     g->nsplit = (p.S - 1) / g->chunk + 1;
-    if (g->nsplit > 65535 || static_cast<int64_t>(p.Hkv) * ((p.group + 15) / 16) > 65535) return B200_SDPA_ERR_UNSUPPORTED;
-    g->own_bytes = aligned(static_cast<uint64_t>(rows) * g->nsplit * (a.D + 2) * sizeof(float));
+    if (g->front) g->n_front = (a.prefix_len - 1) / g->chunk + 1;
+    if (g->nsplit + g->n_front > 65535 || static_cast<int64_t>(p.Hkv) * ((p.group + 15) / 16) > 65535) return B200_SDPA_ERR_UNSUPPORTED;
+    g->own_bytes = aligned(static_cast<uint64_t>(rows) * (g->nsplit + g->n_front) * (a.D + 2) * sizeof(float));
   }
   if (a.prefix_len > 0 && !g->front) {
     const Problem f = prefix_problem(a, nullptr, nullptr);
@@ -339,10 +354,10 @@ int plan_cache_decode(const B200CacheDecodeParams& a, B200SdpaPlan* plan) {
   plan->block_n = fp8 ? 128 : g.chunk;
   plan->grid_x = fp8 ? g.fp8.grid : a.Hkv * ((a.Hq / a.Hkv + 15) / 16);
   plan->grid_y = fp8 ? 1 : a.B;
-  plan->grid_z = fp8 ? 1 : g.nsplit;
+  plan->grid_z = fp8 ? 1 : g.nsplit + g.n_front;
   plan->threads = fp8 ? 192 : 128;
   plan->smem_bytes = 0;
-  plan->kv_splits = fp8 ? g.fp8.grid : g.nsplit;
+  plan->kv_splits = fp8 ? g.fp8.grid : g.nsplit + g.n_front;
   plan->launches = 1 + (plan->kv_splits > 0 ? 1 : 0) + (a.prefix_len > 0 && !g.front ? (gathered(a) ? 2 : 1) : 0);
   plan->workspace_bytes = g.total();
   return B200_SDPA_OK;
@@ -429,11 +444,16 @@ int launch_cache_decode(const B200CacheDecodeParams& a, cudaStream_t stream) {
   }
   if (g.nsplit > 0) {
     float* own_o = reinterpret_cast<float*>(ws);
-    float* own_ml = own_o + rows * g.nsplit * a.D;
+    const int n = g.nsplit + g.n_front;
+    float* own_ml = own_o + rows * n * a.D;
     m.own = {own_o, own_ml};
+    if (g.front) {
+      m.front = g.n_front;
+      m.prefix = m.own;
+    }
     m.n_own = g.nsplit;
     m.chunk = g.chunk;
-    rc = launch_decode_partial_mma(p, a.dtype, g.chunk, g.nsplit, own_o, own_ml, stream, true);
+    rc = launch_decode_partial_mma(p, a.dtype, g.chunk, n, own_o, own_ml, stream, true, FrontKeys{a.prefix_table, a.prefix_len}, g.n_front);
     if (rc != B200_SDPA_OK) return rc;
   }
   return a.dtype == B200_SDPA_BF16 ? launch_combine<__nv_bfloat16>(p, m, stream) : launch_combine<__half>(p, m, stream);

@@ -108,9 +108,14 @@ int launch_decode(const Problem& p, int dtype, int kv_chunk, void* workspace, ui
 int plan_decode(const Problem& p, int dtype, int kv_chunk, B200SdpaPlan* plan);
 bool decode_eligible(const Problem& p, int dtype);
 bool decode_mma_eligible(const Problem& p, int dtype);
+// Keys of a prefix that every sequence shares, read for each of them before its own; len 0: none.
+struct FrontKeys {
+  const int* table;
+  int len;
+};
 // beside: (paged, no append) the launch before it in the stream is none of its inputs'
 int launch_decode_partial_mma(const Problem& p, int dtype, int chunk, int nsplit, float* part_o, float* part_ml,
-                              cudaStream_t stream, bool beside = false);
+                              cudaStream_t stream, bool beside = false, const FrontKeys& front = {}, int n_front = 0);
 int launch_decode_static(const Problem& p, int dtype, int kv_chunk, cudaStream_t stream);
 
 // `workspace` (optional, >= 4 bytes): the counter from which the persistent CTAs draw their work items
@@ -159,11 +164,6 @@ struct Fp8Geometry {
   int heads, units, grid, fixed_blocks;   // units: kv heads x blocks of query heads
   int64_t slots;
   uint64_t bytes;
-};
-// Keys of a prefix that every sequence shares, read for each of them before its own; len 0: none.
-struct FrontKeys {
-  const int* table;
-  int len;
 };
 bool decode_fp8_served(const Problem& p, int n_pages);
 bool decode_fp8_geometry(const Problem& p, int front_keys, int kv_chunk, Fp8Geometry* g);

@@ -149,11 +149,13 @@ __device__ __forceinline__ void rotate8(const Problem& p, int b, int ch, uint16_
 }
 
 // BESIDE: none of the inputs come from the launch before it in the stream, which lets this one in early: it runs beside that one
-// and waits for it at its end, so that whoever waits for this grid waits for both.
+// and waits for it at its end, so that whoever waits for this grid waits for both.  With front.len > 0 it is the first launch of
+// its call instead: ranges z < n_front are of the keys that all sequences share, the others of the sequence's own.
 template <int D, bool BF16, bool PAGED, bool APPEND, bool ROPE, bool BESIDE = false>
 __global__ void __launch_bounds__(kThreads, 3) decode_mma_kernel(const Problem p, const int chunk, const int nsplit,
                                                                  float* __restrict__ part_o,
-                                                                 float* __restrict__ part_ml) {
+                                                                 float* __restrict__ part_ml, const FrontKeys front,
+                                                                 const int n_front) {
   using G = Geo<D>;
   constexpr int KS = D / 16;   // k-steps of the first product
   constexpr int NB = D / 8;    // n-blocks of the second product
@@ -161,12 +163,13 @@ __global__ void __launch_bounds__(kThreads, 3) decode_mma_kernel(const Problem p
 
   // the split index is the slowest grid dimension: the CTAs that run last are the last chunks of the
   // longest sequences (partial, or empty for shorter ones), which keeps the tail of the launch short
-  const int split = blockIdx.z;
+  const bool shared = BESIDE && static_cast<int>(blockIdx.z) < n_front;
+  const int split = BESIDE && !shared ? blockIdx.z - n_front : blockIdx.z;
   const int hk = blockIdx.x % p.Hkv;
   const int gsub = blockIdx.x / p.Hkv;
   const int b = blockIdx.y;
-  if (!BESIDE) pdl_wait();
-  const int n_keys = valid_keys(p, b);
+  if (!BESIDE || n_front > 0) pdl_wait();
+  const int n_keys = shared ? front.len : valid_keys(p, b);
   const int s0 = split * chunk;
   if (s0 >= n_keys && split != 0) return;  // split 0 still writes an (empty) partial
   const int s1 = (s0 + chunk < n_keys) ? s0 + chunk : n_keys;
@@ -184,7 +187,7 @@ __global__ void __launch_bounds__(kThreads, 3) decode_mma_kernel(const Problem p
   const char* kbase = reinterpret_cast<const char*>(p.k) + ((PAGED ? 0 : b * p.ks[0]) + hk * p.ks[1]) * 2;
   const char* vbase = reinterpret_cast<const char*>(p.v) + ((PAGED ? 0 : b * p.vs[0]) + hk * p.vs[1]) * 2;
   const int64_t k_row = p.ks[2] * 2, v_row = p.vs[2] * 2;
-  const int* table = PAGED ? p.block_table + static_cast<int64_t>(b) * p.table_stride : nullptr;
+  const int* table = shared ? front.table : PAGED ? p.block_table + static_cast<int64_t>(b) * p.table_stride : nullptr;
   const int page_mask = (1 << p.page_shift) - 1;
   // append: the row at position `pos` (the sequence's old length) comes from k_new / v_new and is
   // written into the cache by the thread that copies it (a full cache appends nothing)
@@ -217,7 +220,8 @@ __global__ void __launch_bounds__(kThreads, 3) decode_mma_kernel(const Problem p
         const int row = s0 + blk * kBlockKeys + (tid + i * kThreads) / G::kChunksPerRow;
         const int srow = row < s1 ? row : s0;
         // (checked build: the block-table slot of this row exists; page numbers themselves are the caller's)
-        pages[i] = dbg_range(p.status, DBG_DECODE_MMA * 100 + 1, srow >> p.page_shift, 1, p.table_stride)
+        pages[i] = dbg_range(p.status, DBG_DECODE_MMA * 100 + 1, srow >> p.page_shift, 1,
+                             shared ? ((front.len - 1) >> p.page_shift) + 1 : p.table_stride)
                        ? table[srow >> p.page_shift]
                        : 0;
       }
@@ -458,7 +462,7 @@ __global__ void __launch_bounds__(kThreads, 3) decode_mma_kernel(const Problem p
       o = fmaf(sm_o[(w * 16 + row) * D + d], wgt, o);
       lsum = fmaf(sm_ml[(w * 16 + row) * 2 + 1], wgt, lsum);
     }
-    const int64_t slot = (static_cast<int64_t>(b) * p.Hq + (h0 + row)) * nsplit + split;
+    const int64_t slot = (static_cast<int64_t>(b) * p.Hq + (h0 + row)) * nsplit + (BESIDE ? blockIdx.z : split);
     if (!dbg_range(p.status, DBG_DECODE_MMA * 100 + 3, slot, 1, static_cast<int64_t>(p.B) * p.Hq * nsplit) ||
         !dbg_range(p.status, DBG_DECODE_MMA * 100 + 4, h0 + row, 1, p.Hq))
       continue;
@@ -472,7 +476,7 @@ __global__ void __launch_bounds__(kThreads, 3) decode_mma_kernel(const Problem p
 }
 
 template <int D, bool BF16, bool PAGED, bool APPEND, bool ROPE, bool BESIDE = false>
-int launch_one(const Problem& p, int chunk, int nsplit, float* po, float* pml, cudaStream_t stream) {
+int launch_one(const Problem& p, int chunk, int nsplit, float* po, float* pml, cudaStream_t stream, const FrontKeys& front = {}, int n_front = 0) {
   using G = Geo<D>;
   static_assert(kWarps * 16 * D * 4 + kWarps * 16 * 2 * 4 <= G::kSmemBytes, "merge buffer must fit in the ring");
   auto kern = decode_mma_kernel<D, BF16, PAGED, APPEND, ROPE, BESIDE>;
@@ -482,7 +486,7 @@ int launch_one(const Problem& p, int chunk, int nsplit, float* po, float* pml, c
   }
   const int nsub = (p.group + 15) / 16;
   dim3 grid(p.Hkv * nsub, p.B, nsplit);
-  if (!launch_pdl(kern, grid, kThreads, G::kSmemBytes, stream, p, chunk, nsplit, po, pml)) return B200_SDPA_ERR_CUDA;
+  if (!launch_pdl(kern, grid, kThreads, G::kSmemBytes, stream, p, chunk, nsplit, po, pml, front, n_front)) return B200_SDPA_ERR_CUDA;
   count_launch(KID_DECODE);
   return B200_SDPA_OK;
 }
@@ -497,16 +501,16 @@ bool decode_mma_eligible(const Problem& p, int dtype) {
 }
 
 int launch_decode_partial_mma(const Problem& p, int dtype, int chunk, int nsplit, float* po, float* pml,
-                              cudaStream_t stream, bool beside) {
+                              cudaStream_t stream, bool beside, const FrontKeys& front, int n_front) {
   const bool bf16 = dtype == B200_SDPA_BF16;
   const bool d128 = p.E == 128, paged = p.block_table != nullptr, append = p.k_new != nullptr;
   const bool rope = p.rope_cos != nullptr;
   if (beside) {
     if (!paged || append || rope) return B200_SDPA_ERR_UNSUPPORTED;
-    if (d128) return bf16 ? launch_one<128, true, true, false, false, true>(p, chunk, nsplit, po, pml, stream)
-                          : launch_one<128, false, true, false, false, true>(p, chunk, nsplit, po, pml, stream);
-    return bf16 ? launch_one<64, true, true, false, false, true>(p, chunk, nsplit, po, pml, stream)
-                : launch_one<64, false, true, false, false, true>(p, chunk, nsplit, po, pml, stream);
+    if (d128) return bf16 ? launch_one<128, true, true, false, false, true>(p, chunk, nsplit, po, pml, stream, front, n_front)
+                          : launch_one<128, false, true, false, false, true>(p, chunk, nsplit, po, pml, stream, front, n_front);
+    return bf16 ? launch_one<64, true, true, false, false, true>(p, chunk, nsplit, po, pml, stream, front, n_front)
+                : launch_one<64, false, true, false, false, true>(p, chunk, nsplit, po, pml, stream, front, n_front);
   }
   if (rope) {
 #define B200_DECODE_ROPE_CASE(DD, BB, PP)                                                              \
