@@ -49,6 +49,9 @@ CASES = [
     (torch.float32, 2, 5, 5, 3, 18, 6, (0, 3), False, 50),          # nothing is a whole piece, an axis without pairs
     (torch.bfloat16, 1, 1, 1, 700, 256, 256, (128,), False, 10),
     (torch.float16, 65, 12, 12, 41, 64, 48, (24,), False, 9000),    # 2665 tokens: four to a CTA, ragged
+    (torch.float32, 2, 3, 2, 9, 7, 4, (2,), False, 70),             # odd head dims: one element to copy, and three
+    (torch.bfloat16, 3, 2, 1, 6, 5, 4, (1, 1), True, 70),
+    (torch.float16, 1, 30, 7, 11, 33, 2, (1,), False, 700),
 ]
 
 

@@ -54,7 +54,7 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryArgs a) {
   const int n_tok = p.L - l0 < a.tokens ? p.L - l0 : a.tokens;
   pdl_wait();
   pdl_launch_dependents();
-  const int rot_items = a.pairs / V, items = rot_items + (p.D - p.rot) / (2 * V);   // of one head
+  const int rot_items = a.pairs / V, items = rot_items + (p.D - p.rot + (V > 1 ? 0 : 1)) / (2 * V);   // of one head
   // The heads of the queries, then of the keys.  A thread's place (token, head, item) moves on by fixed steps: dividing for
   // each item cost as much as the rotation.
   // The next item's pieces travel while one is turned, the first ones while the sines and cosines are made.
@@ -66,9 +66,12 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryArgs a) {
     int it = threadIdx.x % items, h = threadIdx.x / items % heads, t = threadIdx.x / items / heads;
     const int d_it = kThreads % items, d_h = kThreads / items % heads, d_t = kThreads / items / heads;
     __align__(16) T u[V], w[V], next_u[V], next_w[V];
-    // the two pieces of an item: the halves of V pairs, or 2 V neighbouring elements
+    // the two pieces of an item: the halves of V pairs, or 2 V neighbouring elements (V = 1, an odd number to copy: the last twice)
     auto piece0 = [&](int i) { return i >= rot_items ? p.rot + (i - rot_items) * 2 * V : (p.interleaved ? i * 2 * V : i * V); };
-    auto piece1 = [&](int i, int e0) { return i >= rot_items || p.interleaved ? e0 + V : e0 + a.pairs; };
+    auto piece1 = [&](int i, int e0) {
+      if (i >= rot_items) return V > 1 || e0 + 2 <= p.D ? e0 + V : e0;
+      return p.interleaved ? e0 + V : e0 + a.pairs;
+    };
     auto fetch = [&](int i, int hd, int tk) {
       if (tk >= n_tok) return;
       const int e0 = piece0(i), e1 = piece1(i, e0);
