@@ -73,7 +73,12 @@ template <int D, int HEADS> struct Sync {
   uint32_t scale[kStages][2][kBlockKeys];  // of the keys and of the values: the four bytes around a scale
   uint8_t shift[kStages][2][kBlockKeys];   // ... and the bit at which it starts
   int abort_flag;
+  int issued[2];                           // (left by the warps of the rows and of the scales) blocks whose copies were started
 };
+// Arrivals of a block's barrier: of the warp that brings the rows (one with the bytes of its tensor copies, or its lanes' copies and the
+// block's record), and of the warp that brings the scales (its lanes' copies, and what it stores itself).
+template <bool TMA> constexpr int kRowArrivals = TMA ? 1 : 33;
+constexpr int kScaleArrivals = 33;
 template <int D, int HEADS> constexpr int smem_bytes() {
   return Geo<D, HEADS>::kRingBytes + 1024 + static_cast<int>(sizeof(Sync<D, HEADS>));
 }
@@ -305,10 +310,7 @@ __device__ __forceinline__ void bring_rows(const List& l, const CacheScales& sc,
     for (int i = 0; i < kLook; ++i) entries[i] = next[i];
   }
   if constexpr (!TMA) cp_async_wait_all();
-  if (*static_cast<volatile int*>(&sync->abort_flag) != 0 && lane == 0) {
-    // what was issued has to land before the CTA lets go of its memory
-    for (int s = 0; s < kStages && s < n; ++s) wait_drain(smem_u32(&sync->full[s]), ((n - 1 - s) / kStages) & 1);
-  }
+  if (lane == 0) sync->issued[0] = n;
 }
 
 // The warp that brings the scales of a block's keys l, l + 32, ... and of their values, and with the first block of a pair its query
@@ -338,8 +340,9 @@ __device__ __forceinline__ void bring_scales(const List& l, const CacheScales& s
     ahead.step(l);
   };
   look_up();
+  int n = 0;
 #pragma unroll 1
-  for (int n = 0; n < blocks; ++n) {
+  for (; n < blocks; ++n) {
     if (!wait_read(p, sync, n, 3, lane, wait_limit)) break;
     const int s = n % kStages;
     if (c.unit != unit || c.b != b) {
@@ -385,6 +388,25 @@ __device__ __forceinline__ void bring_scales(const List& l, const CacheScales& s
     look_up();
   }
   cp_async_wait_all();   // (before the CTA lets go of its memory, should it give up)
+  if (lane == 0) sync->issued[1] = n;
+}
+
+// The CTA gives up (every warp has left its loop): what was started has to land before it lets go of its memory.  A block that
+// one of the two warps started and the other did not lacks the other's arrivals, which are made up, so that every stage's barrier
+// completes when its copies have landed.  The two warps are never more than a round of the ring apart.
+template <int D, int HEADS, bool TMA>
+__device__ __forceinline__ void land(Sync<D, HEADS>* sync, int warp, int lane) {
+  constexpr int kStages = Geo<D, HEADS>::kStages;
+  if (warp < kWarps || lane != 0) return;
+  const int rows = sync->issued[0], scales = sync->issued[1], most = rows > scales ? rows : scales;
+  if (warp == kWarps + 1) {
+    for (int n = scales; n < rows; ++n)
+      for (int i = 0; i < kScaleArrivals; ++i) mbar_arrive(smem_u32(&sync->full[n % kStages]));
+    return;
+  }
+  for (int n = rows; n < scales; ++n)
+    for (int i = 0; i < kRowArrivals<TMA>; ++i) mbar_arrive(smem_u32(&sync->full[n % kStages]));
+  for (int s = 0; s < kStages && s < most; ++s) wait_drain(smem_u32(&sync->full[s]), ((most - 1 - s) / kStages) & 1);
 }
 
 // HEADS: query heads of a CTA, 8 or 16.
@@ -401,7 +423,7 @@ __global__ void __launch_bounds__(kThreads, Geo<D, HEADS>::kCtas)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     for (int s = 0; s < G::kStages; ++s) {
-      mbar_init(smem_u32(&sync->full[s]), TMA ? 1 + 33 : 33 + 33);
+      mbar_init(smem_u32(&sync->full[s]), kRowArrivals<TMA> + kScaleArrivals);
       mbar_init(smem_u32(&sync->empty[s]), kWarps);
     }
     sync->abort_flag = 0;
@@ -658,7 +680,11 @@ __global__ void __launch_bounds__(kThreads, Geo<D, HEADS>::kCtas)
       fresh = true;
     }
   }
-  __syncthreads();   // (the warp that brings rows leaves last when the CTA gave up: the ring is its copies' until they have landed)
+  __syncthreads();
+  if (*static_cast<volatile int*>(&sync->abort_flag) != 0) {
+    land<D, HEADS, TMA>(sync, warp, lane);
+    __syncthreads();
+  }
 }
 
 // Pages of the pool as (bytes of a row, rows, heads, pages); one copy takes up to a block's rows of a page.
