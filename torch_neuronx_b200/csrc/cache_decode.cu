@@ -35,6 +35,7 @@ struct Merge {
   int n_own, chunk;    // 16-bit cache: ranges of `chunk` keys, rows (sequence * Hq + head) * n_own + range
   const int2* range;   // 8-bit cache (decode_fp8.cu)
   int heads, units;
+  int slots, grid;     // 8-bit cache: slots there are, and the most that one pair has
   int front;           // the prefix's partials are among these too, each sequence's before its own (16-bit: so many of them)
 };
 
@@ -55,16 +56,20 @@ __global__ void __launch_bounds__(kCombineWarps * 32) cache_combine_kernel(const
   // own partials: rows own0 + s * step; the prefix's: rows pre0 + s * pre_step
   int used = 0, step = 1, n_prefix = a.n_prefix, pre_step = 1;
   int64_t own0 = 0, pre0 = (static_cast<int64_t>(h) * p.B + b) * a.n_prefix;
+  bool torn = false;   // a wait ran out in the launch before, and a pair's slots were not noted: anything may stand there
+  auto slots_ok = [&](int2 r) { return r.x >= 0 && r.x <= r.y && r.y < a.slots && r.y - r.x < a.grid; };
   if (a.range != nullptr) {
     const int in_group = h % p.group, unit = in_group / a.heads * p.Hkv + h / p.group, twice = a.front != 0 ? 1 : 0;
     step = a.heads;
     if (valid_keys(p, b) > 0) {
       const int2 r = a.range[((static_cast<int64_t>(b) << twice) + twice) * a.units + unit];
+      torn = !slots_ok(r);
       used = (r.y - r.x + 1) * kFp8Parts;
       own0 = static_cast<int64_t>(r.x) * kFp8Parts * a.heads + in_group % a.heads;
     }
     if (twice) {
       const int2 r = a.range[(static_cast<int64_t>(b) << 1) * a.units + unit];
+      torn = torn || !slots_ok(r);
       n_prefix = (r.y - r.x + 1) * kFp8Parts;
       pre_step = a.heads;
       pre0 = static_cast<int64_t>(r.x) * kFp8Parts * a.heads + in_group % a.heads;
@@ -78,6 +83,13 @@ __global__ void __launch_bounds__(kCombineWarps * 32) cache_combine_kernel(const
       n_prefix = a.front;
       own0 += a.front;
     }
+  }
+  if (torn) {   // (for all of the row's warps alike) reported by who gave up; the row is not a number
+    if (sub == 0) {
+      for (int c = 0; c < C; ++c) reinterpret_cast<T*>(p.out)[b * p.os[0] + h * p.os[1] + (lane * C + c) * p.os[3]] = from_f32<T>(CUDART_NAN_F);
+      if (p.lse != nullptr && lane == 0) p.lse[b * p.ls[0] + h * p.ls[1]] = CUDART_NAN_F;
+    }
+    return;
   }
   if (!dbg_bhrc(p.status, DBG_CACHE_DECODE * 100 + 1, b, p.B, h, p.Hq, 0, 1, lane * C, C, p.Dv)) return;
   auto row_of = [&](int s) { return s < n_prefix ? pre0 + static_cast<int64_t>(s) * pre_step : own0 + static_cast<int64_t>(s - n_prefix) * step; };
@@ -397,6 +409,8 @@ int launch_cache_decode(const B200CacheDecodeParams& a, cudaStream_t stream) {
     m.range = part.range;
     m.heads = g.fp8.heads;
     m.units = g.fp8.units;
+    m.slots = static_cast<int>(g.fp8.slots);
+    m.grid = g.fp8.grid;
     if (g.front) {
       m.front = 1;
       m.prefix = m.own;
