@@ -8,15 +8,17 @@
 // With a prefix that all sequences share (FrontKeys) and that is not worth launches of its own, every sequence is two in the list:
 // the prefix's keys, then its own.
 // What the format changes:
-//   * e4m3 is exact in fp16, so both products are fp16 m16n8k16 MMAs with the bytes expanded in registers (8-bit MMAs would
+//   * e4m3 is exact in 16 bits, so both products are 16-bit m16n8k16 MMAs with the bytes expanded in registers (8-bit MMAs would
 //     need P and Q in 8 bits).  Both are taken transposed, S^T = K Q^T and O^T = V^T P^T: the keys, then the columns of V,
 //     fill the sixteen rows of an MMA and the query heads its eight columns, so that no row is empty and O of 8 heads
 //     needs D / 4 registers.  A fragment word of K holds four consecutive elements of one key, and the order inside a
 //     k-step is free as long as the query fragments use it too; a transposed fragment word of V holds two keys x two
 //     columns, which one byte permutation makes rows 2 i and 2 i + 1 of V^T.  movmatrix turns the probabilities round.
-//   * scores: s = (q . k8) * 2^e_k, the row's power of two applied to the finished fp32 score.  A query row is brought to
-//     a maximum in [2^14, 2^15) by a power of two first (bf16; fp16 keeps its own scale unless it has room above), so
-//     fp16 holds it exactly but for elements 2^-28 below the row's largest, which round at 2^-39 of it.
+//   * scores: s = (q . k8) * 2^e_k, the row's power of two applied to the finished fp32 score.  A bf16 query row is brought to a
+//     maximum in [2^14, 2^15) by a power of two first (fp16 keeps its own scale unless it has room above); should fp16 not hold it
+//     exactly even so -- elements below 2^-31 of the largest --, the pair's first product is a bf16 one, a byte shifted into
+//     bf16's place being the value times 2^-120 (for all bf16 queries: 64 x 512..8192 keys 134 us, not 123).  That power goes back out with
+//     the softmax's scale: maxima are kept in log2 units, which no ordinary score leaves.  Keys from 2^95 on are multiplied in another order.
 //   * values: o += (p 2^(e_v - r + 9)) v8 with r the largest e_v the warp has met (o is rescaled when it grows), so the
 //     probability stays inside fp16; it enters as hi + lo, two fp16 operands: 22 bits, and never coarser than 2^-34 of
 //     the largest value row the warp has met.
@@ -24,12 +26,14 @@
 // warps compute, 32 keys of a block each, and wait for nothing but their block.  (With plain copies and one barrier a block of 64
 // keys, as decode_mma.cu has them, the address arithmetic and the latency of table and scales stood in the way: 64 x 512..8192
 // keys, 32/8 heads of 128, 194 us.)
-// Softmax in the exp2 domain on raw scores, statistics fp32, the running maximum raised lazily (2^6).
+// Softmax in the exp2 domain, statistics fp32, the running maximum raised lazily (2^6).
 // Bound by HBM in steady state (2450 cycles for 128 keys in each of the two CTAs of an SM, 6.7 TB/s).  With the merge: 64 x 512..8192 keys,
 // 32/8 heads of 128: 118 us, 4.9 TB/s; 16 x 128..4000 keys, 12 heads of 64: 22 us; one sequence of 2001 keys: 11 us.
 #include "debug.cuh"
 #include "fp8.cuh"
 #include "tc_common.cuh"
+
+#include <type_traits>
 
 namespace b200 {
 
@@ -104,11 +108,34 @@ __device__ __forceinline__ void ldsm_x4_trans(uint32_t addr, uint32_t (&r)[4]) {
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(addr));
 }
-__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+template <bool BF16>
+__device__ __forceinline__ void mma_16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if (BF16) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    return;
+  }
   asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Four e4m3 values as two pairs: in fp16 the first two and the others, in bf16 the even and the odd ones, times 2^-120 (sign, exponent and
+// mantissa in their places; subnormal numbers stay what they are).
+template <bool BF16> __device__ __forceinline__ void unpack_key(uint32_t w, uint32_t& a, uint32_t& b) {
+  if (BF16) {
+    a = (w << 8 & 0x80008000u) | (w << 4 & 0x07f007f0u);
+    b = (w & 0x80008000u) | (w >> 4 & 0x07f007f0u);
+  } else {
+    unpack_e4m3_f16(w, a, b);
+  }
+}
+// The power of two that brings a query row, whose largest element has the bits `top`, into [2^want, 2^(want + 1)), up to 2^126.
+template <bool BF16> __device__ __forceinline__ int power_up(uint32_t top, int want) {
+  int up = top == 0u || top >= 0x7f800000u ? 0 : 127 + want - static_cast<int>(top >> 23);   // zeros, infinities and NaN stay as they are
+  if (!BF16 && up < 0) up = 0;
+  return up > 126 ? 126 : up;   // (-113 and more)
 }
 // (lo, hi) as an fp16 pair, and what the rounding left over as another.
 __device__ __forceinline__ void split_f16(float lo, float hi, uint32_t& head, uint32_t& rest) {
@@ -443,11 +470,11 @@ __global__ void __launch_bounds__(kThreads, Geo<D, HEADS>::kCtas)
     const int g = lane >> 2, tq = lane & 3;
     uint2 q[NB][KS];
     float o[D / 16][NB][4];     // O^T: rows 2 g, 2 g + 1 of sixteen columns of V; heads 2 tq, 2 tq + 1 of eight
-    float m[NB][2], lsum[NB][2], sl2[NB][2];   // of heads 2 tq, 2 tq + 1: maximum raw score, this lane's share of the sum, score to exp2 units
+    float m[NB][2], lsum[NB][2], sl2[NB][2];   // of heads 2 tq, 2 tq + 1: maximum in log2 units, this lane's share of the sum, product to log2 units
     float r_exp = -CUDART_INF_F;
     int b = c.b, unit = c.unit, first = 0;     // the pair, and its first block here
     const int blocks = c.left;
-    bool fresh = true, ok = true;
+    bool fresh = true, ok = true, wide = false;   // wide: the pair's query rows are bf16 ones here
     for (int n = 0; n < blocks; ++n) {
       const int st = n % G::kStages;
       ok = __all_sync(0xffffffffu, wait_clocked(smem_u32(&sync->full[st]), (n / G::kStages) & 1, &sync->abort_flag, wait_limit));
@@ -460,39 +487,66 @@ __global__ void __launch_bounds__(kThreads, Geo<D, HEADS>::kCtas)
         fresh = false;
         first = blk;
         r_exp = -CUDART_INF_F;
+        float factor[NB];
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
           // fragments: k-step s holds elements 16 s + 4 tq .. + 3 of head g, as the bytes of a key's fragment word; a head's
           // quad has all of it
-          uint32_t top = 0;   // (magnitudes of either type order like their bits)
+          uint32_t top2 = 0, low2 = 0;   // (magnitudes of either type order like their bits) low2: 2^15 less the smallest that is not 0
 #pragma unroll
           for (int s = 0; s < KS; ++s) {
             q[i][s] = *reinterpret_cast<const uint2*>(&sync->query[st][8 * i + g][16 * s + 4 * tq]);
-            top = max(max(top, max(q[i][s].x & 0x7fffu, (q[i][s].x >> 16) & 0x7fffu)), max(q[i][s].y & 0x7fffu, (q[i][s].y >> 16) & 0x7fffu));
+            const uint32_t x = q[i][s].x & 0x7fff7fffu, y = q[i][s].y & 0x7fff7fffu;
+            top2 = __vmaxu2(top2, __vmaxu2(x, y));
+            if (BF16) low2 = __vmaxu2(low2, __vmaxu2((0x80008000u - x) & 0x7fff7fffu, (0x80008000u - y) & 0x7fff7fffu));
           }
+          uint32_t top = max(top2 & 0xffffu, top2 >> 16);
           top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
           top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-          top = __float_as_uint(half_to_f32<BF16>(static_cast<uint16_t>(top)));
-          // largest element into [2^14, 2^15); zeros, infinities and NaN stay as they are
-          int up = top == 0u || top >= 0x7f800000u ? 0 : 127 + 14 - static_cast<int>(top >> 23);
-          if (!BF16 && up < 0) up = 0;
-          if (up > 126) up = 126;
           const bool here = unit / p.Hkv * HEADS + 8 * i + g < p.group;   // (else the row is whatever was there)
-          const float f = __int_as_float((127 + up) << 23);               // up >= -113
-          const float factor = p.scale * kLog2e * __int_as_float((127 - up) << 23);
+          if (i == 0) wide = false;
+          // (2^15 at the top, 8 bits of 2^-17: the last is fp16's last, 2^-24)
+          if (BF16 && here) wide |= static_cast<int>((0x8000u - max(low2 & 0xffffu, low2 >> 16)) >> 7) < static_cast<int>(top >> 7) - 31;
+          top = __float_as_uint(half_to_f32<BF16>(static_cast<uint16_t>(top)));
+          const int up = power_up<BF16>(top, 14);
+          const float f = __int_as_float((127 + up) << 23);
+          factor[i] = here ? p.scale * kLog2e * __int_as_float((127 - up) << 23) : 0.f;
 #pragma unroll
           for (int s = 0; s < KS; ++s) {
             const uint2 v = q[i][s];
             q[i][s].x = here ? pack16<false>(half_to_f32<BF16>(static_cast<uint16_t>(v.x)) * f, half_to_f32<BF16>(static_cast<uint16_t>(v.x >> 16)) * f) : 0u;
             q[i][s].y = here ? pack16<false>(half_to_f32<BF16>(static_cast<uint16_t>(v.y)) * f, half_to_f32<BF16>(static_cast<uint16_t>(v.y >> 16)) * f) : 0u;
           }
+        }
+        wide = BF16 && __any_sync(0xffffffffu, wide);
+        if (wide) {
+#pragma unroll
+          for (int i = 0; i < NB; ++i) {
+            const bool here = unit / p.Hkv * HEADS + 8 * i + g < p.group;
+            uint32_t top = 0;
+#pragma unroll 1
+            for (int e = 0; e < D; ++e) top = max(top, sync->query[st][8 * i + g][e] & 0x7fffu);
+            const int up = power_up<BF16>(top << 16, 126);
+            const float f = __int_as_float((127 + up) << 23);
+            if (here) factor[i] = p.scale * kLog2e * __int_as_float((127 - up) << 23) * 0x1p120f;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+              const uint2 v = *reinterpret_cast<const uint2*>(&sync->query[st][8 * i + g][16 * s + 4 * tq]);
+              const uint32_t x = pack16<true>(half_to_f32<true>(static_cast<uint16_t>(v.x)) * f, half_to_f32<true>(static_cast<uint16_t>(v.x >> 16)) * f);
+              const uint32_t y = pack16<true>(half_to_f32<true>(static_cast<uint16_t>(v.y)) * f, half_to_f32<true>(static_cast<uint16_t>(v.y >> 16)) * f);
+              q[i][s] = here ? make_uint2(__byte_perm(x, y, 0x5410), __byte_perm(x, y, 0x7632)) : make_uint2(0u, 0u);   // (as unpack_key has them)
+            }
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
 #pragma unroll
           for (int j = 0; j < D / 16; ++j)
 #pragma unroll
             for (int r = 0; r < 4; ++r) o[j][i][r] = 0.f;
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            sl2[i][e] = __shfl_sync(0xffffffffu, here ? factor : 0.f, (2 * tq + e) * 4);
+            sl2[i][e] = __shfl_sync(0xffffffffu, factor[i], (2 * tq + e) * 4);
             m[i][e] = -CUDART_INF_F;
             lsum[i][e] = 0.f;
           }
@@ -506,6 +560,7 @@ __global__ void __launch_bounds__(kThreads, Geo<D, HEADS>::kCtas)
         auto piece = [&](int x) { return static_cast<uint32_t>(((x + (lane >> 4)) ^ G::swizzle(lane & 7)) << 4); };
         float kx[2][2], ev[2][2];
         int e_max = -1;
+        bool far = false;
         uint32_t kf[2][KS / 2][4];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
@@ -518,10 +573,12 @@ __global__ void __launch_bounds__(kThreads, Geo<D, HEADS>::kCtas)
             // 2^e as bits (2^-127 is subnormal), and e as a number, by way of 2^23 + code
             kx[t][i] = __uint_as_float(k == 255u ? 0x7fffffffu : max(k << 23, 0x00400000u));
             ev[t][i] = v == 255u ? CUDART_NAN_F : __uint_as_float(0x4b000000u | v) - (8388608.f + 127.f);
+            far |= k - 222u < 33u;   // (not the NaN)
             if (v < 255u && key_w + 16 * t + g + 8 * i < n_keys) e_max = max(e_max, static_cast<int>(v));
           }
         }
         e_max = __reduce_max_sync(0xffffffffu, e_max);
+        far = __any_sync(0xffffffffu, far);
         const float e_top = e_max < 0 ? -CUDART_INF_F : static_cast<float>(e_max - 127);   // the largest e of a value here
         const bool tail = key_w + kWarpKeys > n_keys;
         if (tail) {
@@ -548,16 +605,21 @@ __global__ void __launch_bounds__(kThreads, Geo<D, HEADS>::kCtas)
             for (int x = 0; x < kChains; ++x)
 #pragma unroll
               for (int r = 0; r < 4; ++r) part_s[t][i][x][r] = 0.f;
+        auto scores = [&](auto as_bf16) {
+          constexpr bool kBf16 = decltype(as_bf16)::value;
 #pragma unroll
-        for (int s = 0; s < KS; ++s)
+          for (int s = 0; s < KS; ++s)
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            uint32_t a0, a1, a2, a3;
-            unpack_e4m3_f16(kf[t][s / 2][2 * (s & 1)], a0, a2);
-            unpack_e4m3_f16(kf[t][s / 2][2 * (s & 1) + 1], a1, a3);
+            for (int t = 0; t < 2; ++t) {
+              uint32_t a0, a1, a2, a3;
+              unpack_key<kBf16>(kf[t][s / 2][2 * (s & 1)], a0, a2);
+              unpack_key<kBf16>(kf[t][s / 2][2 * (s & 1) + 1], a1, a3);
 #pragma unroll
-            for (int i = 0; i < NB; ++i) mma_f16(part_s[t][i][s % kChains], a0, a1, a2, a3, q[i][s].x, q[i][s].y);
-          }
+              for (int i = 0; i < NB; ++i) mma_16<kBf16>(part_s[t][i][s % kChains], a0, a1, a2, a3, q[i][s].x, q[i][s].y);
+            }
+        };
+        if (BF16 && wide) scores(std::true_type{});
+        else scores(std::false_type{});
         float mn[NB][2];
         bool grow = e_top > r_exp;
 #pragma unroll
@@ -566,7 +628,9 @@ __global__ void __launch_bounds__(kThreads, Geo<D, HEADS>::kCtas)
           for (int t = 0; t < 2; ++t)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              sv[t][i][r] = (kChains == 2 ? part_s[t][i][0][r] + part_s[t][i][kChains - 1][r] : part_s[t][i][0][r]) * kx[t][r >> 1];
+              const float x = kChains == 2 ? part_s[t][i][0][r] + part_s[t][i][kChains - 1][r] : part_s[t][i][0][r];
+              // |x| <= 2^32, so below code 222 (2^95) the first product is finite; beyond, one that is not is none in the end either
+              sv[t][i][r] = far ? x * sl2[i][r & 1] * kx[t][r >> 1] : x * kx[t][r >> 1] * sl2[i][r & 1];
               if (tail && key_w + 16 * t + g + 8 * (r >> 1) >= n_keys) sv[t][i][r] = -CUDART_INF_F;
             }
 #pragma unroll
@@ -575,7 +639,7 @@ __global__ void __launch_bounds__(kThreads, Geo<D, HEADS>::kCtas)
 #pragma unroll
             for (int d = 4; d < 32; d *= 2) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
             mn[i][e] = fmaxf(m[i][e], x);
-            grow |= (mn[i][e] - m[i][e]) * sl2[i][e] > kRescaleThreshold;
+            grow |= mn[i][e] - m[i][e] > kRescaleThreshold;   // false for NaN (-inf - -inf)
           }
         }
         // ---- o is rescaled when the largest value exponent or a row maximum grows
@@ -588,7 +652,7 @@ __global__ void __launch_bounds__(kThreads, Geo<D, HEADS>::kCtas)
             float f[2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              f[e] = mn[i][e] == m[i][e] ? 1.f : ex2((m[i][e] - mn[i][e]) * sl2[i][e]);
+              f[e] = mn[i][e] == m[i][e] ? 1.f : ex2(m[i][e] - mn[i][e]);
               m[i][e] = mn[i][e];
               lsum[i][e] *= f[e];
               f[e] *= down;
@@ -611,9 +675,9 @@ __global__ void __launch_bounds__(kThreads, Geo<D, HEADS>::kCtas)
             float x[4];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const float nm = (m[i][e] == -CUDART_INF_F) ? 0.f : -m[i][e] * sl2[i][e];
-              x[e] = ex2(fmaf(sv[t][i][e], sl2[i][e], nm));
-              x[2 + e] = ex2(fmaf(sv[t][i][2 + e], sl2[i][e], nm));
+              const float nm = (m[i][e] == -CUDART_INF_F) ? 0.f : -m[i][e];
+              x[e] = ex2(sv[t][i][e] + nm);
+              x[2 + e] = ex2(sv[t][i][2 + e] + nm);
               lsum[i][e] += x[e] + x[2 + e];
             }
 #pragma unroll
@@ -638,8 +702,8 @@ __global__ void __launch_bounds__(kThreads, Geo<D, HEADS>::kCtas)
               unpack_e4m3_f16(__byte_perm(vf[2 * u + 1], 0, 0x3120), a2, a3);
 #pragma unroll
               for (int i = 0; i < NB; ++i) {
-                mma_f16(o[j + u][i], a0, a1, a2, a3, ph[t][i][0], ph[t][i][1]);
-                mma_f16(o[j + u][i], a0, a1, a2, a3, pl[t][i][0], pl[t][i][1]);
+                mma_16<false>(o[j + u][i], a0, a1, a2, a3, ph[t][i][0], ph[t][i][1]);
+                mma_16<false>(o[j + u][i], a0, a1, a2, a3, pl[t][i][0], pl[t][i][1]);
               }
             }
           }
@@ -673,7 +737,7 @@ __global__ void __launch_bounds__(kThreads, Geo<D, HEADS>::kCtas)
           for (int j = 0; j < D / 16; ++j)
             *reinterpret_cast<float2*>(part.o + row * D + 16 * j + 2 * g) = make_float2(o[j][i][e] * back * back, o[j][i][2 + e] * back * back);
           if (g == 0)
-            *reinterpret_cast<float2*>(part.ml + row * 2) = make_float2(m[i][e] == -CUDART_INF_F ? -CUDART_INF_F : m[i][e] * sl2[i][e], sum);
+            *reinterpret_cast<float2*>(part.ml + row * 2) = make_float2(m[i][e], sum);
         }
       b = next_b;
       unit = next_unit;
