@@ -224,7 +224,8 @@ def shared_prefix_decode(
     Sequence ``b`` attends to the ``prefix_len`` keys in the pages of ``prefix_table`` (int32, ``(pages,)``) and then to its own
     ``kv_lens[b]`` keys (0 is allowed) in the pages of ``block_table[b]`` -- which does not list the prefix's pages.  The result is
     that of :func:`ops.paged_decode` over the joined tables, but the prefix is read and multiplied once for the whole batch (a
-    short prefix of few sequences is read for each of them, where that is faster).
+    short prefix of few sequences is read for each of them, where that is faster), and sums are taken in another order.  As there,
+    probabilities are rounded to the type of a 16-bit cache before they meet the values, and carried as two 16-bit parts for an 8-bit one.
     ``query`` is ``(B, Hq, 1, D)`` with D 64 or 128 and at most 128 query heads for a key head; the pools are in its dtype, or 8-bit with
     ``k_scales`` and ``v_scales`` (for fp16 queries, cached values of an 8-bit prefix beyond 65504 may count as 65504).  ``prefix_len`` is a number of the host, part of a captured graph."""
     if int(prefix_len) < 0:

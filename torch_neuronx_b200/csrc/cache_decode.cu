@@ -450,10 +450,10 @@ int launch_cache_decode(const B200CacheDecodeParams& a, cudaStream_t stream) {
     r.status = a.status;
     rc = launch_cache_gather(r, g.fp8.grid > 0, stream);
     if (rc != B200_SDPA_OK) return rc;
-    rc = launch_prefix_partial(prefix_problem(a, r.k, r.v), a.dtype, g.pack, pre_o, pre_ml, stream, 0);
+    rc = launch_prefix_partial(prefix_problem(a, r.k, r.v), a.dtype, g.pack, pre_o, pre_ml, stream, 0, a.k_scales != nullptr);
     if (rc != B200_SDPA_OK) return rc;
   } else if (a.prefix_len > 0) {
-    rc = launch_prefix_partial(prefix_problem(a, nullptr, nullptr), a.dtype, g.pack, pre_o, pre_ml, stream, a.n_pages);
+    rc = launch_prefix_partial(prefix_problem(a, nullptr, nullptr), a.dtype, g.pack, pre_o, pre_ml, stream, a.n_pages, false);
     if (rc != B200_SDPA_OK) return rc;
   }
   if (g.nsplit > 0) {

@@ -184,7 +184,8 @@ bool prefix_eligible(const Problem& p, int dtype);
 void prefix_geometry(const Problem& p, PackGeom* g);
 bool prefix_paged(const Problem& p, int n_pages);
 // n_pages: k and v are pools of that many pages and block_table is the prefix's (prefix_paged() has agreed); 0: dense
-int launch_prefix_partial(const Problem& p, int dtype, const PackGeom& g, float* part_o, float* part_ml, cudaStream_t stream, int n_pages);
+// lo: (dense) probabilities enter the second product as hi + lo
+int launch_prefix_partial(const Problem& p, int dtype, const PackGeom& g, float* part_o, float* part_ml, cudaStream_t stream, int n_pages, bool lo);
 
 int launch_bwd_generic(const BwdProblem& bp, int dtype, cudaStream_t stream);
 int plan_bwd_generic(const BwdProblem& bp, int dtype, B200SdpaPlan* plan);

@@ -133,13 +133,16 @@ struct PackArgs {
 // the products run over ceil(E / 16) k-steps and ceil(Dv / 16) * 16 output columns only.  These shapes had fp32
 // probabilities on the CUDA-core kernel, so P goes into the second product as hi + lo (remainder2), lo in the second
 // half of the columns of S.
-template <int D, bool BF16, bool BIAS, bool ACC, bool PAD, bool PACK, bool PAGED = false>
+// LO: P goes in as hi + lo for a full head dimension too -- a prefix of an 8-bit cache, whose other form (decode_fp8.cu) carries 22
+// bits of P.  At D = 64 P then lies over S, as at D = 128, since tensor memory has no other columns for lo.
+template <int D, bool BF16, bool BIAS, bool ACC, bool PAD, bool PACK, bool PAGED = false, bool LO = PAD>
 __global__ void __launch_bounds__(kThreads, 1)
 prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_o, const Problem p,
                const int n_qblk, const int pair_heads, const int streams_per_wave, const long long wait_limit,
                const PackArgs pack) {
   using C = Cfg<D>;
+  constexpr bool kSplitP = C::kSplitP && !LO;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
   const uint32_t tiles = (raw_addr + 1023u) & ~1023u;            // 1024-byte aligned tile area
@@ -394,7 +397,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         constexpr int t = decltype(tile_const)::value;
         const uint64_t vd = kv_desc_v + static_cast<uint64_t>(stage * (C::kTileBytes >> 4) + half * 4 * (2048 >> 4));
         const uint32_t d_addr = tmem_base + static_cast<uint32_t>(256 + t * D);
-        const uint32_t a_addr = tmem_base + static_cast<uint32_t>(C::kSplitP ? 384 + t * 64 + half * 32 : t * 128 + half * 32);
+        const uint32_t a_addr = tmem_base + static_cast<uint32_t>(kSplitP ? 384 + t * 64 + half * 32 : t * 128 + half * 32);
         const uint32_t acc0 = (accumulate || half > 0) ? 1u : 0u;
         if (elect_one() && dbg_tmem(p.status, DBG_PREFILL * 100 + 2, d_addr, tmem_base, D, 512) &&
             dbg_tmem(p.status, DBG_PREFILL * 100 + 3, a_addr, tmem_base, 32, 512)) {
@@ -402,7 +405,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
           for (int kk = 0; kk < 4; ++kk) {
             mma_ts(d_addr, a_addr + static_cast<uint32_t>(kk * 8), vd + static_cast<uint64_t>(kk * (2048 >> 4)), idesc_pv,
                    kk > 0 ? 1u : acc0);
-            if (PAD)
+            if (LO)
               mma_ts(d_addr, a_addr + static_cast<uint32_t>(64 + kk * 8), vd + static_cast<uint64_t>(kk * (2048 >> 4)), idesc_pv, 1u);
           }
         }
@@ -443,7 +446,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
           constexpr int t = decltype(tile_const)::value;
           const int nt = t == 0 ? tg0.n_tiles : tg1.n_tiles;
           if (j >= nt) return;
-          if (C::kSplitP && j + 1 < nt) {   // as below: next scores first
+          if (kSplitP && j + 1 < nt) {   // as below: next scores first
             alive = wait_clocked(smem_u32(&sync->s_free[t]), j & 1, abort_flag, wait_limit);
             if (!alive) {
               if (lane == 0) report(p.status, 9, j, t);
@@ -468,9 +471,9 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
             issue_pv_half(tile_const, stage_addr(4 * j + 2 + t), half, j > 0);
           }
           commit(empty_bar(4 * j + 2 + t));
-          if (C::kSplitP) commit(smem_u32(&sync->pv_done[t]));
+          if (kSplitP) commit(smem_u32(&sync->pv_done[t]));
           if (j + 1 >= nt) commit(smem_u32(&sync->o_done[t]));
-          else if (!C::kSplitP) scores(tile_const, j + 1);
+          else if (!kSplitP) scores(tile_const, j + 1);
         };
         if (alive && tg0.n_tiles > 0) scores(T0, 0);
         if (alive && tg1.n_tiles > 0) scores(T1, 0);
@@ -506,7 +509,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         auto serve = [&](auto tile_const) {
           constexpr int t = decltype(tile_const)::value;
           const int nt = t == 0 ? tg0.n_tiles : tg1.n_tiles;
-          if (C::kSplitP) {
+          if (kSplitP) {
             // next scores first: S_t(j) only has to be out of tensor memory, not consumed
             if (t == 0 && has_next) {
               alive = wait_full(item_kn);
@@ -535,7 +538,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
               issue_pv_half(tile_const, stage_addr(item_v), half, j > 0);
             }
           }
-          if (C::kSplitP) {
+          if (kSplitP) {
             if (j < nt) {
               commit(smem_u32(&sync->pv_done[t]));
               if (j + 1 >= nt) commit(smem_u32(&sync->o_done[t]));
@@ -572,7 +575,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
     const uint32_t lane_off = static_cast<uint32_t>(quad * 32) << 16;
     const uint32_t s_addr = tmem_base + lane_off + static_cast<uint32_t>(t) * 128u;
     const uint32_t o_addr = tmem_base + lane_off + 256u + static_cast<uint32_t>(t) * D;
-    const uint32_t p_addr = C::kSplitP ? tmem_base + lane_off + 384u + static_cast<uint32_t>(t) * 64u : s_addr;
+    const uint32_t p_addr = kSplitP ? tmem_base + lane_off + 384u + static_cast<uint32_t>(t) * 64u : s_addr;
     // checked build: the three column ranges this thread reads and writes; a violation drains the CTA
     if (!dbg_tmem(p.status, DBG_PREFILL * 100 + 4, s_addr, tmem_base, 128, 512) ||
         !dbg_tmem(p.status, DBG_PREFILL * 100 + 5, o_addr, tmem_base, D, 512) ||
@@ -652,7 +655,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
           mxb = max3(mxb, __uint_as_float(sv[i + 2]), __uint_as_float(sv[i + 3]));
         }
         tmem_ld_wait();
-        if (C::kSplitP) {
+        if (kSplitP) {
           tc_fence_before_sync();
           mbar_arrive(smem_u32(&sync->s_free[t]));
         }
@@ -678,7 +681,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
           l_run *= alpha;
           m_run = m_new;
         }
-        if (C::kSplitP && j > 0) {
+        if (kSplitP && j > 0) {
           // here S(j) can be ready before P V of the previous tile has retired, and that product
           // still reads the P columns and writes O_t: wait for it before touching either
           bool pv_ok = wait_clocked(smem_u32(&sync->pv_done[t]), (j - 1) & 1, abort_flag, wait_limit);
@@ -712,17 +715,17 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         uint64_t sum2[2] = {0ull, 0ull};           // two packed accumulators = four chains
 #pragma unroll
         for (int c = 0; c < kBlockN / 32; ++c) {
-          uint32_t pk[16], lo[PAD ? 16 : 1];
+          uint32_t pk[16], lo[LO ? 16 : 1];
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
             const float p0 = ex2(fmaf(__uint_as_float(sv[c * 32 + i]), sl2, nms));
             const float p1 = ex2(fmaf(__uint_as_float(sv[c * 32 + i + 1]), sl2, nms));
             sum2[(i >> 1) & 1] = f2_add(sum2[(i >> 1) & 1], f2_pack(p0, p1));
             pk[i >> 1] = pack2<BF16>(p0, p1);
-            if constexpr (PAD) lo[i >> 1] = remainder2<BF16>(p0, p1, pk[i >> 1]);
+            if constexpr (LO) lo[i >> 1] = remainder2<BF16>(p0, p1, pk[i >> 1]);
           }
           tmem_st_32x16(p_addr + c * 16, pk);
-          if constexpr (PAD) tmem_st_32x16(p_addr + 64 + c * 16, lo);
+          if constexpr (LO) tmem_st_32x16(p_addr + 64 + c * 16, lo);
           if (c == 1) {
             // first 64 keys of P are in TMEM: let P V start on them while the rest is computed
             tmem_st_wait();
@@ -1111,8 +1114,8 @@ bool pack_geometry(const Problem& p, PackGeom* best) {
   return found;
 }
 
-// pages: PAGED, the problem's k and v are pools of `n_pages` pages; 0: dense.
-template <int D, bool BF16, bool PAGED = false>
+// PAGED: the problem's k and v are pools of `n_pages` pages; else dense.
+template <int D, bool BF16, bool PAGED = false, bool LO = false>
 int launch_pack_partial(const Problem& p, const PackGeom& g, float* part_o, float* part_ml, cudaStream_t stream, int n_pages = 0) {
   using C = Cfg<D>;
   CUtensorMap tq, tk, tv;
@@ -1120,7 +1123,7 @@ int launch_pack_partial(const Problem& p, const PackGeom& g, float* part_o, floa
   if (!make_map(&tq, p.q, BF16, D, p.L, p.Hq, p.B, p.qs, g.lb, p.group) || !make_map(&tk, p.k, BF16, D, rows, p.Hkv, outer, p.ks, box) ||
       !make_map(&tv, p.v, BF16, D, rows, p.Hkv, outer, p.vs, box))
     return B200_SDPA_ERR_CUDA;
-  auto kern = prefill_kernel<D, BF16, false, false, false, true, PAGED>;
+  auto kern = prefill_kernel<D, BF16, false, false, false, true, PAGED, LO>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes) != cudaSuccess) {
     cudaGetLastError();
     return B200_SDPA_ERR_CUDA;
@@ -1199,19 +1202,22 @@ void prefix_geometry(const Problem& p, PackGeom* best) {
   }
 }
 
-int launch_prefix_partial(const Problem& p, int dtype, const PackGeom& g, float* part_o, float* part_ml, cudaStream_t stream, int n_pages) {
-  if (g.grid <= 0 || g.grid > 0x7fffffffLL) return B200_SDPA_ERR_UNSUPPORTED;
+int launch_prefix_partial(const Problem& p, int dtype, const PackGeom& g, float* part_o, float* part_ml, cudaStream_t stream, int n_pages, bool lo) {
+  if (g.grid <= 0 || g.grid > 0x7fffffffLL || (n_pages > 0 && lo)) return B200_SDPA_ERR_UNSUPPORTED;
   const bool bf16 = dtype == B200_SDPA_BF16;
-  if (n_pages > 0) {
-    if (p.E == 128)
-      return bf16 ? launch_pack_partial<128, true, true>(p, g, part_o, part_ml, stream, n_pages)
-                  : launch_pack_partial<128, false, true>(p, g, part_o, part_ml, stream, n_pages);
-    return bf16 ? launch_pack_partial<64, true, true>(p, g, part_o, part_ml, stream, n_pages)
-                : launch_pack_partial<64, false, true>(p, g, part_o, part_ml, stream, n_pages);
+#define B200_PREFIX_CASE(PAGED, LO)                                                                     \
+  if ((n_pages > 0) == PAGED && lo == LO) {                                                             \
+    if (p.E == 128)                                                                                     \
+      return bf16 ? launch_pack_partial<128, true, PAGED, LO>(p, g, part_o, part_ml, stream, n_pages)   \
+                  : launch_pack_partial<128, false, PAGED, LO>(p, g, part_o, part_ml, stream, n_pages); \
+    return bf16 ? launch_pack_partial<64, true, PAGED, LO>(p, g, part_o, part_ml, stream, n_pages)      \
+                : launch_pack_partial<64, false, PAGED, LO>(p, g, part_o, part_ml, stream, n_pages);    \
   }
-  if (p.E == 128)
-    return bf16 ? launch_pack_partial<128, true>(p, g, part_o, part_ml, stream) : launch_pack_partial<128, false>(p, g, part_o, part_ml, stream);
-  return bf16 ? launch_pack_partial<64, true>(p, g, part_o, part_ml, stream) : launch_pack_partial<64, false>(p, g, part_o, part_ml, stream);
+  B200_PREFIX_CASE(true, false)
+  B200_PREFIX_CASE(false, false)
+  B200_PREFIX_CASE(false, true)
+#undef B200_PREFIX_CASE
+  return B200_SDPA_ERR_UNSUPPORTED;
 }
 
 bool prefill_eligible(const Problem& p, int dtype, bool* alignment_only_failure) {
