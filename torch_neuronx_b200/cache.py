@@ -4,7 +4,7 @@ An 8-bit cache is two pools of e4m3 values beside two of row scales: ``(pages, p
 ``torch.float8_e4m3fn`` and ``(pages, page_size, Hkv)`` of ``torch.float8_e8m0fnu`` for ``layout="NHD"``,
 ``(pages, Hkv, page_size, D)`` and ``(pages, Hkv, page_size)`` for ``"HND"``.  A row (one token, one head) stands for
 ``value * scale``; the scale is the least power of two with which the row fits e4m3.  Pages, block tables and lengths are
-those of :func:`ops.paged_decode`.
+those of :func:`ops.paged_decode`.  No gradient flows through any of this, and a trace cannot record it.
 """
 
 from __future__ import annotations
@@ -129,6 +129,7 @@ def paged_write(
     if native is not None and layout in _LAYOUTS and native.paged_write(
             key, value, k_pages, v_pages, k_scales, v_scales, block_table, start, lens, _LAYOUTS[layout]):
         return
+    ops._check_visible("paged_write")
     if key.dim() != 4 or value.shape != key.shape:
         raise RuntimeError("paged_write: key and value must be 4-D (B, Hkv, L, D) and of the same shape")
     if key.dtype not in _HALF or value.dtype != key.dtype or value.device != key.device:
@@ -171,6 +172,7 @@ def paged_read(
         got = native.paged_read(k_pages, v_pages, k_scales, v_scales, block_table, kv_lens, max_len, dtype == torch.bfloat16, _LAYOUTS[layout])
         if got is not None:
             return got
+    ops._check_visible("paged_read")
     hd, rd = _dims(layout)
     if dtype not in _HALF:
         raise RuntimeError("paged_read: dtype must be float16 or bfloat16")
@@ -252,6 +254,7 @@ def _decode(op, query, k_pages, v_pages, k_scales, v_scales, block_table, kv_len
                                   _LAYOUTS[layout], out, lse, need_lse, kv_chunk)
         if got is not None:
             return got
+    ops._check_visible(op)
     hd, rd = _dims(layout)
     if query.dim() != 4 or query.shape[2] != 1:
         raise RuntimeError(f"{op}: query must be (B, Hq, 1, D) and the page pools 4-D")

@@ -114,6 +114,17 @@ def release_workspaces() -> None:
     _retired_workspaces.clear()
 
 
+def _check_visible(op: str) -> None:
+    """Raise where a call that goes to the library by pointers would be lost: a trace would record nothing of it but its
+    allocations, and a function transform hands out tensors without memory."""
+    if torch.compiler.is_compiling():
+        return   # (a call by pointers ends the compiled graph by itself)
+    if torch.jit.is_tracing() or torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None:
+        raise RuntimeError(f"{op}: a trace cannot record this call")
+    if torch._C._functorch.maybe_current_level() is not None:
+        raise RuntimeError(f"{op}: no function transform knows this call")
+
+
 def check_device_status(device=None) -> None:
     """Synchronise and raise if any kernel reported a device-side error (a bounded
     wait that gave up).  Cheap enough for tests; not called on the hot path."""

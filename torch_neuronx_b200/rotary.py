@@ -33,12 +33,14 @@ def rotary_embedding(
     int32 or int64, ``(axes, B, L)``, or ``(B, L)`` or ``(L,)`` for one axis; extents of 1 are broadcast.  ``sections``
     says how many consecutive pairs belong to each axis (their sum is ``R / 2``).  Pair ``i`` is elements ``(i, i + R / 2)``, or
     ``(2 i, 2 i + 1)`` when ``interleaved``, and is turned by ``positions[axis of i] * inv_freq[i]``, an angle that is formed in
-    64 bits; the rest is computed in 32 and rounded once.  Gradients flow to ``query`` and ``key``; a backward pass
+    64 bits; the rest is computed in 32 and rounded once.  Gradients flow to ``query`` and ``key``; a trace cannot record
+    the call.  A backward pass
     captured into a CUDA graph is refused while an eager graph that was built on the default stream still holds one of its leaves."""
     if _lib.native is not None and not torch.compiler.is_compiling():
         got = _lib.native.rotary(query, key, positions, inv_freq, sections, interleaved)
         if got is not None:
             return got
+    ops._check_visible("rotary_embedding")
     args = _check(query, key, positions, inv_freq, sections)
     wants = torch.is_grad_enabled() and (query.requires_grad or (key is not None and key.requires_grad))
     if wants:
