@@ -4,7 +4,7 @@ refused, never lost."""
 import pytest
 import torch
 
-from tests.test_gpu_rotary import _freqs
+from tests.test_gpu_rotary import _check, _freqs, _want
 from tests.test_gpu_shared_prefix import _cuda, _setup
 
 pytestmark = pytest.mark.gpu
@@ -72,3 +72,47 @@ def test_function_transforms_are_refused(name, transform):
             torch.func.jvp(f, (x,), (torch.ones_like(x),))
         else:
             torch.func.vmap(f)(torch.stack((x, x)))
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotary_tangents(interleaved):
+    """A rotation is linear: the tangent is rotated like its tensor, and the gradient flows beside it."""
+    import torch.autograd.forward_ad as fw
+
+    import torch_neuronx_b200 as T
+
+    g = torch.Generator().manual_seed(5)
+    q, k, tq, tk = (torch.randn(2, h, 7, 32, generator=g) for h in (3, 2, 3, 2))
+    pos, freq, sections = torch.randint(0, 900, (2, 2, 7), generator=g), _freqs(24), (5, 7)
+    args = (pos.cuda(), freq.cuda())
+    kw = dict(sections=sections, interleaved=interleaved)
+    with fw.dual_level():
+        for which in ("both", "query", "key", "alone"):
+            dq = fw.make_dual(q.cuda(), tq.cuda()) if which != "key" else q.cuda()
+            dk = fw.make_dual(k.cuda(), tk.cuda()) if which in ("both", "key") else k.cuda()
+            y, z = T.rotary_embedding(dq, None if which == "alone" else dk, *args, **kw)
+            for got, x, t, has in ((y, q, tq, which != "key"), (z, k, tk, which in ("both", "key"))):
+                if got is None:
+                    assert which == "alone"
+                    continue
+                primal, tangent = fw.unpack_dual(got)
+                _check(primal.cpu(), _want(x, pos, freq, sections, interleaved))
+                assert (tangent is not None) == has
+                if has:
+                    _check(tangent.cpu(), _want(t, pos, freq, sections, interleaved))
+        leaf = q.cuda().requires_grad_()
+        y, _ = T.rotary_embedding(fw.make_dual(leaf * 1, tq.cuda()), None, *args, **kw)
+        (d,) = torch.autograd.grad(y, leaf, tq.cuda())
+        _check(d.cpu(), _want(tq, pos, freq, sections, interleaved, -1.0))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            T.rotary_embedding(q.cuda(), None, args[0], fw.make_dual(args[1], args[1]), **kw)
+
+
+def test_tangents_of_the_cache_operators_are_refused():
+    import torch.autograd.forward_ad as fw
+
+    for name, (f, x) in _calls().items():
+        if name in ("rotary", "read"):
+            continue
+        with fw.dual_level(), pytest.raises((NotImplementedError, RuntimeError)):
+            f(fw.make_dual(x, torch.ones_like(x)))

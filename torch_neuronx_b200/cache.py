@@ -129,7 +129,7 @@ def paged_write(
     if native is not None and layout in _LAYOUTS and native.paged_write(
             key, value, k_pages, v_pages, k_scales, v_scales, block_table, start, lens, _LAYOUTS[layout]):
         return
-    ops._check_visible("paged_write")
+    ops._check_visible("paged_write", key, value)
     if key.dim() != 4 or value.shape != key.shape:
         raise RuntimeError("paged_write: key and value must be 4-D (B, Hkv, L, D) and of the same shape")
     if key.dtype not in _HALF or value.dtype != key.dtype or value.device != key.device:
@@ -172,7 +172,7 @@ def paged_read(
         got = native.paged_read(k_pages, v_pages, k_scales, v_scales, block_table, kv_lens, max_len, dtype == torch.bfloat16, _LAYOUTS[layout])
         if got is not None:
             return got
-    ops._check_visible("paged_read")
+    ops._check_visible("paged_read", k_pages, v_pages)
     hd, rd = _dims(layout)
     if dtype not in _HALF:
         raise RuntimeError("paged_read: dtype must be float16 or bfloat16")
@@ -254,7 +254,7 @@ def _decode(op, query, k_pages, v_pages, k_scales, v_scales, block_table, kv_len
                                   _LAYOUTS[layout], out, lse, need_lse, kv_chunk)
         if got is not None:
             return got
-    ops._check_visible(op)
+    ops._check_visible(op, query, k_pages, v_pages)
     hd, rd = _dims(layout)
     if query.dim() != 4 or query.shape[2] != 1:
         raise RuntimeError(f"{op}: query must be (B, Hq, 1, D) and the page pools 4-D")

@@ -32,6 +32,7 @@ from typing import Optional
 
 import torch
 import torch.overrides
+from torch.autograd import forward_ad
 
 from . import _lib, masks
 
@@ -114,15 +115,18 @@ def release_workspaces() -> None:
     _retired_workspaces.clear()
 
 
-def _check_visible(op: str) -> None:
+def _check_visible(op: str, *tensors) -> None:
     """Raise where a call that goes to the library by pointers would be lost: a trace would record nothing of it but its
-    allocations, and a function transform hands out tensors without memory."""
+    allocations, a function transform hands out tensors without memory, and a forward-mode tangent would be dropped."""
     if torch.compiler.is_compiling():
         return   # (a call by pointers ends the compiled graph by itself)
     if torch.jit.is_tracing() or torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None:
         raise RuntimeError(f"{op}: a trace cannot record this call")
     if torch._C._functorch.maybe_current_level() is not None:
         raise RuntimeError(f"{op}: no function transform knows this call")
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{op}: there is no forward-mode derivative")
 
 
 def check_device_status(device=None) -> None:

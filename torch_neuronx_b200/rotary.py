@@ -11,6 +11,7 @@ import ctypes as C
 from typing import Optional, Sequence
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib, ops
 
@@ -33,19 +34,36 @@ def rotary_embedding(
     int32 or int64, ``(axes, B, L)``, or ``(B, L)`` or ``(L,)`` for one axis; extents of 1 are broadcast.  ``sections``
     says how many consecutive pairs belong to each axis (their sum is ``R / 2``).  Pair ``i`` is elements ``(i, i + R / 2)``, or
     ``(2 i, 2 i + 1)`` when ``interleaved``, and is turned by ``positions[axis of i] * inv_freq[i]``, an angle that is formed in
-    64 bits; the rest is computed in 32 and rounded once.  Gradients flow to ``query`` and ``key``; a trace cannot record
+    64 bits; the rest is computed in 32 and rounded once.  Gradients and forward-mode tangents flow to ``query`` and ``key``; a trace cannot record
     the call.  A backward pass
     captured into a CUDA graph is refused while an eager graph that was built on the default stream still holds one of its leaves."""
     if _lib.native is not None and not torch.compiler.is_compiling():
         got = _lib.native.rotary(query, key, positions, inv_freq, sections, interleaved)
         if got is not None:
             return got
-    ops._check_visible("rotary_embedding")
+    ops._check_visible("rotary_embedding", inv_freq)
     args = _check(query, key, positions, inv_freq, sections)
+    tangents = [None if x is None else forward_ad.unpack_dual(x).tangent for x in (query, key)]
+    if any(t is not None for t in tangents):
+        return _forward_mode(query, key, tangents, *args, interleaved)
     wants = torch.is_grad_enabled() and (query.requires_grad or (key is not None and key.requires_grad))
     if wants:
         return _Rotary.apply(query, key, *args, bool(interleaved), False)
     return _rotate(query, key, *args, bool(interleaved), False)
+
+
+def _forward_mode(query, key, tangents, positions, inv_freq, sections, interleaved):
+    """A rotation is linear: the tangents are rotated like the tensors that carry them."""
+    got = []
+    for x, t in zip((query, key), tangents):
+        if x is None:
+            got.append(None)
+            continue
+        y, _ = rotary_embedding(forward_ad.unpack_dual(x).primal, None, positions, inv_freq, sections=sections, interleaved=interleaved)
+        if t is not None:
+            y = forward_ad.make_dual(y, rotary_embedding(t, None, positions, inv_freq, sections=sections, interleaved=interleaved)[0])
+        got.append(y)
+    return tuple(got)
 
 
 def _check(query, key, positions, inv_freq, sections):
