@@ -116,3 +116,16 @@ def test_tangents_of_the_cache_operators_are_refused():
             continue
         with fw.dual_level(), pytest.raises((NotImplementedError, RuntimeError)):
             f(fw.make_dual(x, torch.ones_like(x)))
+
+
+def test_a_gradient_of_the_frequencies_is_refused():
+    import torch_neuronx_b200 as T
+
+    q, pos = torch.randn(1, 2, 5, 32, device="cuda"), torch.arange(5, device="cuda")
+    freq = torch.rand(16, device="cuda", requires_grad=True)
+    for x in (q, q.clone().requires_grad_()):
+        with pytest.raises(RuntimeError, match="inv_freq"):
+            T.rotary_embedding(x, None, pos, freq)
+        with torch.no_grad():
+            T.rotary_embedding(x, None, pos, freq)
+        T.rotary_embedding(x, None, pos, freq.detach())

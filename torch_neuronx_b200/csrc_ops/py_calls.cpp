@@ -496,7 +496,7 @@ PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const int64_t axes = positions.dim() == 3 ? positions.size(0) : 1, pd = positions.dim();
   if ((positions.size(pd - 1) != L && positions.size(pd - 1) != 1) || (pd > 1 && positions.size(pd - 2) != B && positions.size(pd - 2) != 1)) NOT_SERVED();
   if ((r.inv_freq.scalar_type() != at::kFloat && r.inv_freq.scalar_type() != at::kDouble) || r.inv_freq.dim() != 1 ||
-      r.inv_freq.device() != q.device() || !r.inv_freq.is_contiguous())
+      r.inv_freq.device() != q.device() || !r.inv_freq.is_contiguous() || (at::GradMode::is_enabled() && wants_grad(r.inv_freq)))
     NOT_SERVED();
   const int64_t pairs = r.inv_freq.size(0);
   if (pairs < 1 || 2 * pairs > D || axes < 1 || axes > 4) NOT_SERVED();

@@ -34,7 +34,7 @@ def rotary_embedding(
     int32 or int64, ``(axes, B, L)``, or ``(B, L)`` or ``(L,)`` for one axis; extents of 1 are broadcast.  ``sections``
     says how many consecutive pairs belong to each axis (their sum is ``R / 2``).  Pair ``i`` is elements ``(i, i + R / 2)``, or
     ``(2 i, 2 i + 1)`` when ``interleaved``, and is turned by ``positions[axis of i] * inv_freq[i]``, an angle that is formed in
-    64 bits; the rest is computed in 32 and rounded once.  Gradients and forward-mode tangents flow to ``query`` and ``key``; a trace cannot record
+    64 bits; the rest is computed in 32 and rounded once.  Gradients and forward-mode tangents flow to ``query`` and ``key``, none to ``inv_freq``; a trace cannot record
     the call.  A backward pass
     captured into a CUDA graph is refused while an eager graph that was built on the default stream still holds one of its leaves."""
     if _lib.native is not None and not torch.compiler.is_compiling():
@@ -86,6 +86,8 @@ def _check(query, key, positions, inv_freq, sections):
         raise RuntimeError(f"rotary_embedding: positions {tuple(positions.shape)} do not broadcast to ({axes}, {B}, {L})") from None
     if inv_freq.dtype not in (torch.float32, torch.float64) or inv_freq.dim() != 1 or inv_freq.device != query.device or not inv_freq.is_contiguous():
         raise RuntimeError("rotary_embedding: inv_freq must be a contiguous float32 or float64 vector on the query's device")
+    if inv_freq.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("rotary_embedding: no gradient flows to inv_freq, which requires one; detach it")
     pairs = inv_freq.shape[0]
     if pairs < 1 or 2 * pairs > D:
         raise RuntimeError(f"rotary_embedding: inv_freq has {pairs} frequencies, the head dim {D} has room for 1 to {D // 2}")
