@@ -326,7 +326,9 @@ def _decode(op, query, k_pages, v_pages, k_scales, v_scales, block_table, kv_len
     rc = lib.b200_sdpa_cache_decode_plan(C.byref(p), C.byref(plan))
     if rc != _lib.OK:
         raise RuntimeError(f"b200_sdpa_cache_decode_plan: {_lib.strerror(rc)}")
-    ws = ops._workspace(dev, int(plan.workspace_bytes))
+    # scratch of this call's own: the interpreter lock is not held while its launches are queued, and another thread's, on the same
+    # stream, may come between them.  The block goes back to the (stream-ordered) allocator when they have been.
+    ws = torch.empty(max(int(plan.workspace_bytes), 16), dtype=torch.uint8, device=query.device)
     p.workspace = ws.data_ptr()
     p.workspace_bytes = ws.numel()
     _launch("b200_sdpa_cache_decode", p)
