@@ -165,8 +165,8 @@ def paged_read(
 ):
     """The first ``max_len`` cached rows of each sequence as dense ``(B, Hkv, max_len, D)`` keys and values in fp16 or
     bf16 -- what :func:`ops.sdpa_forward` takes for the next chunk of a prompt.  Rows at or behind ``kv_lens[b]`` are zeros.
-    ``max_len`` is the table's capacity by default.  bf16 holds every cached value exactly; fp16 rounds those below ``2^-14`` and
-    overflows beyond 65504.  ``out`` is a pair of tensors to write into (any strides with a unit inner stride)."""
+    ``max_len`` is the table's capacity by default.  bf16 holds every cached value exactly but ``2^128``, to which the write rounds
+    bf16 magnitudes from ``248 * 2^120`` on and which is an infinity there; fp16 rounds those below ``2^-14`` and overflows beyond 65504.  ``out`` is a pair of tensors to write into (any strides with a unit inner stride)."""
     native = _native()
     if native is not None and layout in _LAYOUTS and out is None and dtype in _HALF:
         got = native.paged_read(k_pages, v_pages, k_scales, v_scales, block_table, kv_lens, max_len, dtype == torch.bfloat16, _LAYOUTS[layout])
@@ -229,7 +229,8 @@ def shared_prefix_decode(
     short prefix of few sequences is read for each of them, where that is faster), and sums are taken in another order.  As there,
     probabilities are rounded to the type of a 16-bit cache before they meet the values, and carried as two 16-bit parts for an 8-bit one.
     ``query`` is ``(B, Hq, 1, D)`` with D 64 or 128 and at most 128 query heads for a key head; the pools are in its dtype, or 8-bit with
-    ``k_scales`` and ``v_scales`` (for fp16 queries, cached values of an 8-bit prefix beyond 65504 may count as 65504).  ``prefix_len`` is a number of the host, part of a captured graph."""
+    ``k_scales`` and ``v_scales`` (cached values of an 8-bit prefix beyond the query type's largest number, 65504 or
+    ``255 * 2^120``, may count as that).  ``prefix_len`` is a number of the host, part of a captured graph."""
     if int(prefix_len) < 0:
         raise RuntimeError("shared_prefix_decode: prefix_len must not be negative")
     if prefix_table.dtype != torch.int32 or prefix_table.dim() != 1 or prefix_table.device != query.device:

@@ -4,7 +4,8 @@
 // (e8m0, one byte): the least e with amax <= 448 * 2^e, so the largest value uses the format's top binade.  A power of two
 // costs a float format nothing (only values 2^-15 below the row's largest lose bits they would keep under a finer scale)
 // and makes both directions exact where it matters: x * 2^-e is exact, so a value is rounded once, to e4m3; value * 2^e is
-// exact in bf16, so reading back rounds nothing (fp16: once, below 2^-14 and beyond 65504).  A row of zeros has e = 0; a
+// exact in bf16, so reading back rounds nothing but 2^128, which e4m3 makes of bf16's largest numbers (from 248 * 2^120 on) and
+// which reads as an infinity (fp16: once, below 2^-14, and beyond 65504 likewise).  A row of zeros has e = 0; a
 // row with a NaN or an infinity has the scale NaN (255) and reads as NaN; e is at least -127.
 //
 // Bound by HBM.  A row is D / 16 lanes with 16 elements each: 32 bytes on the 16-bit side, 16 on the other; writing, the maximum
@@ -130,9 +131,12 @@ __global__ void __launch_bounds__(kThreads) cache_write_kernel(const B200CacheRo
   }
 }
 
-// A gathered fp16 row holds nothing beyond 65504: e4m3 makes 65536 of what was at most 65504, half an fp16 step more, and an infinite
-// key or value would stand for a finite one.  NaN stays.
-__device__ __forceinline__ float within_f16(float x) { return fabsf(x) > 65504.f ? copysignf(65504.f, x) : x; }
+// A gathered row holds nothing beyond its type's largest number, 65504 or 255 * 2^120: e4m3 makes 65536 and 2^128 of it, half a step
+// more, and an infinite key or value would stand for a finite one.  NaN stays.
+template <bool BF16> __device__ __forceinline__ float within(float x) {
+  constexpr float kMost = BF16 ? 255.f * 0x1p120f : 65504.f;
+  return fabsf(x) > kMost ? copysignf(kMost, x) : x;
+}
 
 // LPR: lanes of a row, a power of two >= D / 16.  QUANT false: the pools hold the rows' own 16-bit type (strides in
 // elements).  Without lens every row is there.  GATHERED: rows for this library's own products.
@@ -172,7 +176,7 @@ __global__ void __launch_bounds__(kThreads) cache_read_kernel(const B200CacheRow
             float f[4];
             unpack_e4m3x4(in[i], f);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) f[j] = GATHERED && !BF16 ? within_f16(f[j] * scale) : f[j] * scale;
+            for (int j = 0; j < 4; ++j) f[j] = GATHERED ? within<BF16>(f[j] * scale) : f[j] * scale;
             out[2 * i] = pack16<BF16>(f[0], f[1]);
             out[2 * i + 1] = pack16<BF16>(f[2], f[3]);
           }
