@@ -51,7 +51,9 @@ typedef enum b200_sdpa_status {
   B200_SDPA_ERR_TOO_LARGE = 11,   /* exceeds a fixed-capacity entry point's limit   */
   B200_SDPA_ERR_CACHE_FULL = 12,  /* (status word only) decode with append met a
                                      sequence whose cache is full: its new row was
-                                     not stored and not attended to; [1] = batch    */
+                                     not stored and not attended to, or a row was
+                                     written behind the table's last page: it was
+                                     dropped; [1] = batch                           */
   B200_SDPA_ERR_BOUNDS = 13,      /* (status word only, checked build of the library)
                                      an index left its tensor, a scratch slot its
                                      buffer or a tensor-memory access its columns;
@@ -59,8 +61,11 @@ typedef enum b200_sdpa_status {
                                      [3] = limit                                    */
   B200_SDPA_ERR_PAGE = 14         /* (status word only) a block table names a page
                                      outside the pool, or a position lies before the
-                                     table: nothing was read or written there;
-                                     [1] = sequence, [2] = position, [3] = pages    */
+                                     table.  Nothing was written there; rows read back
+                                     are zeros; attention took page 0 instead.
+                                     [1] = sequence (-1: the shared prefix), [2] =
+                                     position (of the row when writing, of the page's
+                                     first row when reading), [3] = pages of the pool */
 } b200_sdpa_status;
 
 typedef enum b200_sdpa_dtype {

@@ -11,7 +11,8 @@
 // Bound by HBM.  A row is D / 16 lanes with 16 elements each: 32 bytes on the 16-bit side, 16 on the other; writing, the maximum
 // meets over those lanes.  8 heads of 128, bf16: 16 prompts of 512..4096 tokens written in 41 us (5.8 TB/s), 8 sequences of
 // 4096..8192 rows read in 66 us (5.7 TB/s).
-// A page number outside the pool is reported through the status word and nothing is read or written there.
+// A page number outside the pool is reported through the status word, and nothing is read or written there: such rows read as zeros.
+// (Gathered rows are page 0's, as in the kernels that read the pages themselves.)
 #include "common.cuh"
 #include "debug.cuh"
 #include "fp8.cuh"
@@ -160,9 +161,15 @@ __global__ void __launch_bounds__(kThreads) cache_read_kernel(const B200CacheRow
     uint16_t* x = static_cast<uint16_t*>(const_cast<void*>(is_v ? p.v : p.k)) + b * xs[0] + h * xs[1] + (i0 + t) * xs[2] + c0;
     __align__(16) uint32_t out[8] = {};
     if (i0 + t < n) {
-      int64_t page;
-      int row;
-      if (locate(p, page_shift, b, i0 + t, &page, &row)) {
+      int64_t page = 0;
+      int row = 0;
+      bool there = locate(p, page_shift, b, i0 + t, &page, &row);
+      if (!there) {
+        report_page(p.status, B200_SDPA_ERR_PAGE, GATHERED ? kSharedPrefix : b, (i0 + t) >> page_shift << page_shift, p.n_pages);
+        page = 0;
+        there = GATHERED;
+      }
+      if (there) {
         const int64_t* ps = is_v ? p.v_pages_stride : p.k_pages_stride;
         const int64_t at = page * ps[0] + h * ps[1] + row * ps[2] + c0;
         const void* pool = is_v ? p.v_pages : p.k_pages;
@@ -184,8 +191,6 @@ __global__ void __launch_bounds__(kThreads) cache_read_kernel(const B200CacheRow
           *reinterpret_cast<uint4*>(out) = ld_stream_16B(static_cast<const uint16_t*>(pool) + at);
           *reinterpret_cast<uint4*>(out + 4) = ld_stream_16B(static_cast<const uint16_t*>(pool) + at + 8);
         }
-      } else {
-        report_page(p.status, B200_SDPA_ERR_PAGE, b, i0 + t, p.n_pages);
       }
     }
     if (rows_16b) {

@@ -158,6 +158,7 @@ struct List {
   __device__ __forceinline__ int count() const { return p.B << twice; }
   __device__ __forceinline__ int keys(int e) const { return twice && (e & 1) == 0 ? front.len : valid_keys(p, e >> twice); }
   __device__ __forceinline__ int blocks(int e) const { return (keys(e) + kBlockKeys - 1) / kBlockKeys; }
+  __device__ __forceinline__ int sequence(int e) const { return twice && (e & 1) == 0 ? kSharedPrefix : e >> twice; }   // as it is reported
   __device__ __forceinline__ const int* table(int e) const {
     return twice && (e & 1) == 0 ? front.table : p.block_table + static_cast<int64_t>(e >> twice) * p.table_stride;
   }
@@ -236,7 +237,7 @@ __device__ __forceinline__ int entry_of(const List& l, const Cursor& c, int row)
 __device__ __forceinline__ int page_of(const List& l, const CacheScales& sc, const Cursor& c, int entry, int row) {
   if (row >= c.n_keys) return -1;
   if (static_cast<unsigned>(entry) < static_cast<unsigned>(sc.n_pages)) return entry;
-  report_page(l.p.status, B200_SDPA_ERR_PAGE, c.b >> l.twice, row, sc.n_pages);
+  report_page(l.p.status, B200_SDPA_ERR_PAGE, l.sequence(c.b), row >> l.p.page_shift << l.p.page_shift, sc.n_pages);
   return 0;
 }
 
@@ -393,7 +394,7 @@ __device__ __forceinline__ void bring_scales(const List& l, const CacheScales& s
 #pragma unroll
       for (int i = 0; i < kLook; ++i)
         if (static_cast<unsigned>(e[i]) >= static_cast<unsigned>(sc.n_pages)) {
-          report_page(p.status, B200_SDPA_ERR_PAGE, b >> l.twice, c.blk * kBlockKeys + lane + 32 * i, sc.n_pages);
+          report_page(p.status, B200_SDPA_ERR_PAGE, l.sequence(b), (c.blk * kBlockKeys + lane + 32 * i) & ~page_mask, sc.n_pages);
           e[i] = 0;
         }
     }

@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(kThreads, 3) decode_mma_kernel(const Problem p
       if (PAGED) {
         int64_t page = pages[i];
         if (BESIDE && static_cast<unsigned>(pages[i]) >= static_cast<unsigned>(p.n_pages)) {   // reported, and page 0 read in its place
-          report_page(p.status, B200_SDPA_ERR_PAGE, b, srow, p.n_pages);
+          report_page(p.status, B200_SDPA_ERR_PAGE, shared ? kSharedPrefix : b, srow & ~page_mask, p.n_pages);
           page = 0;
         }
         const int in_page = srow & page_mask;

@@ -324,7 +324,7 @@ prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
           const int key = (key_tile0 + item_tile(item)) * kBlockN + lane * rows;
           const bool mine = lane * rows < kBlockN && key < kv_limit;
           if (mine && static_cast<unsigned>(entry) >= static_cast<unsigned>(pack.n_pages)) {   // reported, and page 0 read in its place
-            report_page(p.status, B200_SDPA_ERR_PAGE, -1, key, pack.n_pages);
+            report_page(p.status, B200_SDPA_ERR_PAGE, kSharedPrefix, key & ~(page - 1), pack.n_pages);
             entry = 0;
           }
           const unsigned copies = __popc(__ballot_sync(0xffffffffu, mine));
