@@ -176,14 +176,20 @@ __global__ void __launch_bounds__(kThreads) cache_read_kernel(const B200CacheRow
         if constexpr (QUANT) {
           const int64_t* ss = is_v ? p.v_scales_stride : p.k_scales_stride;
           const uint4 w = ld_stream_16B(static_cast<const uint8_t*>(pool) + at);
-          const float scale = scale_value(static_cast<const uint8_t*>(is_v ? p.v_scales : p.k_scales)[page * ss[0] + h * ss[1] + row * ss[2]]);
+          const int code = static_cast<const uint8_t*>(is_v ? p.v_scales : p.k_scales)[page * ss[0] + h * ss[1] + row * ss[2]];
+          const float scale = scale_value(code);
+          const bool beyond = GATHERED && code > (BF16 ? 246 : 134);   // (448 times the scale is more than the type's largest)
           const uint32_t in[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             float f[4];
             unpack_e4m3x4(in[i], f);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) f[j] = GATHERED ? within<BF16>(f[j] * scale) : f[j] * scale;
+            for (int j = 0; j < 4; ++j) f[j] *= scale;
+            if (beyond) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) f[j] = within<BF16>(f[j]);
+            }
             out[2 * i] = pack16<BF16>(f[0], f[1]);
             out[2 * i + 1] = pack16<BF16>(f[2], f[3]);
           }
