@@ -415,11 +415,14 @@ std::array<at::Tensor, 2> rotate(const at::Tensor& query, const at::Tensor& key,
 
 // Inside a stream capture a gradient cannot flow to a leaf whose accumulation node was made on the default stream, by an
 // eager graph that is still alive: the engine would have the default stream wait for the capture, which ends the capture.
-// This runs before that wait, so that the capture itself is still whole when the error reaches its caller.
+// This runs before that wait, so that the capture itself is still whole when the error reaches its caller.  (A leaf that the pass
+// reaches with an undefined gradient is waited for too, one that it leaves out is not.)
 void check_leaf_streams() {
   const auto node = torch::autograd::get_current_node();
   if (node == nullptr) return;
-  for (const auto& edge : node->next_edges()) {
+  for (uint32_t i = 0; i < node->num_outputs(); ++i) {
+    const auto& edge = node->next_edge(i);
+    if (!edge.is_valid() || !node->task_should_compute_output(i)) continue;
     if (dynamic_cast<torch::autograd::AccumulateGrad*>(edge.function.get()) == nullptr) continue;
     const auto made_on = edge.function->stream();
     if (!made_on.has_value() || made_on->device_type() != c10::kCUDA) continue;
