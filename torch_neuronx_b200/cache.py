@@ -136,6 +136,8 @@ def paged_write(
         raise RuntimeError("paged_write: key and value must share a float16 or bfloat16 dtype and a device")
     if key.shape[3] % 16 or not 16 <= key.shape[3] <= 256 or (key.numel() and (key.stride(3) != 1 or value.stride(3) != 1)):
         raise RuntimeError("paged_write: the head dim must be a multiple of 16 up to 256 with a unit inner stride")
+    if max(key.shape) > ops._MOST:
+        raise RuntimeError("paged_write: extents are counted in 32 bits")
     B = key.shape[0]
     block_table = _check_table("paged_write", block_table, B, key.device)
     start = _check_vector("paged_write", "start", start, B, key.device)

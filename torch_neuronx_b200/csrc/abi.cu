@@ -305,6 +305,8 @@ int choose_bwd(const B200SdpaBwdParams* a, const BwdProblem& bp, int* path) {
 bool half_dtype(int dtype) { return dtype == B200_SDPA_F16 || dtype == B200_SDPA_BF16; }
 bool page_size_ok(int n) { return n >= 1 && (n & (n - 1)) == 0; }
 
+constexpr int kMostRows = 0x7ffffe00;   // (rows are counted in 32 bits, up to a CTA's share beyond the last)
+
 int validate_rotary(const B200RotaryParams* a) {
   if (a == nullptr) return B200_SDPA_ERR_NULL;
   if (a->struct_size != sizeof(B200RotaryParams)) return B200_SDPA_ERR_STRUCT;
@@ -319,7 +321,7 @@ int validate_rotary(const B200RotaryParams* a) {
   }
   if (pairs != a->rot / 2) return B200_SDPA_ERR_SHAPE;
   // the grid's second dimension, and the shared-memory table of four tokens
-  if (a->B > 65535 || a->rot > 1024 || static_cast<int64_t>(a->heads[0]) + a->heads[1] > (1 << 16)) return B200_SDPA_ERR_UNSUPPORTED;
+  if (a->B > 65535 || a->rot > 1024 || static_cast<int64_t>(a->heads[0]) + a->heads[1] > (1 << 16) || a->L > kMostRows) return B200_SDPA_ERR_UNSUPPORTED;
   for (int w = 0; w < 2; ++w)
     if (a->heads[w] > 0 && (a->x[w] == nullptr || a->y[w] == nullptr)) return B200_SDPA_ERR_NULL;
   if (a->positions == nullptr || a->inv_freq == nullptr) return B200_SDPA_ERR_NULL;
@@ -340,7 +342,7 @@ int validate_rows(const B200CacheRowsParams* a) {
   if (!half_dtype(a->dtype)) return B200_SDPA_ERR_DTYPE;
   if (a->B <= 0 || a->Hkv <= 0 || a->L <= 0 || a->D <= 0 || a->n_pages <= 0) return B200_SDPA_ERR_SHAPE;
   if (!page_size_ok(a->page_size) || a->block_table_stride < 1) return B200_SDPA_ERR_SHAPE;
-  if (a->D % 16 != 0 || a->D > 256 || a->B > 65535 || a->Hkv > (1 << 16)) return B200_SDPA_ERR_UNSUPPORTED;
+  if (a->D % 16 != 0 || a->D > 256 || a->B > 65535 || a->Hkv > (1 << 16) || a->L > kMostRows) return B200_SDPA_ERR_UNSUPPORTED;
   if (static_cast<int64_t>(a->block_table_stride) * a->page_size >= (1 << 30)) return B200_SDPA_ERR_UNSUPPORTED;
   if (a->k == nullptr || a->v == nullptr || a->k_pages == nullptr || a->v_pages == nullptr || a->k_scales == nullptr ||
       a->v_scales == nullptr || a->block_table == nullptr)

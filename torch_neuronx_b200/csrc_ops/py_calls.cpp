@@ -367,6 +367,13 @@ PyObject* py_decode(PyObject*, PyObject* const* args, Py_ssize_t n) {
 // Rotary embedding
 // ---------------------------------------------------------------------------------------------------------------------
 
+// The extents are counted in 32 bits (a broadcast dimension can have more without the memory for it).
+bool in_32_bits(const at::Tensor& t) {
+  for (int64_t n : t.sizes())
+    if (n > 0x7fffffff) return false;
+  return true;
+}
+
 struct RotaryRest {
   at::Tensor positions, inv_freq;   // (axes, B, L), (B, L) or (L,), extents of 1 broadcast
   std::vector<int64_t> sections;
@@ -488,10 +495,10 @@ PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const at::Tensor& q = THPVariable_Unpack(args[0]);
   const at::Tensor& positions = THPVariable_Unpack(args[2]);
   r.inv_freq = THPVariable_Unpack(args[3]);
-  if (q.dim() != 4 || q.numel() == 0 || dtype_code(q.scalar_type()) < 0) NOT_SERVED();
+  if (q.dim() != 4 || q.numel() == 0 || dtype_code(q.scalar_type()) < 0 || !in_32_bits(q)) NOT_SERVED();
   const int64_t B = q.size(0), L = q.size(2), D = q.size(3);
   if (key.defined() && (key.dim() != 4 || key.numel() == 0 || key.scalar_type() != q.scalar_type() || key.device() != q.device() ||
-                        key.size(0) != B || key.size(2) != L || key.size(3) != D))
+                        key.size(0) != B || key.size(2) != L || key.size(3) != D || !in_32_bits(key)))
     NOT_SERVED();
   if ((positions.scalar_type() != at::kInt && positions.scalar_type() != at::kLong) || positions.device() != q.device() ||
       positions.dim() < 1 || positions.dim() > 3)
@@ -608,7 +615,7 @@ PyObject* py_paged_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const at::Tensor& start = THPVariable_Unpack(args[7]);
   const int hd = layout == 1 ? 2 : 1, rd = layout == 1 ? 1 : 2;
   const auto dt = key.scalar_type();
-  if (key.dim() != 4 || key.numel() == 0 || value.sizes() != key.sizes() || (dt != at::kHalf && dt != at::kBFloat16) ||
+  if (key.dim() != 4 || key.numel() == 0 || !in_32_bits(key) || value.sizes() != key.sizes() || (dt != at::kHalf && dt != at::kBFloat16) ||
       value.scalar_type() != dt || value.device() != key.device() || key.stride(3) != 1 || value.stride(3) != 1 || key.size(3) % 16 != 0 ||
       key.size(3) > 256)
     NOT_SERVED();

@@ -42,6 +42,7 @@ _DTYPE_CODE = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16:
 # per-device scratch and status words
 # ----------------------------------------------------------------------------
 
+_MOST = 0x7FFFFFFF   # extents are counted in 32 bits
 _status_words: dict[int, torch.Tensor] = {}
 _zero_scalars: dict[int, tuple] = {}
 _workspaces: dict[tuple[int, int], torch.Tensor] = {}

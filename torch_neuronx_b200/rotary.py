@@ -77,6 +77,8 @@ def _check(query, key, positions, inv_freq, sections):
     B, _, L, D = query.shape
     if key is not None and (key.dtype != query.dtype or key.device != query.device or key.shape[0] != B or key.shape[2:] != query.shape[2:]):
         raise RuntimeError("rotary_embedding: key must share the query's batch, length, head dim, dtype and device")
+    if max(query.shape) > ops._MOST or (key is not None and key.shape[1] > ops._MOST):
+        raise RuntimeError("rotary_embedding: extents are counted in 32 bits")
     if positions.dtype not in (torch.int32, torch.int64) or positions.device != query.device or not 1 <= positions.dim() <= 3:
         raise RuntimeError("rotary_embedding: positions must be an int32 or int64 tensor (axes, B, L), (B, L) or (L,) on the query's device")
     axes = positions.shape[0] if positions.dim() == 3 else 1
