@@ -1,4 +1,4 @@
-"""A captured backward pass of the rotary embedding is refused for the leaves that it reaches, and for no others."""
+"""The direct route of the rotary embedding: which captured backward passes it refuses, and what it takes as sections."""
 
 import contextlib
 import gc
@@ -47,3 +47,16 @@ def test_a_leaf_that_is_not_reached_may_be_held(direct):
     assert alive[0].grad_fn is not None
     del alive
     gc.collect()
+
+
+def test_sections_of_a_list_take_the_direct_route():
+    """A model's configuration holds a list."""
+    from torch_neuronx_b200 import _lib
+
+    if _lib.native is None:
+        pytest.skip("there is no direct route")
+    q, pos, freq = torch.randn(1, 2, 5, 64, device="cuda"), torch.arange(15, device="cuda").view(3, 1, 5), _freqs(64).cuda()
+    with torch._C.DisableTorchFunction():
+        got = [_lib.native.rotary(q, None, pos, freq, s, False) for s in ((8, 12, 12), [8, 12, 12])]
+        assert got[1] is not None and torch.equal(got[0][0], got[1][0])
+        assert _lib.native.rotary(q, None, pos, freq, [8, 12, "12"], False) is None and _lib.native.rotary(q, None, pos, freq, [8, 24], False) is None

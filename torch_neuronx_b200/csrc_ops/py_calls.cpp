@@ -490,7 +490,7 @@ PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
   at::Tensor key;
   RotaryRest r;
   if (n != 6 || !plain(args[0]) || !optional_plain(args[1], &key) || !plain(args[2]) || !plain(args[3]) ||
-      (args[4] != Py_None && !PyTuple_CheckExact(args[4])) || !as_bool(args[5], &r.interleaved) || !no_modes())
+      (args[4] != Py_None && !PyTuple_CheckExact(args[4]) && !PyList_CheckExact(args[4])) || !as_bool(args[5], &r.interleaved) || !no_modes())
     NOT_SERVED();
   const at::Tensor& q = THPVariable_Unpack(args[0]);
   const at::Tensor& positions = THPVariable_Unpack(args[2]);
@@ -515,10 +515,10 @@ PyObject* py_rotary(PyObject*, PyObject* const* args, Py_ssize_t n) {
     r.sections = {pairs};
   } else {
     int64_t sum = 0;
-    if (PyTuple_GET_SIZE(args[4]) != axes) NOT_SERVED();
+    if (PySequence_Fast_GET_SIZE(args[4]) != axes) NOT_SERVED();
     for (int64_t i = 0; i < axes; ++i) {
       int64_t v = 0;
-      if (!as_int(PyTuple_GET_ITEM(args[4], i), &v) || v < 0 || v > pairs) NOT_SERVED();
+      if (!as_int(PySequence_Fast_GET_ITEM(args[4], i), &v) || v < 0 || v > pairs) NOT_SERVED();
       r.sections.push_back(v);
       sum += v;
     }
