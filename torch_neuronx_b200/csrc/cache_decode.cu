@@ -3,12 +3,13 @@
 // With a shared prefix of P keys the softmax runs over P + kv_lens[b] keys, but only the sequence's own keys differ:
 //   * prefix: the batch's query rows are the rows of one attention problem (B * group rows for each kv head against P
 //     keys, no mask), so its keys are read once for all of them and multiplied by full tensor-core tiles -- the split form
-//     of the prefill kernel (prefill_sm100.cu), whose fp32 partials stay in the scratch;
+//     of the prefill kernel (prefill_sm100.cu), whose fp32 partials stay in the scratch; probabilities enter its second product as the
+//     own keys' do, rounded to the type of a 16-bit cache, as two 16-bit parts for an 8-bit one;
 //   * own keys: split-KV decode (decode_mma.cu, decode_fp8.cu), partials beside them;
 //   * one merge over both lists, exact in the usual way: o = sum 2^(m_i - m) o_i / sum 2^(m_i - m) l_i.
 // Bound by HBM: (P + sum of own lengths) Hkv rows once; the prefix's products by the tensor cores from about 60 sequences
 // on (32 / 8 heads).  64 sequences under 16384 + 16..1000 keys: 67 us (bytes and products: 31), of which the prefix's tiles 15, their
-// start and end 9.  128 sequences under 8192 + 16..500 keys of an 8-bit cache: 68 us.
+// start and end 9.  128 sequences under 8192 + 16..500 keys of an 8-bit cache: 76 us.
 #include "common.cuh"
 #include "debug.cuh"
 
@@ -278,10 +279,11 @@ namespace {
 // L2 all but once.
 // 8-bit: once for all costs two more launches (gathered rows, then tiles of 128 query rows whether there are as many or not).  Both in
 // us, fitted to 1 to 128 sequences under 300 to 11008 keys (each against once, with up to 100 own keys): 1 sequence, 8192 keys, 8 kv
-// heads of 128: 16.4 against 27.7; 5, 3708, 4: 15.8 against 20.5; 8, 4096, 8: 26.7 against 25.9; 16, 2048, 8: 26.9 against 23.0;
-// 128, 2048, 8: 105 against 38; 64, 4096, 2 heads of 64: 28.1 against 20.6.
-// 16-bit: one more launch, and the own keys run beside it; so for each only while its elements, for all sequences, are few.  With up to
-// 100 own keys: 1, 300, 2: 6.9 against 11.0; 5, 1000, 4 heads of 64: 8.2 against 10.3; 2, 2048, 8: 11.0 against 12.3; 4, 2048, 8: 13.7
+// heads of 128: 16.4 against 29.9; 5, 3708, 4: 16.4 against 21.9; 8, 4096, 8: 28.0 against 27.4; 16, 2048, 8: 28.2 against 24.5;
+// 128, 2048, 8: 110 against 40; 64, 4096, 2 heads of 64: 29.4 against 21.3.
+// 16-bit: one more launch, and the own keys run beside it; so for each only while the elements that its grid covers, prefix and room of
+// the table, for all sequences, are few.  (The lengths are the device's to know: a table far wider than its sequences takes the other
+// form sooner than it need.)  With up to 100 own keys in a table of 128: 1, 300, 2: 6.9 against 11.0; 5, 1000, 4 heads of 64: 8.2 against 10.3; 2, 2048, 8: 11.0 against 12.3; 4, 2048, 8: 13.7
 // against 12.6; 8, 1024, 8: 13.7 against 13.0; 16, 2048, 8: 27.7 against 14.6.
 bool in_front(const B200CacheDecodeParams& a) {
   const Problem f = prefix_problem(a, nullptr, nullptr);

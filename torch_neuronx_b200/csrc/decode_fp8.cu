@@ -27,8 +27,8 @@
 // keys, as decode_mma.cu has them, the address arithmetic and the latency of table and scales stood in the way: 64 x 512..8192
 // keys, 32/8 heads of 128, 194 us.)
 // Softmax in the exp2 domain, statistics fp32, the running maximum raised lazily (2^6).
-// Bound by HBM in steady state (2450 cycles for 128 keys in each of the two CTAs of an SM, 6.7 TB/s).  With the merge: 64 x 512..8192 keys,
-// 32/8 heads of 128: 118 us, 4.9 TB/s; 16 x 128..4000 keys, 12 heads of 64: 22 us; one sequence of 2001 keys: 11 us.
+// Bound by HBM once the ring is full (2450 cycles for 128 keys in each of the two CTAs of an SM).  With the merge: 64 x 512..8192 keys,
+// 32/8 heads of 128: 119 us, 4.9 TB/s; 16 x 128..4000 keys, 12 heads of 64: 24 us; one sequence of 2001 keys: 11 us.
 #include "debug.cuh"
 #include "fp8.cuh"
 #include "tc_common.cuh"

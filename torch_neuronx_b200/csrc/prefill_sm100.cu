@@ -134,7 +134,8 @@ struct PackArgs {
 // probabilities on the CUDA-core kernel, so P goes into the second product as hi + lo (remainder2), lo in the second
 // half of the columns of S.
 // LO: P goes in as hi + lo for a full head dimension too -- a prefix of an 8-bit cache, whose other form (decode_fp8.cu) carries 22
-// bits of P.  At D = 64 P then lies over S, as at D = 128, since tensor memory has no other columns for lo.
+// bits of P.  At D = 64 P then lies over S, as at D = 128, since tensor memory has no other columns for lo.  (128 sequences of 32 heads
+// under 8192 keys, 8 x 128: 33 us, 28 without.)
 template <int D, bool BF16, bool BIAS, bool ACC, bool PAD, bool PACK, bool PAGED = false, bool LO = PAD>
 __global__ void __launch_bounds__(kThreads, 1)
 prefill_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
