@@ -21,7 +21,8 @@
 //     the softmax's scale: maxima are kept in log2 units, which no ordinary score leaves.  Keys from 2^95 on are multiplied in another order.
 //   * values: o += (p 2^(e_v - r + 9)) v8 with r the largest e_v the warp has met (o is rescaled when it grows), so the
 //     probability stays inside fp16; it enters as hi + lo, two fp16 operands: 22 bits, and never coarser than 2^-34 of
-//     the largest value row the warp has met.
+//     the largest value row the warp has met.  That row may have no weight at all, so a warp's keys with a row 2^10 below it are
+//     multiplied in bf16, hi + lo: 16 bits at any size.
 // One warp brings the rows into a ring of blocks by tensor copies, one for each page and operand, and another the scales; four
 // warps compute, 32 keys of a block each, and wait for nothing but their block.  (With plain copies and one barrier a block of 64
 // keys, as decode_mma.cu has them, the address arithmetic and the latency of table and scales stood in the way: 64 x 512..8192
@@ -32,8 +33,6 @@
 #include "debug.cuh"
 #include "fp8.cuh"
 #include "tc_common.cuh"
-
-#include <type_traits>
 
 namespace b200 {
 
@@ -48,6 +47,8 @@ constexpr int kBlockKeys = 128;
 constexpr int kWarpKeys = kBlockKeys / kWarps;
 constexpr float kRescaleThreshold = 6.0f;
 constexpr float kProbShift = 9.0f;   // p <= 2^6, p 2^9 <= 2^15 in fp16
+constexpr float kDeep = 10.0f;       // a row this many binades below the largest has its block multiplied in bf16 ...
+constexpr float kDeepShift = 110.0f; // ... with probabilities of up to 2^125
 
 // A block of the ring: its rows of K, then of V, swizzled in 16-byte pieces as a tensor copy leaves them (128-byte pattern for
 // D = 128, 64-byte for D = 64), so that ldmatrix meets no bank twice.
@@ -121,15 +122,12 @@ __device__ __forceinline__ void mma_16(float (&d)[4], uint32_t a0, uint32_t a1, 
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// Four e4m3 values as two pairs: in fp16 the first two and the others, in bf16 the even and the odd ones, times 2^-120 (sign, exponent and
-// mantissa in their places; subnormal numbers stay what they are).
-template <bool BF16> __device__ __forceinline__ void unpack_key(uint32_t w, uint32_t& a, uint32_t& b) {
-  if (BF16) {
-    a = (w << 8 & 0x80008000u) | (w << 4 & 0x07f007f0u);
-    b = (w & 0x80008000u) | (w >> 4 & 0x07f007f0u);
-  } else {
-    unpack_e4m3_f16(w, a, b);
-  }
+// Four e4m3 values as two bf16 pairs, the even and the odd ones, times 2^-120: sign, exponent and mantissa in their places; subnormal
+// numbers and NaN stay what they are.
+__device__ __forceinline__ void unpack_e4m3_bf16(uint32_t w, uint32_t& even, uint32_t& odd) {
+  const uint32_t x = w << 4 & 0x07f007f0u, y = w >> 4 & 0x07f007f0u;
+  even = (w << 8 & 0x80008000u) | x | __vcmpeq2(x, 0x07f007f0u);
+  odd = (w & 0x80008000u) | y | __vcmpeq2(y, 0x07f007f0u);
 }
 // The power of two that brings a query row, whose largest element has the bits `top`, into [2^want, 2^(want + 1)), up to 2^126.
 template <bool BF16> __device__ __forceinline__ int power_up(uint32_t top, int want) {
@@ -137,11 +135,11 @@ template <bool BF16> __device__ __forceinline__ int power_up(uint32_t top, int w
   if (!BF16 && up < 0) up = 0;
   return up > 126 ? 126 : up;   // (-113 and more)
 }
-// (lo, hi) as an fp16 pair, and what the rounding left over as another.
-__device__ __forceinline__ void split_f16(float lo, float hi, uint32_t& head, uint32_t& rest) {
-  head = pack16<false>(lo, hi);
-  const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&head));
-  rest = pack16<false>(lo - h.x, hi - h.y);
+// (lo, hi) as a 16-bit pair, and what the rounding left over as another.
+template <bool BF16> __device__ __forceinline__ void split_16(float lo, float hi, uint32_t& head, uint32_t& rest) {
+  head = pack16<BF16>(lo, hi);
+  const float h0 = half_to_f32<BF16>(static_cast<uint16_t>(head)), h1 = half_to_f32<BF16>(static_cast<uint16_t>(head >> 16));
+  rest = pack16<BF16>(lo - h0, hi - h1);
 }
 // The transpose of an 8 x 8 matrix of 16-bit elements: lane 4 i + j holds elements 2 j, 2 j + 1 of row i.
 __device__ __forceinline__ uint32_t turn8x8(uint32_t x) {
@@ -437,6 +435,109 @@ __device__ __forceinline__ void land(Sync<D, HEADS>* sync, int warp, int lane) {
   for (int s = 0; s < kStages && s < most; ++s) wait_drain(smem_u32(&sync->full[s]), ((most - 1 - s) / kStages) & 1);
 }
 
+// What fp16 has no room for goes through functions of their own, which take their operands through memory, so that the usual path keeps
+// its registers and its place in the instruction caches (inlined, 128 sequences under a prefix took 80 us instead of 76).
+//
+// Query rows that fp16 does not hold exactly, in bf16: factor[i] is what goes back out of head 8 i + g's scores.
+template <int D, int NB> struct Wide {
+  uint2 q[NB][D / 16];
+  float factor[NB], score[2][NB][4];
+};
+template <int D, int NB> __device__ __noinline__ void wide_query(Wide<D, NB>& d, const uint16_t* query, int g, int tq) {
+#pragma unroll 1
+  for (int i = 0; i < NB; ++i) {
+    const uint16_t* row = query + (8 * i + g) * (D + 16);
+    uint32_t top = 0;
+#pragma unroll 1
+    for (int e = 0; e < D; ++e) top = max(top, row[e] & 0x7fffu);
+    const int up = power_up<true>(top << 16, 126);
+    const float f = __int_as_float((127 + up) << 23);
+    d.factor[i] = __int_as_float((127 - up) << 23) * 0x1p120f;
+#pragma unroll 1
+    for (int s = 0; s < D / 16; ++s) {
+      const uint2 v = *reinterpret_cast<const uint2*>(row + 16 * s + 4 * tq);
+      const uint32_t x = pack16<true>(half_to_f32<true>(static_cast<uint16_t>(v.x)) * f, half_to_f32<true>(static_cast<uint16_t>(v.x >> 16)) * f);
+      const uint32_t y = pack16<true>(half_to_f32<true>(static_cast<uint16_t>(v.y)) * f, half_to_f32<true>(static_cast<uint16_t>(v.y >> 16)) * f);
+      d.q[i][s] = make_uint2(__byte_perm(x, y, 0x5410), __byte_perm(x, y, 0x7632));   // (as unpack_e4m3_bf16 has the key's)
+    }
+  }
+}
+// Their products with a warp's keys.
+template <int D, int NB> __device__ __noinline__ void wide_scores(Wide<D, NB>& d, uint32_t k_row, int lane) {
+  float score[2][NB][4] = {};
+#pragma unroll 1
+  for (int s = 0; s < D / 16; s += 2) {
+    const uint32_t at = k_row + static_cast<uint32_t>(((s + (lane >> 4)) ^ Geo<D, 8>::swizzle(lane & 7)) << 4);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      uint32_t kf[4];
+      ldsm_x4(at + t * 16 * D, kf);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        uint32_t a0, a1, a2, a3;
+        unpack_e4m3_bf16(kf[2 * u], a0, a2);
+        unpack_e4m3_bf16(kf[2 * u + 1], a1, a3);
+#pragma unroll
+        for (int i = 0; i < NB; ++i) mma_16<true>(score[t][i], a0, a1, a2, a3, d.q[i][s + u].x, d.q[i][s + u].y);
+      }
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) d.score[t][i][r] = score[t][i][r];
+}
+// A warp's products with its values where a row lies far below the largest.
+template <int D, int NB> struct Deep {
+  float o[D / 16][NB][4], sv[2][NB][4], nm[NB][2], lsum[NB][2];
+  float w[2][2];   // 2^(e_v - r + 119)
+};
+template <int D, int NB> __device__ __noinline__ void deep_products(Deep<D, NB>& d, uint32_t v_row, int lane) {
+  uint32_t ph[2][NB][2], pl[2][NB][2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      float x[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        x[r] = ex2(d.sv[t][i][r] + d.nm[i][r & 1]);
+        d.lsum[i][r & 1] += x[r];
+      }
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        split_16<true>(x[2 * y] * d.w[t][y], x[2 * y + 1] * d.w[t][y], ph[t][i][y], pl[t][i][y]);
+        ph[t][i][y] = turn8x8(ph[t][i][y]);
+        pl[t][i][y] = turn8x8(pl[t][i][y]);
+      }
+    }
+#pragma unroll 1
+  for (int j = 0; j < D / 16; j += 2) {
+    const uint32_t at = v_row + static_cast<uint32_t>(((j + (lane >> 4)) ^ Geo<D, 8>::swizzle(lane & 7)) << 4);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      uint32_t vf[4];
+      ldsm_x4_trans(at + t * 16 * D, vf);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        uint32_t a0, a1, a2, a3;
+        unpack_e4m3_bf16(vf[2 * u], a0, a1);
+        unpack_e4m3_bf16(vf[2 * u + 1], a2, a3);
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+          float part[4] = {0.f, 0.f, 0.f, 0.f};
+          mma_16<true>(part, a0, a1, a2, a3, pl[t][i][0], pl[t][i][1]);
+          mma_16<true>(part, a0, a1, a2, a3, ph[t][i][0], ph[t][i][1]);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) d.o[j + u][i][r] = fmaf(part[r], 0x1p10f, d.o[j + u][i][r]);   // (2^120 of the bytes less 2^110)
+        }
+      }
+    }
+  }
+}
+
 // HEADS: query heads of a CTA, 8 or 16.
 template <int D, bool BF16, int HEADS, bool TMA>
 __global__ void __launch_bounds__(kThreads, Geo<D, HEADS>::kCtas)
@@ -521,22 +622,14 @@ __global__ void __launch_bounds__(kThreads, Geo<D, HEADS>::kCtas)
         }
         wide = BF16 && __any_sync(0xffffffffu, wide);
         if (wide) {
+          Wide<D, NB> d;
+          wide_query<D, NB>(d, &sync->query[st][0][0], g, tq);
 #pragma unroll
           for (int i = 0; i < NB; ++i) {
             const bool here = unit / p.Hkv * HEADS + 8 * i + g < p.group;
-            uint32_t top = 0;
-#pragma unroll 1
-            for (int e = 0; e < D; ++e) top = max(top, sync->query[st][8 * i + g][e] & 0x7fffu);
-            const int up = power_up<BF16>(top << 16, 126);
-            const float f = __int_as_float((127 + up) << 23);
-            if (here) factor[i] = p.scale * kLog2e * __int_as_float((127 - up) << 23) * 0x1p120f;
+            if (here) factor[i] = p.scale * kLog2e * d.factor[i];
 #pragma unroll
-            for (int s = 0; s < KS; ++s) {
-              const uint2 v = *reinterpret_cast<const uint2*>(&sync->query[st][8 * i + g][16 * s + 4 * tq]);
-              const uint32_t x = pack16<true>(half_to_f32<true>(static_cast<uint16_t>(v.x)) * f, half_to_f32<true>(static_cast<uint16_t>(v.x >> 16)) * f);
-              const uint32_t y = pack16<true>(half_to_f32<true>(static_cast<uint16_t>(v.y)) * f, half_to_f32<true>(static_cast<uint16_t>(v.y >> 16)) * f);
-              q[i][s] = here ? make_uint2(__byte_perm(x, y, 0x5410), __byte_perm(x, y, 0x7632)) : make_uint2(0u, 0u);   // (as unpack_key has them)
-            }
+            for (int s = 0; s < KS; ++s) q[i][s] = here ? d.q[i][s] : make_uint2(0u, 0u);
           }
         }
 #pragma unroll
@@ -606,21 +699,31 @@ __global__ void __launch_bounds__(kThreads, Geo<D, HEADS>::kCtas)
             for (int x = 0; x < kChains; ++x)
 #pragma unroll
               for (int r = 0; r < 4; ++r) part_s[t][i][x][r] = 0.f;
-        auto scores = [&](auto as_bf16) {
-          constexpr bool kBf16 = decltype(as_bf16)::value;
+        if (BF16 && wide) {
+          Wide<D, NB> d;
+#pragma unroll
+          for (int i = 0; i < NB; ++i)
+#pragma unroll
+            for (int s = 0; s < KS; ++s) d.q[i][s] = q[i][s];
+          wide_scores<D, NB>(d, k_row, lane);
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < NB; ++i)
+#pragma unroll
+              for (int r = 0; r < 4; ++r) part_s[t][i][0][r] = d.score[t][i][r];
+        } else {
 #pragma unroll
           for (int s = 0; s < KS; ++s)
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
               uint32_t a0, a1, a2, a3;
-              unpack_key<kBf16>(kf[t][s / 2][2 * (s & 1)], a0, a2);
-              unpack_key<kBf16>(kf[t][s / 2][2 * (s & 1) + 1], a1, a3);
+              unpack_e4m3_f16(kf[t][s / 2][2 * (s & 1)], a0, a2);
+              unpack_e4m3_f16(kf[t][s / 2][2 * (s & 1) + 1], a1, a3);
 #pragma unroll
-              for (int i = 0; i < NB; ++i) mma_16<kBf16>(part_s[t][i][s % kChains], a0, a1, a2, a3, q[i][s].x, q[i][s].y);
+              for (int i = 0; i < NB; ++i) mma_16<false>(part_s[t][i][s % kChains], a0, a1, a2, a3, q[i][s].x, q[i][s].y);
             }
-        };
-        if (BF16 && wide) scores(std::true_type{});
-        else scores(std::false_type{});
+        }
         float mn[NB][2];
         bool grow = e_top > r_exp;
 #pragma unroll
@@ -664,50 +767,88 @@ __global__ void __launch_bounds__(kThreads, Geo<D, HEADS>::kCtas)
               for (int r = 0; r < 4; ++r) o[j][i][r] *= f[r & 1];
           }
         }
-        // ---- probabilities; times the value scale relative to r, hi and lo, turned round: heads g x keys 2 tq, 2 tq + 1
-        uint32_t ph[2][NB][2], pl[2][NB][2];
+        // ---- probabilities; times the value scale relative to r, hi and lo, turned round: heads g x keys 2 tq, 2 tq + 1.  Then
+        // O^T += V^T P^T, sixteen columns of V at a time.
+        bool deep = false;
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          float w[2];
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) w[i] = ev[t][i] == -CUDART_INF_F ? 0.f : ex2(ev[t][i] - r_exp + kProbShift);
+          for (int i = 0; i < 2; ++i) deep |= ev[t][i] < r_exp - kDeep && ev[t][i] != -CUDART_INF_F;
+        if (__any_sync(0xffffffffu, deep)) {
+          Deep<D, NB> d;
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) d.w[t][i] = ev[t][i] == -CUDART_INF_F ? 0.f : ex2(ev[t][i] - r_exp + (kProbShift + kDeepShift));
 #pragma unroll
           for (int i = 0; i < NB; ++i) {
-            float x[4];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const float nm = (m[i][e] == -CUDART_INF_F) ? 0.f : -m[i][e];
-              x[e] = ex2(sv[t][i][e] + nm);
-              x[2 + e] = ex2(sv[t][i][2 + e] + nm);
-              lsum[i][e] += x[e] + x[2 + e];
+              d.nm[i][e] = (m[i][e] == -CUDART_INF_F) ? 0.f : -m[i][e];
+              d.lsum[i][e] = lsum[i][e];
             }
 #pragma unroll
-            for (int y = 0; y < 2; ++y) {
-              split_f16(x[2 * y] * w[y], x[2 * y + 1] * w[y], ph[t][i][y], pl[t][i][y]);
-              ph[t][i][y] = turn8x8(ph[t][i][y]);
-              pl[t][i][y] = turn8x8(pl[t][i][y]);
+            for (int r = 0; r < 4; ++r) {
+              d.sv[0][i][r] = sv[0][i][r];
+              d.sv[1][i][r] = sv[1][i][r];
+#pragma unroll
+              for (int j = 0; j < D / 16; ++j) d.o[j][i][r] = o[j][i][r];
             }
           }
-        }
-        // ---- O^T += V^T P^T, sixteen columns of V at a time
+          deep_products<D, NB>(d, v_row, lane);
 #pragma unroll
-        for (int j = 0; j < D / 16; j += 2)
+          for (int i = 0; i < NB; ++i) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) lsum[i][e] = d.lsum[i][e];
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+              for (int j = 0; j < D / 16; ++j) o[j][i][r] = d.o[j][i][r];
+          }
+        } else {
+          uint32_t ph[2][NB][2], pl[2][NB][2];
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
-            uint32_t vf[4];
-            ldsm_x4_trans(v_row + t * 16 * D + piece(j), vf);
+            float w[2];
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              uint32_t a0, a1, a2, a3;   // even and odd columns of keys 0-7, then of keys 8-15
-              unpack_e4m3_f16(__byte_perm(vf[2 * u], 0, 0x3120), a0, a1);
-              unpack_e4m3_f16(__byte_perm(vf[2 * u + 1], 0, 0x3120), a2, a3);
+            for (int i = 0; i < 2; ++i) w[i] = ev[t][i] == -CUDART_INF_F ? 0.f : ex2(ev[t][i] - r_exp + kProbShift);
 #pragma unroll
-              for (int i = 0; i < NB; ++i) {
-                mma_16<false>(o[j + u][i], a0, a1, a2, a3, ph[t][i][0], ph[t][i][1]);
-                mma_16<false>(o[j + u][i], a0, a1, a2, a3, pl[t][i][0], pl[t][i][1]);
+            for (int i = 0; i < NB; ++i) {
+              float x[4];
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const float nm = (m[i][e] == -CUDART_INF_F) ? 0.f : -m[i][e];
+                x[e] = ex2(sv[t][i][e] + nm);
+                x[2 + e] = ex2(sv[t][i][2 + e] + nm);
+                lsum[i][e] += x[e] + x[2 + e];
+              }
+#pragma unroll
+              for (int y = 0; y < 2; ++y) {
+                split_16<false>(x[2 * y] * w[y], x[2 * y + 1] * w[y], ph[t][i][y], pl[t][i][y]);
+                ph[t][i][y] = turn8x8(ph[t][i][y]);
+                pl[t][i][y] = turn8x8(pl[t][i][y]);
               }
             }
           }
+#pragma unroll
+          for (int j = 0; j < D / 16; j += 2)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              uint32_t vf[4];
+              ldsm_x4_trans(v_row + t * 16 * D + piece(j), vf);
+#pragma unroll
+              for (int u = 0; u < 2; ++u) {
+                uint32_t a0, a1, a2, a3;   // even and odd columns of keys 0-7, then of keys 8-15
+                unpack_e4m3_f16(__byte_perm(vf[2 * u], 0, 0x3120), a0, a1);
+                unpack_e4m3_f16(__byte_perm(vf[2 * u + 1], 0, 0x3120), a2, a3);
+#pragma unroll
+                for (int i = 0; i < NB; ++i) {
+                  mma_16<false>(o[j + u][i], a0, a1, a2, a3, ph[t][i][0], ph[t][i][1]);
+                  mma_16<false>(o[j + u][i], a0, a1, a2, a3, pl[t][i][0], pl[t][i][1]);
+                }
+              }
+            }
+        }
       }
       const int last = sync->block[st].last, next_unit = sync->block[st].next_unit, next_b = sync->block[st].next_b;
       const bool ends = blk + 1 == (n_keys + kBlockKeys - 1) / kBlockKeys;
