@@ -22,7 +22,7 @@
 //   * values: o += (p 2^(e_v - r + 9)) v8 with r the largest e_v the warp has met (o is rescaled when it grows), so the
 //     probability stays inside fp16; it enters as hi + lo, two fp16 operands: 22 bits, and never coarser than 2^-34 of
 //     the largest value row the warp has met.  That row may have no weight at all, so a warp's keys with a row 2^10 below it are
-//     multiplied in bf16, hi + lo: 16 bits at any size.
+//     multiplied in bf16, hi + lo: 16 bits at any size.  (Either bf16 product in every block: 64 x 512..8192 keys 240 us, not 120.)
 // One warp brings the rows into a ring of blocks by tensor copies, one for each page and operand, and another the scales; four
 // warps compute, 32 keys of a block each, and wait for nothing but their block.  (With plain copies and one barrier a block of 64
 // keys, as decode_mma.cu has them, the address arithmetic and the latency of table and scales stood in the way: 64 x 512..8192
